@@ -242,7 +242,7 @@ def _slots(table, lens, new, tokens, bs):
 
 def _plan(s):
     """Released requests push their blocks on the stack of free blocks; then each request, in order, pops what its new tokens need
-    beyond the blocks it has. Requests that do not fit any more get nothing. Lengths and the stack's height come back new."""
+    beyond the blocks it has. A request whose blocks do not fit any more gets nothing. Lengths and the stack's height come back new."""
     table, free, bs = s["table"], s["free"], s["bs"]
     lens, new, count = s["lens"].long(), s["new"].long(), s["count"].long()
     have = (lens + bs - 1) // bs
@@ -259,7 +259,7 @@ def _plan(s):
         lens, have, may = torch.where(s["released"], 0, lens), torch.where(s["released"], 0, have), ~s["released"]
     need = torch.where(may, (lens + new + bs - 1) // bs - have, 0)
     top = need.cumsum(0)
-    served = (new == 0) | (may & (top <= count))
+    served = (new == 0) | (may & ((need == 0) | (top <= count)))
     need, top = torch.where(served, need, 0), torch.where(served, top, 0)
     k = j - have[:, None]
     fresh = (k >= 0) & (k < need[:, None])
