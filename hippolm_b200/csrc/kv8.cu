@@ -1,0 +1,438 @@
+// 8-bit paged key / value cache: planning (block tables and slot maps) and the quantising write.
+//
+// Cache: codes [2][blocks][heads][bs][D] (int8 or e4m3; keys, then values), scales [2][blocks][heads] fp32 = 2^e. A value is
+// code * scale. With a power of two the scaled value is rounded exactly once (x * 2^-e is exact), and a block whose scale has to
+// grow by 2^k only shifts its older codes: exact in e4m3 above the subnormals, one more rounding in int8.
+// The reference has no cache (src/models/model.py:180-219 re-runs the forward for every token).
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include "sm100.cuh"
+#include "kv8_common.cuh"
+
+namespace hippo {
+
+// ------------------------------------------------------------------------------------------------ planning
+// One CTA of 1024 threads walks the requests 1024 at a time: a thread owns a request, prefix sums over the CTA give the
+// positions in the stack of free blocks, in the packed tokens, and decide who still fits. Released requests push first. The work
+// is a few dependent loads and five barriers (latency-bound); more CTAs would need a grid-wide order between pushes and pops.
+constexpr int kPlanThreads = 1024;
+
+__device__ __forceinline__ long long block_inclusive_scan(long long v, long long* warp_sum, long long& total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  long long x = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
+  }
+  if (lane == 31) warp_sum[w] = x;
+  __syncthreads();
+  if (w == 0) {
+    long long s = warp_sum[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d) s += y;
+    }
+    warp_sum[lane] = s;
+  }
+  __syncthreads();
+  total = warp_sum[31];
+  const long long before = w ? warp_sum[w - 1] : 0;
+  __syncthreads();                                   // warp_sum is free for the next scan
+  return x + before;
+}
+
+// slot of the token at position `pos` of a request whose table row is `row`; -1 where the row holds no block there
+__device__ __forceinline__ long long slot_of(const int* row, int pos, int sh) {
+  const int b = row[pos >> sh];
+  return b < 0 ? -1ll : ((long long)b << sh) + (pos & ((1 << sh) - 1));
+}
+
+__global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(
+    int* table, long long table_ld, int M, const int* __restrict__ lens, const int* __restrict__ new_lens, int N,
+    int* free_list, int cap, const int* __restrict__ free_count, const unsigned char* __restrict__ release, int sh,
+    long long num_tokens, long long* __restrict__ slots, int* __restrict__ lens_out, int* __restrict__ count_out,
+    unsigned char* __restrict__ served, int* __restrict__ cu, int write_slots) {
+  __shared__ long long warp_sum[32];
+  __shared__ int s_end[kPlanThreads], s_pos[kPlanThreads];      // packed end of a request's tokens, position of its first one
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int bs1 = (1 << sh) - 1;
+  const long long room = (long long)M << sh;
+  long long count = min(max(*free_count, 0), cap), total;
+
+  if (release) {
+    for (int base = 0; base < N; base += kPlanThreads) {
+      const int n = base + tid;
+      int back = 0;
+      if (n < N && release[n]) back = (int)((min((long long)max(lens[n], 0), room) + bs1) >> sh);
+      const long long at = count + block_inclusive_scan(back, warp_sum, total) - back;
+      for (unsigned todo = __ballot_sync(0xffffffffu, back > 0); todo; todo &= todo - 1) {
+        const int src = __ffs(todo) - 1;
+        const int cnt = __shfl_sync(0xffffffffu, back, src);
+        const long long a = __shfl_sync(0xffffffffu, at, src);
+        const int* row = table + (long long)(n - lane + src) * table_ld;
+        for (int j = lane; j < cnt; j += 32)
+          if (a + j < cap) free_list[a + j] = row[j];
+      }
+      count = min(count + total, (long long)cap);
+    }
+    __syncthreads();                                 // pushes are visible to the pops of every thread
+  }
+
+  long long tokens = 0, asked = 0, used = 0;         // packed tokens, blocks asked for, blocks handed out so far
+  for (int base = 0; base < N; base += kPlanThreads) {
+    const int n = base + tid;
+    const bool in = n < N, gone = in && release && release[n];
+    long long len = in && !gone ? min((long long)max(lens[n], 0), room) : 0;
+    const int want = in ? max(new_lens[n], 0) : 0;
+    const long long end = tokens + block_inclusive_scan(want, warp_sum, total);
+    const long long chunk_begin = tokens;
+    tokens += total;
+    const bool fits = in && !gone && len + want <= room && end <= num_tokens;
+    const int have = (int)((len + bs1) >> sh);
+    int need = fits ? (int)((len + want + bs1) >> sh) - have : 0;
+    const long long top = asked + block_inclusive_scan(need, warp_sum, total);
+    asked += total;
+    const bool ok = want == 0 || (fits && (need == 0 || top <= count));
+    const long long at = count - 1 - (top - need);   // first pop; the rows that get blocks are a prefix of those that ask
+    if (!ok) need = 0;
+    if (need == 1) table[(long long)n * table_ld + have] = free_list[at];
+    for (unsigned todo = __ballot_sync(0xffffffffu, need > 1); todo; todo &= todo - 1) {
+      const int src = __ffs(todo) - 1;
+      const int cnt = __shfl_sync(0xffffffffu, need, src), h0 = __shfl_sync(0xffffffffu, have, src);
+      const long long a = __shfl_sync(0xffffffffu, at, src);
+      int* row = table + (long long)(n - lane + src) * table_ld;
+      for (int j = lane; j < cnt; j += 32) row[h0 + j] = free_list[a - j];
+    }
+    block_inclusive_scan(need, warp_sum, total);
+    used += total;
+    if (in) {
+      lens_out[n] = (int)(ok ? len + want : len);
+      served[n] = ok;
+      cu[n + 1] = (int)min(end, (long long)0x7fffffff);
+    }
+    if (write_slots) {
+      s_end[tid] = (int)min(end, num_tokens);
+      s_pos[tid] = ok ? (int)len : -1;
+      __syncthreads();
+      const long long last = min(tokens, num_tokens);
+      for (long long t = chunk_begin + tid; t < last; t += kPlanThreads) {
+        int lo = 0, hi = kPlanThreads - 1;           // first request of the chunk whose tokens end behind t
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (s_end[mid] > t) hi = mid; else lo = mid + 1;
+        }
+        const int first = lo ? s_end[lo - 1] : (int)chunk_begin;
+        long long slot = -1;
+        if (s_pos[lo] >= 0 && base + lo < N)
+          slot = slot_of(table + (long long)(base + lo) * table_ld, s_pos[lo] + (int)t - first, sh);
+        slots[t] = slot;
+      }
+      __syncthreads();
+    }
+  }
+  if (write_slots)
+    for (long long t = min(tokens, num_tokens) + tid; t < num_tokens; t += kPlanThreads) slots[t] = -1;
+  if (tid == 0) { cu[0] = 0; *count_out = (int)(count - used); }
+}
+
+// Slot map of many tokens (prompts): 4 tokens a thread, the request of the first found in the packed ends, the table rows stay in
+// L1. Runs behind the planning kernel, whose single CTA would write 8 bytes a token at one SM's rate.
+__global__ void __launch_bounds__(256) kv8_slots_kernel(
+    const int* __restrict__ table, long long table_ld, const int* __restrict__ lens_out, const unsigned char* __restrict__ served,
+    const int* __restrict__ cu, int N, int sh, long long num_tokens, long long* __restrict__ slots) {
+  const long long t0 = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (t0 >= num_tokens) return;
+  int lo = 0, hi = N;                                // first n with cu[n + 1] > t0, N behind the last token
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid + 1] > t0) hi = mid; else lo = mid + 1;
+  }
+  int n = lo;
+  for (int i = 0; i < 4 && t0 + i < num_tokens; ++i) {
+    const long long t = t0 + i;
+    while (n < N && cu[n + 1] <= t) ++n;
+    long long slot = -1;
+    if (n < N && served[n])                          // lens_out counts the new tokens: the last one is at lens_out - 1
+      slot = slot_of(table + (long long)n * table_ld, lens_out[n] - (int)(cu[n + 1] - t), sh);
+    slots[t] = slot;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ write
+template <typename T> struct Row8;                   // 8 consecutive values as they are loaded, and as fp32
+template <> struct Row8<float> {
+  float4 a, b;
+  __device__ void load(const float* p) { a = __ldg((const float4*)p); b = __ldg((const float4*)p + 1); }
+  __device__ void zero() { a = b = make_float4(0, 0, 0, 0); }
+  __device__ void get(float* f) const { f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w; }
+};
+template <> struct Row8<__nv_bfloat16> {
+  uint4 a;
+  __device__ void load(const __nv_bfloat16* p) { a = __ldg((const uint4*)p); }
+  __device__ void zero() { a = make_uint4(0, 0, 0, 0); }
+  __device__ void get(float* f) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+};
+template <> struct Row8<__half> {
+  uint4 a;
+  __device__ void load(const __half* p) { a = __ldg((const uint4*)p); }
+  __device__ void zero() { a = make_uint4(0, 0, 0, 0); }
+  __device__ void get(float* f) const {
+    const __half2* h = (const __half2*)&a;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float2 v = __half22float2(h[i]); f[2 * i] = v.x; f[2 * i + 1] = v.y; }
+  }
+};
+
+// largest |x| of the 8 values as bits (integer order keeps infinities and NaN on top)
+template <typename R> __device__ __forceinline__ uint32_t amax_bits(const R& r, uint32_t m) {
+  float f[8];
+  r.get(f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+  return m;
+}
+
+// What a run of new tokens does to its (block, head): the exponent of the scale, how far older codes shift, poison.
+struct RunScale { int e, down; bool bad; };
+template <int E4M3> __device__ __forceinline__ RunScale run_scale(uint32_t amax, float old_scale, bool holds) {
+  RunScale r;
+  r.bad = amax >= 0x7f800000u || (holds && isnan_bits(old_scale));
+  r.e = scale_exponent<E4M3>(r.bad ? 0u : amax);
+  r.down = 0;
+  if (holds && !r.bad) {
+    const int old = max((int)((__float_as_uint(old_scale) >> 23) & 255) - 127, kMinExp);
+    r.e = max(r.e, old);
+    r.down = old - r.e;
+  }
+  return r;
+}
+
+// older codes of the block shift by 2^down (threads `i` of `step` take 16 bytes each)
+template <int E4M3> __device__ __forceinline__ void shift_codes(uint8_t* codes, int bytes, int down, int i, int step) {
+  const float f = pow2f(max(down, -126));
+  for (int o = i * 16; o < bytes; o += step * 16) {
+    uint4 w = *(uint4*)(codes + o);
+    uint8_t* c = (uint8_t*)&w;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) c[j] = encode1<E4M3>(decode1<E4M3>(c[j]) * f);
+    *(uint4*)(codes + o) = w;
+  }
+}
+
+template <int E4M3, typename R> __device__ __forceinline__ uint2 encode_row(const R& r, float inv, bool bad) {
+  float f[8];
+  r.get(f);
+  uint2 o;
+  uint8_t* c = (uint8_t*)&o;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = bad ? 0 : encode1<E4M3>(f[i] * inv);
+  return o;
+}
+
+struct WriteArgs {
+  const void *k, *v;
+  long long k_t, k_h, v_t, v_h;                      // strides in elements
+  const long long* slots;
+  long long T, limit;                                // tokens, blocks * bs
+  uint8_t* codes;
+  float* scales;
+  int H, sh;
+  long long half_codes, half_scales;                 // elements of the key half
+};
+
+__device__ __forceinline__ bool slot_ok(const WriteArgs& a, long long s) { return s >= 0 && s < a.limit; }
+// token t continues the run of token t - 1: the next slot of the same block
+__device__ __forceinline__ bool continues(const WriteArgs& a, long long prev, long long s) {
+  return slot_ok(a, prev) && s == prev + 1 && (s & ((1 << a.sh) - 1)) != 0;
+}
+
+// One warp for a (run of tokens in a block, head, half): the form for few tokens (decoding), where every token is a run of its own.
+// Warps whose token is not the first of a run leave at once.
+template <typename T, int D, int E4M3>
+__global__ void __launch_bounds__(256) kv8_write_rows_kernel(WriteArgs a) {
+  constexpr int LPR = D / 8, RPW = 32 / LPR;         // lanes a row, rows of a warp's load
+  const int lane = threadIdx.x & 31;
+  const long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int half = blockIdx.y;
+  const long long t = u / a.H;
+  const int h = (int)(u - t * a.H);
+  if (t >= a.T) return;
+  const long long s = a.slots[t];
+  if (!slot_ok(a, s) || (t > 0 && continues(a, a.slots[t - 1], s))) return;
+  const int bs = 1 << a.sh, off = (int)(s & (bs - 1));
+  const T* x = (const T*)(half ? a.v : a.k) + t * (half ? a.v_t : a.k_t) + h * (half ? a.v_h : a.k_h);
+  const long long ld = half ? a.v_t : a.k_t;
+  const int r0 = lane / LPR, col = (lane % LPR) * 8;
+  const long long bh = (s >> a.sh) * a.H + h;
+  float* scale = a.scales + half * a.half_scales + bh;
+  uint8_t* codes = a.codes + half * a.half_codes + (bh << a.sh) * D;
+  // length of the run
+  int L = 1;
+  for (int base = 1; base < bs - off; base += 32) {
+    const long long i = base + lane;
+    const bool go = off + i < bs && t + i < a.T && a.slots[t + i] == s + i;
+    const unsigned m = __ballot_sync(0xffffffffu, go);
+    if (m != 0xffffffffu) { L = base + __ffs(~m) - 1; break; }
+    L = base + 32;
+  }
+  const float old = off ? *scale : 0.f;
+  constexpr int U = 4;
+  Row8<T> keep[U];                                   // the first U * RPW rows stay in registers between the two passes
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int r = r0 + i * RPW;
+    if (r < L) keep[i].load(x + r * ld + col); else keep[i].zero();
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) m = amax_bits(keep[i], m);
+  for (int r = r0 + U * RPW; r < L; r += RPW) {
+    Row8<T> row;
+    row.load(x + r * ld + col);
+    m = amax_bits(row, m);
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  const RunScale rs = run_scale<E4M3>(m, old, off > 0);
+  if (rs.down < 0) shift_codes<E4M3>(codes, off * D, rs.down, lane, 32);
+  const float inv = pow2f(-rs.e);
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int r = r0 + i * RPW;
+    if (r < L) *(uint2*)(codes + (off + r) * D + col) = encode_row<E4M3>(keep[i], inv, rs.bad);
+  }
+  for (int r = r0 + U * RPW; r < L; r += RPW) {
+    Row8<T> row;
+    row.load(x + r * ld + col);
+    *(uint2*)(codes + (off + r) * D + col) = encode_row<E4M3>(row, inv, rs.bad);
+  }
+  if (lane == 0) *scale = rs.bad ? __uint_as_float(0x7fffffffu) : pow2f(rs.e);
+}
+
+// One CTA for the runs that start in a window of bs tokens, of one head and half: the form for prompts. A run (at most bs rows) is
+// read once into registers, reduced over the CTA and stored: HBM-bound, bytes = T * H * D * (element + 1) a half.
+template <typename T, int D, int E4M3, int BS>
+__global__ void __launch_bounds__(128) kv8_write_blocks_kernel(WriteArgs a) {
+  constexpr int LPR = D / 8, RPP = 128 / LPR, P = (BS + RPP - 1) / RPP;   // lanes a row, rows a pass, passes
+  __shared__ unsigned s_cont[4];                     // bit i: token w0 + i continues the run of the token before it
+  __shared__ unsigned s_ok[4];
+  __shared__ uint32_t s_max[4];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const int h = blockIdx.y >> 1, half = blockIdx.y & 1;
+  const long long w0 = (long long)blockIdx.x * BS;
+  bool ok = false, cont = false;
+  if (tid < 2 * BS && w0 + tid < a.T) {
+    const long long s = a.slots[w0 + tid];
+    ok = slot_ok(a, s);
+    cont = ok && w0 + tid > 0 && continues(a, a.slots[w0 + tid - 1], s);
+  }
+  const unsigned bc = __ballot_sync(0xffffffffu, cont), bo = __ballot_sync(0xffffffffu, ok);
+  if (lane == 0) { s_cont[w] = bc; s_ok[w] = bo; }
+  __syncthreads();
+  const unsigned long long c0 = s_cont[0] | ((unsigned long long)s_cont[1] << 32), c1 = s_cont[2] | ((unsigned long long)s_cont[3] << 32);
+  unsigned long long heads = (s_ok[0] | ((unsigned long long)s_ok[1] << 32)) & ~c0;
+  if (BS < 64) heads &= (1ull << (BS & 63)) - 1;
+  const int r0 = tid / LPR, col = (tid % LPR) * 8;
+  const T* base = (const T*)(half ? a.v : a.k) + h * (half ? a.v_h : a.k_h) + col;
+  const long long ld = half ? a.v_t : a.k_t;
+  for (; heads; heads &= heads - 1) {
+    const int i0 = __ffsll(heads) - 1;
+    // consecutive "continues" bits behind i0
+    const unsigned long long rest = i0 == 63 ? c1 : (c0 >> (i0 + 1)) | (c1 << (63 - i0));
+    const int L = min(~rest ? __ffsll(~rest) : 64, BS);
+    const long long t = w0 + i0, s = a.slots[t];
+    const int off = (int)(s & (BS - 1));
+    const long long bh = (s >> a.sh) * a.H + h;
+    float* scale = a.scales + half * a.half_scales + bh;
+    uint8_t* codes = a.codes + half * a.half_codes + bh * BS * D;
+    const float old = off ? *scale : 0.f;
+    Row8<T> row[P];
+    uint32_t m = 0;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int r = r0 + p * RPP;
+      if (r < L) row[p].load(base + (t + r) * ld); else row[p].zero();
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) m = amax_bits(row[p], m);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) s_max[w] = m;
+    __syncthreads();                                 // also: every thread has read the old scale
+    m = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+    const RunScale rs = run_scale<E4M3>(m, old, off > 0);
+    if (rs.down < 0) shift_codes<E4M3>(codes, off * D, rs.down, tid, 128);
+    const float inv = pow2f(-rs.e);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int r = r0 + p * RPP;
+      if (r < L) *(uint2*)(codes + (off + r) * D + col) = encode_row<E4M3>(row[p], inv, rs.bad);
+    }
+    if (tid == 0) *scale = rs.bad ? __uint_as_float(0x7fffffffu) : pow2f(rs.e);
+    __syncthreads();                                 // s_max is free for the next run
+  }
+}
+
+// The rows form wins while a token is a run of its own or there are few of them; a prompt's warps mostly leave at once there.
+constexpr long long kRowsMaxTokens = 2048;
+
+template <typename T, int D, int E4M3> int launch_write(const WriteArgs& a, int form, cudaStream_t st) {
+  const bool rows = form == 1 || (form == 0 && a.T <= kRowsMaxTokens);
+  if (rows) {
+    const long long g = (a.T * a.H + 7) / 8;
+    if (g > 0x7fffffffll) return -2;
+    kv8_write_rows_kernel<T, D, E4M3><<<dim3((unsigned)g, 2), 256, 0, st>>>(a);
+    return (int)cudaGetLastError();
+  }
+  const dim3 grid((unsigned)((a.T + (1 << a.sh) - 1) >> a.sh), (unsigned)(2 * a.H));
+  if (a.sh == 4) kv8_write_blocks_kernel<T, D, E4M3, 16><<<grid, 128, 0, st>>>(a);
+  else if (a.sh == 5) kv8_write_blocks_kernel<T, D, E4M3, 32><<<grid, 128, 0, st>>>(a);
+  else kv8_write_blocks_kernel<T, D, E4M3, 64><<<grid, 128, 0, st>>>(a);
+  return (int)cudaGetLastError();
+}
+template <typename T> int dispatch_write(const WriteArgs& a, int D, int e4m3, int form, cudaStream_t st) {
+  if (D == 128) return e4m3 ? launch_write<T, 128, 1>(a, form, st) : launch_write<T, 128, 0>(a, form, st);
+  if (D == 64) return e4m3 ? launch_write<T, 64, 1>(a, form, st) : launch_write<T, 64, 0>(a, form, st);
+  return -1;
+}
+}  // namespace hippo
+
+using namespace hippo;
+
+// table [N][M] int32 (row pitch table_ld), lens / new_lens [N], free_list [cap], free_count [1], release [N] or null; out: slots
+// [num_tokens], lens_out [N], count_out [1], served [N], cu [N + 1].
+extern "C" int hippo_kv8_plan(int* table, long long table_ld, int M, const int* lens, const int* new_lens, int N, int* free_list,
+                              int cap, const int* free_count, const unsigned char* release, int block_size, long long num_tokens,
+                              long long* slots, int* lens_out, int* count_out, unsigned char* served, int* cu, void* stream) {
+  const int sh = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : -1;
+  if (sh < 0 || N < 1 || M < 1 || cap < 1 || num_tokens < 0 || num_tokens > 0x7fffffffll) return -1;
+  const bool many = num_tokens > 16384;
+  kv8_plan_kernel<<<1, kPlanThreads, 0, (cudaStream_t)stream>>>(table, table_ld, M, lens, new_lens, N, free_list, cap, free_count,
+                                                                release, sh, num_tokens, slots, lens_out, count_out, served, cu,
+                                                                many ? 0 : 1);
+  if (many)
+    kv8_slots_kernel<<<(unsigned)((num_tokens + 1023) / 1024), 256, 0, (cudaStream_t)stream>>>(table, table_ld, lens_out, served,
+                                                                                               cu, N, sh, num_tokens, slots);
+  return (int)cudaGetLastError();
+}
+
+// k / v: [T][H][D] with strides (elements); dtype 0 bf16, 1 fp16, 2 fp32; codes / scales of `blocks` blocks; form 0 = by size,
+// 1 = a warp a run, 2 = a CTA a window of block_size tokens.
+extern "C" int hippo_kv8_write(const void* k, const void* v, int dtype, long long k_t, long long k_h, long long v_t, long long v_h,
+                               const long long* slots, long long T, int H, int D, int block_size, long long blocks, int e4m3,
+                               void* codes, float* scales, int form, void* stream) {
+  if (T <= 0) return 0;
+  const int sh = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : -1;
+  if (sh < 0 || H < 1 || 2 * H > 65535 || blocks < 1 || T > 0x7fffffffll) return -1;
+  WriteArgs a{k, v, k_t, k_h, v_t, v_h, slots, T, blocks << sh, (uint8_t*)codes, scales, H, sh,
+              ((blocks * H) << sh) * D, blocks * H};
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == 0) return dispatch_write<__nv_bfloat16>(a, D, e4m3, form, st);
+  if (dtype == 1) return dispatch_write<__half>(a, D, e4m3, form, st);
+  if (dtype == 2) return dispatch_write<float>(a, D, e4m3, form, st);
+  return -1;
+}

@@ -11,3 +11,5 @@ from .functional import (  # noqa: F401
     nvfp4_quantize, nvfp4_dequantize, nvfp4_linear, newton_schulz5, adamw_update,
     lce_chunk_stats, lce_chunk_grad, gemm_tn_accumulate, cuda_ext_loaded,
 )
+from .kv8 import KV8Plan, attention_decode_kv8, kv8_empty, kv8_plan, kv8_write  # noqa: F401
+from .logprob import TokenLogprobs, token_logprobs  # noqa: F401
