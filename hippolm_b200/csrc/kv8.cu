@@ -403,36 +403,46 @@ template <typename T> int dispatch_write(const WriteArgs& a, int D, int e4m3, in
 
 using namespace hippo;
 
+// Arguments come as one block (a packed struct costs the caller a fifth of converting twenty arguments one by one).
+
 // table [N][M] int32 (row pitch table_ld), lens / new_lens [N], free_list [cap], free_count [1], release [N] or null; out: slots
 // [num_tokens], lens_out [N], count_out [1], served [N], cu [N + 1].
-extern "C" int hippo_kv8_plan(int* table, long long table_ld, int M, const int* lens, const int* new_lens, int N, int* free_list,
-                              int cap, const int* free_count, const unsigned char* release, int block_size, long long num_tokens,
-                              long long* slots, int* lens_out, int* count_out, unsigned char* served, int* cu, void* stream) {
-  const int sh = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : -1;
-  if (sh < 0 || N < 1 || M < 1 || cap < 1 || num_tokens < 0 || num_tokens > 0x7fffffffll) return -1;
-  const bool many = num_tokens > 16384;
-  kv8_plan_kernel<<<1, kPlanThreads, 0, (cudaStream_t)stream>>>(table, table_ld, M, lens, new_lens, N, free_list, cap, free_count,
-                                                                release, sh, num_tokens, slots, lens_out, count_out, served, cu,
-                                                                many ? 0 : 1);
+struct KvPlanCall {
+  int* table; const int *lens, *new_lens; int* free_list; const int* free_count; const unsigned char* release;
+  long long* slots; int *lens_out, *count_out; unsigned char* served; int* cu; void* stream;
+  long long table_ld, num_tokens;
+  int M, N, cap, block_size;
+};
+extern "C" int hippo_kv8_plan(const KvPlanCall* c) {
+  const int sh = c->block_size == 16 ? 4 : c->block_size == 32 ? 5 : c->block_size == 64 ? 6 : -1;
+  if (sh < 0 || c->N < 1 || c->M < 1 || c->cap < 1 || c->num_tokens < 0 || c->num_tokens > 0x7fffffffll) return -1;
+  const bool many = c->num_tokens > 16384;
+  cudaStream_t st = (cudaStream_t)c->stream;
+  kv8_plan_kernel<<<1, kPlanThreads, 0, st>>>(c->table, c->table_ld, c->M, c->lens, c->new_lens, c->N, c->free_list, c->cap,
+                                              c->free_count, c->release, sh, c->num_tokens, c->slots, c->lens_out, c->count_out,
+                                              c->served, c->cu, many ? 0 : 1);
   if (many)
-    kv8_slots_kernel<<<(unsigned)((num_tokens + 1023) / 1024), 256, 0, (cudaStream_t)stream>>>(table, table_ld, lens_out, served,
-                                                                                               cu, N, sh, num_tokens, slots);
+    kv8_slots_kernel<<<(unsigned)((c->num_tokens + 1023) / 1024), 256, 0, st>>>(c->table, c->table_ld, c->lens_out, c->served,
+                                                                                c->cu, c->N, sh, c->num_tokens, c->slots);
   return (int)cudaGetLastError();
 }
 
 // k / v: [T][H][D] with strides (elements); dtype 0 bf16, 1 fp16, 2 fp32; codes / scales of `blocks` blocks; form 0 = by size,
 // 1 = a warp a run, 2 = a CTA a window of block_size tokens.
-extern "C" int hippo_kv8_write(const void* k, const void* v, int dtype, long long k_t, long long k_h, long long v_t, long long v_h,
-                               const long long* slots, long long T, int H, int D, int block_size, long long blocks, int e4m3,
-                               void* codes, float* scales, int form, void* stream) {
-  if (T <= 0) return 0;
-  const int sh = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : -1;
-  if (sh < 0 || H < 1 || 2 * H > 65535 || blocks < 1 || T > 0x7fffffffll) return -1;
-  WriteArgs a{k, v, k_t, k_h, v_t, v_h, slots, T, blocks << sh, (uint8_t*)codes, scales, H, sh,
-              ((blocks * H) << sh) * D, blocks * H};
-  cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == 0) return dispatch_write<__nv_bfloat16>(a, D, e4m3, form, st);
-  if (dtype == 1) return dispatch_write<__half>(a, D, e4m3, form, st);
-  if (dtype == 2) return dispatch_write<float>(a, D, e4m3, form, st);
+struct KvWriteCall {
+  const void *k, *v; const long long* slots; void* codes; float* scales; void* stream;
+  long long k_t, k_h, v_t, v_h, T, blocks;
+  int H, D, block_size, dtype, e4m3, form;
+};
+extern "C" int hippo_kv8_write(const KvWriteCall* c) {
+  if (c->T <= 0) return 0;
+  const int sh = c->block_size == 16 ? 4 : c->block_size == 32 ? 5 : c->block_size == 64 ? 6 : -1;
+  if (sh < 0 || c->H < 1 || 2 * c->H > 65535 || c->blocks < 1 || c->T > 0x7fffffffll) return -1;
+  WriteArgs a{c->k, c->v, c->k_t, c->k_h, c->v_t, c->v_h, c->slots, c->T, c->blocks << sh, (uint8_t*)c->codes, c->scales, c->H, sh,
+              ((c->blocks * c->H) << sh) * c->D, c->blocks * c->H};
+  cudaStream_t st = (cudaStream_t)c->stream;
+  if (c->dtype == 0) return dispatch_write<__nv_bfloat16>(a, c->D, c->e4m3, c->form, st);
+  if (c->dtype == 1) return dispatch_write<__half>(a, c->D, c->e4m3, c->form, st);
+  if (c->dtype == 2) return dispatch_write<float>(a, c->D, c->e4m3, c->form, st);
   return -1;
 }

@@ -448,40 +448,40 @@ template <int D, int E4M3> int launch_kv8_attention(const KvAttnArgs& a, const C
 
 using namespace hippo;
 
-// Workers (warps) of a launch over `tiles` tiles at most: the caller sizes the workspace with it.
-extern "C" int hippo_kv8_attention_workers(long long tiles) {
-  const long long ctas = (tiles + kWarps - 1) / kWarps, most = 3ll * sm_count();
-  return (int)(ctas < 1 ? 1 : ctas < most ? ctas : most) * kWarps;
-}
-
 // q [N][Hq][D] (strides in elements), out [N][Hq][D], codes [2][blocks][H][bs][D], scales [2][blocks][H], table [N][M] (pitch
-// table_ld); dtype 0 bf16, 1 fp16, 2 fp32. ws: workers * 2 * min(Hq / H, 8) * (D + 2)
-// floats, then workers * 4 ints, 16-byte aligned.
-extern "C" int hippo_kv8_attention(const void* q, int dtype, long long q_n, long long q_h, void* out, const void* codes,
-                                   const float* scales, int e4m3, long long blocks, int H, int Hq, int D, int block_size,
-                                   const int* table, long long table_ld, int M, const int* lens, int N, float scale, int workers,
-                                   float* ws, void* stream) {
-  const int sh = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : -1;
-  if (sh < 0 || N < 1 || M < 1 || H < 1 || Hq % H || blocks < 1 || workers < kWarps || workers % kWarps || dtype < 0 || dtype > 2)
+// table_ld); dtype 0 bf16, 1 fp16, 2 fp32. workers: warps of the launch, a multiple of 4; ws: workers * 2 * min(Hq / H, 8) * (D + 2)
+// floats, then workers * 4 ints, 16-byte aligned. One block of arguments, as in kv8.cu.
+struct KvAttendCall {
+  const void* q; void* out; const void* codes; const float* scales; const int *table, *lens; float* ws; void* stream;
+  long long q_n, q_h, table_ld, blocks;
+  int N, H, Hq, D, block_size, M, dtype, e4m3, workers;
+  float scale;
+};
+extern "C" int hippo_kv8_attention(const KvAttendCall* c) {
+  const int sh = c->block_size == 16 ? 4 : c->block_size == 32 ? 5 : c->block_size == 64 ? 6 : -1;
+  if (sh < 0 || c->N < 1 || c->M < 1 || c->H < 1 || c->Hq % c->H || c->blocks < 1 || c->workers < kWarps || c->workers % kWarps ||
+      c->dtype < 0 || c->dtype > 2 || (c->D != 64 && c->D != 128))
     return -1;
-  const long long half_rows = (blocks * H) << sh;
+  const int D = c->D;
+  const long long half_rows = (c->blocks * c->H) << sh;
   if (2 * half_rows > 0x7fffffffll) return -2;       // TMA coordinates are 32-bit
   auto fn = get_encode_fn();
   if (!fn) return -100;
   CUtensorMap map;
-  const int box = block_size < kTile ? block_size : kTile;
+  const int box = c->block_size < kTile ? c->block_size : kTile;
   const cuuint64_t dim[2] = {(cuuint64_t)D, (cuuint64_t)(2 * half_rows)}, pitch[1] = {(cuuint64_t)D};
   const cuuint32_t bx[2] = {(cuuint32_t)D, (cuuint32_t)box}, one[2] = {1, 1};
-  const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dim, pitch, bx, one,
+  const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(c->codes), dim, pitch, bx, one,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return -102 - (int)r;
-  const int G = Hq / H, rows = G < 8 ? G : 8;
-  KvAttnArgs a{q, out, q_n, q_h, scales, blocks * H, table, table_ld, M, lens, N, H, G, (G + 7) / 8, sh, (int)blocks, dtype,
-               half_rows, scale, ws, ws + (long long)workers * 2 * rows * D, (int4*)(ws + (long long)workers * 2 * rows * (D + 2)), workers, rows};
-  cudaStream_t st = (cudaStream_t)stream;
-  const int grid = workers / kWarps;
-  if (D == 128) return e4m3 ? launch_kv8_attention<128, 1>(a, map, grid, st) : launch_kv8_attention<128, 0>(a, map, grid, st);
-  if (D == 64) return e4m3 ? launch_kv8_attention<64, 1>(a, map, grid, st) : launch_kv8_attention<64, 0>(a, map, grid, st);
-  return -1;
+  const int G = c->Hq / c->H, rows = G < 8 ? G : 8;
+  const long long parts = 2ll * c->workers * rows;
+  KvAttnArgs a{c->q, c->out, c->q_n, c->q_h, c->scales, c->blocks * c->H, c->table, c->table_ld, c->M, c->lens, c->N, c->H, G,
+               (G + 7) / 8, sh, (int)c->blocks, c->dtype, half_rows, c->scale, c->ws, c->ws + parts * D,
+               (int4*)(c->ws + parts * (D + 2)), c->workers, rows};
+  cudaStream_t st = (cudaStream_t)c->stream;
+  const int grid = c->workers / kWarps;
+  if (D == 128) return c->e4m3 ? launch_kv8_attention<128, 1>(a, map, grid, st) : launch_kv8_attention<128, 0>(a, map, grid, st);
+  return c->e4m3 ? launch_kv8_attention<64, 1>(a, map, grid, st) : launch_kv8_attention<64, 0>(a, map, grid, st);
 }

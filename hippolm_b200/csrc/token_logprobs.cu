@@ -3,10 +3,13 @@
 //   l = sum e^(z - m),  logprob = (z_y - m) - log l,  entropy = log l - sum (z - m) e^(z - m) / l      (m: the row's maximum)
 //   dz_v = g_lp (1[v = y] - p_v) - g_H p_v (log p_v + H)
 //
-// Forward is one pass over the logits: a warp takes segments of 512 consecutive logits, every lane carries its own (m, l, sum) and
-// rescales them when a segment brings a larger maximum; the maximum of each segment is kept. The k largest logits lie in the k
-// segments that come first by (maximum, lowest index), so only those are read again (from L2). Bound by HBM for many rows; for few
-// rows a cluster of up to 8 CTAs shares a row and joins its parts through distributed shared memory.
+// Forward is one pass over the logits: a warp takes segments of 512 consecutive logits, the next one in flight while it works; every
+// lane carries its own (m, l, sum) and rescales them when a segment brings a larger maximum. Besides HBM the exponentials are the
+// bound (one a logit: 11.6 of the 16 a clock that a multiprocessor has, at the card's copy rate in 16 bits), so the rest is kept to
+// four instructions a logit: maximum and clamp on packed pairs, sums and products as fp32 pairs. For the alternatives the maximum
+// of every granule (8, 64 or 512 consecutive logits, by the vocabulary) is kept: the k largest logits lie in the k granules that
+// come first by (maximum, lowest index), so only those are read again (from L2). With few rows a cluster of up to 8 CTAs shares a
+// row and joins its parts through distributed shared memory.
 // The backward pass reads the logits once more and writes their gradient: HBM-bound.
 // The reference computes losses only (fla/modules/fused_linear_cross_entropy.py:516-679); it has no per-token scores.
 #include <cooperative_groups.h>
@@ -18,40 +21,102 @@
 namespace cg = cooperative_groups;
 
 namespace hippo {
-constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kSeg = 512, kPerLane = kSeg / 32;
-constexpr int kMaxSegs = 1024, kCand = 1024, kMaxTop = 32;
+constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kSeg = 512;
+constexpr int kMaxGranules = 1024, kCand = 1024, kMaxTop = 32;
 constexpr float kL2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float lp_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float lp_lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
+// two fp32 in one register pair
+__device__ __forceinline__ uint64_t pack(float a, float b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void unpack(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) { uint64_t r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+
 // Order of the values as signed integers; -0 counts as 0, every NaN as the largest.
 __device__ __forceinline__ int order_key(float x) {
   const int b = __float_as_int(x + 0.f);
-  if ((b & 0x7fffffff) > 0x7f800000) return 0x7fffffff;
+  if ((b & 0x7fffffff) > 0x7f800000) return 0x7fffffff;               // (-inf is far above the smallest integer)
   return b < 0 ? b ^ 0x7fffffff : b;
 }
 
-// 8 consecutive logits
-__device__ __forceinline__ void load8(const float* p, float* f) {
-  const float4 a = __ldg((const float4*)p), b = __ldg((const float4*)p + 1);
-  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* f) {
-  const uint4 a = __ldg((const uint4*)p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-}
-__device__ __forceinline__ void load8(const __half* p, float* f) {
-  const uint4 a = __ldg((const uint4*)p);
-  const __half2* h = (const __half2*)&a;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { const float2 v = __half22float2(h[i]); f[2 * i] = v.x; f[2 * i + 1] = v.y; }
-}
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+
+// 8 consecutive logits as they are loaded. max(): the largest, NaN if there is one. clamp(lo): what is below lo (far below the
+// maximum: its exponential is 0) or NaN becomes lo. kLow: maxima above it leave room for such a lo.
+template <typename T> struct Vec8;
+template <> struct Vec8<float> {
+  float f[8];
+  static constexpr float kLow = -1e38f;
+  __device__ void load(const float* p) {
+    const float4 a = __ldg((const float4*)p), b = __ldg((const float4*)p + 1);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  }
+  __device__ void set(int i, float x) { f[i] = x; }
+  __device__ void fill(float x) { for (int i = 0; i < 8; ++i) f[i] = x; }
+  __device__ float max() const {
+    float m = f[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(f[i]));
+    return m;
+  }
+  __device__ void clamp(float lo) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = fmaxf(f[i], lo);
+  }
+  __device__ void get(float* o) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = f[i];
+  }
+};
+template <> struct Vec8<__nv_bfloat16> {
+  __nv_bfloat162 h[4];
+  static constexpr float kLow = -1e38f;
+  __device__ void load(const __nv_bfloat16* p) { *(uint4*)h = __ldg((const uint4*)p); }
+  __device__ void set(int i, __nv_bfloat16 x) { if (i & 1) h[i >> 1].y = x; else h[i >> 1].x = x; }
+  __device__ void fill(float x) { for (int i = 0; i < 4; ++i) h[i] = __float2bfloat162_rn(x); }
+  __device__ float max() const {
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return __bfloat162float(__hmax_nan(m.x, m.y));
+  }
+  __device__ void clamp(float lo) {
+    const __nv_bfloat162 l = __bfloat162bfloat162(__float2bfloat16_rd(lo));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __hmax2(h[i], l);
+  }
+  __device__ void get(float* o) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = *(const uint32_t*)&h[i];
+      o[2 * i] = __uint_as_float(w << 16);
+      o[2 * i + 1] = __uint_as_float(w & 0xffff0000u);
+    }
+  }
+};
+template <> struct Vec8<__half> {
+  __half2 h[4];
+  static constexpr float kLow = -6e4f;
+  __device__ void load(const __half* p) { *(uint4*)h = __ldg((const uint4*)p); }
+  __device__ void set(int i, __half x) { if (i & 1) h[i >> 1].y = x; else h[i >> 1].x = x; }
+  __device__ void fill(float x) { for (int i = 0; i < 4; ++i) h[i] = __float2half2_rn(x); }
+  __device__ float max() const {
+    const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return __half2float(__hmax_nan(m.x, m.y));
+  }
+  __device__ void clamp(float lo) {
+    const __half2 l = __half2half2(__float2half_rd(lo));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __hmax2(h[i], l);
+  }
+  __device__ void get(float* o) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float2 v = __half22float2(h[i]); o[2 * i] = v.x; o[2 * i + 1] = v.y; }
+  }
+};
 
 struct LpArgs {
   const void* z; long long ld; long long rows; int V;
@@ -76,60 +141,106 @@ __device__ __forceinline__ LpStat lp_join(LpStat a, LpStat b) {
 
 // A row is cut in vectors of 8 from the aligned address at or before its start: index v of that grid is logit v - skew. What lies
 // outside [0, V) is not read and counts as -inf.
-template <typename T> __device__ __forceinline__ void load_row8(const T* base, int skew, int V, int v, float* f) {
-  if (v >= skew && v + 8 <= skew + V) { load8(base + v, f); return; }
+template <typename T> __device__ __forceinline__ void load_vec(const T* base, int skew, int V, int v, Vec8<T>& x) {
+  if (v >= skew && v + 8 <= skew + V) { x.load(base + v); return; }
+  x.fill(-INFINITY);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = (v + i >= skew && v + i < skew + V) ? to_f(base[v + i]) : -INFINITY;
+  for (int i = 0; i < 8; ++i)
+    if (v + i >= skew && v + i < skew + V) x.set(i, base[v + i]);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(LpArgs a) {
+// candidates are ordered by (value, lowest index) as one whole number
+__device__ __forceinline__ unsigned long long cand_of(int key, int index) {
+  return ((unsigned long long)((unsigned)key ^ 0x80000000u) << 32) | (0xffffffffu - (unsigned)index);
+}
+__device__ __forceinline__ unsigned cand_index(unsigned long long c) { return 0xffffffffu - (unsigned)c; }
+
+// GR: logits a granule (0: no alternatives are asked for)
+template <typename T, int GR>
+__global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(LpArgs a) {
   cg::cluster_group cl = cg::this_cluster();
   const int part = (int)cl.block_rank(), parts = (int)cl.num_blocks();
   const long long row = blockIdx.x / parts;
-  __shared__ int s_seg[kMaxSegs];                    // order keys of the segments' maxima (of all parts, in part 0)
+  __shared__ int s_gran[GR ? kMaxGranules : 1];      // order keys of the granules' maxima (of all parts, in part 0)
   __shared__ LpStat s_stat[kLpWarps], s_part[8];
   __shared__ int s_pick[kMaxTop];
-  __shared__ unsigned long long s_cand[kCand];
+  __shared__ unsigned long long s_cand[GR ? kCand : 1];
   __shared__ int s_n, s_floor;
   __shared__ float2 s_ml;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const T* z = (const T*)a.z + row * a.ld;
-  const int skew = (int)(((uintptr_t)z & 15) / sizeof(T)) & 7;
+  const int skew = (int)(((uintptr_t)z & 15) / sizeof(T));
   const T* base = z - skew;
-  const int segs = (skew + a.V + kSeg - 1) / kSeg;
-  int* seg0 = cl.map_shared_rank(s_seg, 0);
+  const int span = skew + a.V, segs = (span + kSeg - 1) / kSeg;
+  int* gran0 = GR ? cl.map_shared_rank(s_gran, 0) : nullptr;
   if (parts > 1) cl.sync();                          // part 0 runs: its shared memory may be written
 
   LpStat st{-INFINITY, 0.f, 0.f};
-  for (int g = part * kLpWarps + w; g < segs; g += parts * kLpWarps) {
-    float f[kPerLane];
+  const int step = parts * kLpWarps;
+  int g = part * kLpWarps + w;
+  Vec8<T> next[2];
+  if (g < segs) {
 #pragma unroll
-    for (int i = 0; i < kPerLane / 8; ++i) load_row8(base, skew, a.V, g * kSeg + i * 256 + lane * 8, f + 8 * i);
-    float mx = f[0];
-    bool nan = f[0] != f[0];
+    for (int i = 0; i < 2; ++i) load_vec(base, skew, a.V, g * kSeg + i * 256 + lane * 8, next[i]);
+  }
+  for (; g < segs; g += step) {
+    Vec8<T> x[2] = {next[0], next[1]};
+    if (g + step < segs) {
 #pragma unroll
-    for (int i = 1; i < kPerLane; ++i) { mx = fmaxf(mx, f[i]); nan |= f[i] != f[i]; }
-    if (nan) mx = __int_as_float(0x7fffffff);
-    if (a.top > 0) {
+      for (int i = 0; i < 2; ++i) load_vec(base, skew, a.V, (g + step) * kSeg + i * 256 + lane * 8, next[i]);
+    }
+    const float m0 = x[0].max(), m1 = x[1].max();
+    float mx;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(mx) : "f"(m0), "f"(m1));
+    if constexpr (GR == 512) {
       const int k = __reduce_max_sync(0xffffffffu, order_key(mx));
-      if (lane == 0) seg0[g] = k;
+      if (lane == 0) gran0[g] = k;
+    } else if constexpr (GR > 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        int k = order_key(i ? m1 : m0);
+        if (GR == 64)
+#pragma unroll
+          for (int d = 1; d < 8; d <<= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, d));
+        const int at = g * (kSeg / GR) + (i * 256 + lane * 8) / GR;
+        if (lane % (GR / 8) == 0 && at * GR < span) gran0[at] = k;
+      }
     }
     if (mx > st.m || mx != mx) {
-      const LpStat old = st;
+      const float d = (st.m - mx) * kL2e, p = lp_ex2(d);
       st.m = mx;
-      const float d = (old.m - mx) * kL2e, p = lp_ex2(d);
-      st.l = old.l * p;
-      st.s = p == 0.f ? 0.f : p * (old.s + d * old.l);
+      st.s = p == 0.f ? 0.f : p * (st.s + d * st.l);
+      st.l *= p;
     }
     if (st.m == -INFINITY) continue;
-    const float off = st.m;
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      const float d = (f[i] - off) * kL2e, p = lp_ex2(d);
-      st.l += p;
-      st.s += p == 0.f ? 0.f : p * d;
+    uint64_t l2[2] = {0, 0}, s2[2] = {0, 0};
+    const uint64_t off = pack(-st.m, -st.m), l2e = pack(kL2e, kL2e);
+    const bool safe = st.m > Vec8<T>::kLow;
+    if (safe) {                                      // from here on (z - m) log2(e) is finite and its exponential 0 where it should be
+      const float lo = st.m - fmaxf(104.f, fabsf(st.m) * 0.015625f);
+      x[0].clamp(lo);
+      x[1].clamp(lo);
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float f[8];
+      x[i].get(f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint64_t d = mul2(add2(pack(f[2 * j], f[2 * j + 1]), off), l2e);
+        float d0, d1;
+        unpack(d, d0, d1);
+        if (!safe) { d0 = fmaxf(d0, -200.f); d1 = fmaxf(d1, -200.f); d = pack(d0, d1); }
+        const uint64_t p = pack(lp_ex2(d0), lp_ex2(d1));
+        l2[j & 1] = add2(l2[j & 1], p);
+        s2[j & 1] = fma2(p, d, s2[j & 1]);
+      }
+    }
+    float u, v;
+    unpack(add2(l2[0], l2[1]), u, v);
+    st.l += u + v;
+    unpack(add2(s2[0], s2[1]), u, v);
+    st.s += u + v;
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
@@ -146,102 +257,111 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(LpArgs a) {
     for (int i = 1; i < kLpWarps; ++i) st = lp_join(st, s_stat[i]);
     *cl.map_shared_rank(&s_part[part], 0) = st;
   }
-  cl.sync();
+  if (parts > 1) cl.sync(); else __syncthreads();
   if (part) return;                                  // part 0 has everything and reads no other block's memory from here on
-  if (tid == 0) {
+  if (tid == kLpThreads - 1) {
     st = s_part[0];
     for (int i = 1; i < parts; ++i) st = lp_join(st, s_part[i]);
     const float2 ml = make_float2(st.m, lp_lg2(st.l) * kLn2);
     const long long y = a.ids[row];
     a.logprob[row] = y >= 0 && y < a.V ? log_prob(to_f(z[y]), ml) : 0.f;
     a.entropy[row] = st.m == -INFINITY ? 0.f : ml.y - st.s / st.l * kLn2;
-    a.stat[row] = ml;
+    if (a.stat) a.stat[row] = ml;
     s_ml = ml;
   }
-  if (a.top == 0) return;
-  // the first `top` segments by (maximum, lowest index): one warp, keys in registers, a round each
-  const int want = min(a.top, segs);
-  if (w == 0) {
-    int key[kMaxSegs / 32];
-    unsigned taken = 0;
-#pragma unroll
-    for (int i = 0; i < kMaxSegs / 32; ++i) key[i] = i * 32 + lane < segs ? s_seg[i * 32 + lane] : (int)0x80000000;
-    for (int r = 0; r < want; ++r) {
-      int best = (int)0x80000000, at = 0x7fffffff;
-#pragma unroll
-      for (int i = 0; i < kMaxSegs / 32; ++i)
-        if (!(taken >> i & 1) && i * 32 + lane < segs && (key[i] > best || at == 0x7fffffff)) { best = key[i]; at = i * 32 + lane; }
-      const int top = __reduce_max_sync(0xffffffffu, best);
-      const int win = __reduce_min_sync(0xffffffffu, best == top ? at : 0x7fffffff);
-      if (at == win) taken |= 1u << (win >> 5);
-      if (lane == 0) { s_pick[r] = win; s_floor = top; }
-    }
-  }
-  __syncthreads();
-  // candidates: logits of those segments that reach the smallest of their maxima (fewer segments than `top`: all logits)
-  const int floor_key = want < a.top ? (int)0x80000000 : s_floor;
-  for (int r = w; r < want; r += kLpWarps) {
-    const int g = s_pick[r];
-#pragma unroll
-    for (int i = 0; i < kPerLane / 8; ++i) {
-      float f[8];
-      const int v = g * kSeg + i * 256 + lane * 8;
-      load_row8(base, skew, a.V, v, f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int k = order_key(f[j]);
-        if (v + j >= skew && v + j < skew + a.V && k >= floor_key) {
-          const int at = atomicAdd(&s_n, 1);         // the order of arrival does not matter: candidates are ranked below
-          if (at < kCand) s_cand[at] = ((unsigned long long)((unsigned)k ^ 0x80000000u) << 32) | (0xffffffffu - (unsigned)(v + j - skew));
+  if constexpr (GR > 0) {
+    // the first `top` granules by (maximum, lowest index): one warp, a round each
+    const int grans = (span + GR - 1) / GR, want = min(a.top, grans);
+    if (w == 0) {
+      for (int r = 0; r < want; ++r) {
+        int best = (int)0x80000000, at = 0x7fffffff;                 // a key is never the smallest integer: that marks the taken ones
+        for (int i = lane; i < grans; i += 32) {
+          const int k = s_gran[i];
+          if (k > best) { best = k; at = i; }
         }
+        const int top = __reduce_max_sync(0xffffffffu, best);
+        const int win = __reduce_min_sync(0xffffffffu, best == top ? at : 0x7fffffff);
+        if (lane == 0) { s_gran[win] = (int)0x80000000; s_pick[r] = win; s_floor = top; }
+        __syncwarp();
       }
     }
-  }
-  __syncthreads();
-  const float2 ml = s_ml;
-  const int n = s_n;
-  if (n <= kCand) {
-    // rank = number of candidates before this one in (value, lowest index) order; all are different
-    for (int i = tid; i < n; i += kLpThreads) {
-      const unsigned long long c = s_cand[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += s_cand[j] > c;
-      if (rank < a.top) {
-        const unsigned v = 0xffffffffu - (unsigned)c;
-        a.top_id[row * a.top + rank] = v;
-        a.top_lp[row * a.top + rank] = log_prob(to_f(z[v]), ml);
+    __syncthreads();
+    // candidates: logits of those granules that reach the smallest of their maxima (fewer granules than `top`: all logits)
+    const int floor_key = want < a.top ? (int)0x80000000 : s_floor;
+    constexpr int VPG = GR / 8;                      // vectors a granule
+    for (int q0 = 0; q0 < want * VPG; q0 += 4 * kLpThreads) {
+      Vec8<T> x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int q = q0 + u * kLpThreads + tid;
+        if (q < want * VPG) load_vec(base, skew, a.V, s_pick[q / VPG] * GR + q % VPG * 8, x[u]);
       }
-    }
-    return;
-  }
-  // Many equal logits (a row of constants): a round for each alternative, the next key below the last one. No list, exact.
-  unsigned long long below = ~0ull;
-  for (int r = 0; r < a.top; ++r) {
-    unsigned long long best = 0;
-    for (int q = w; q < want; q += kLpWarps)
-      for (int i = 0; i < kPerLane / 8; ++i) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int q = q0 + u * kLpThreads + tid;
+        if (q >= want * VPG) break;
+        const int v = s_pick[q / VPG] * GR + q % VPG * 8;
+        if (order_key(x[u].max()) < floor_key) continue;
         float f[8];
-        const int v = s_pick[q] * kSeg + i * 256 + lane * 8;
-        load_row8(base, skew, a.V, v, f);
+        x[u].get(f);
+#pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (v + j < skew || v + j >= skew + a.V) continue;
-          const unsigned long long c = ((unsigned long long)((unsigned)order_key(f[j]) ^ 0x80000000u) << 32) | (0xffffffffu - (unsigned)(v + j - skew));
-          if (c < below && c > best) best = c;
+          const int k = order_key(f[j]);
+          if (v + j >= skew && v + j < span && k >= floor_key) {
+            const int at = atomicAdd(&s_n, 1);       // the order of arrival does not matter: candidates are ranked below
+            if (at < kCand) s_cand[at] = cand_of(k, v + j - skew);
+          }
         }
       }
-    for (int d = 16; d; d >>= 1) {
-      const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, d);
-      if (o > best) best = o;
     }
-    if (lane == 0) s_cand[w] = best;
     __syncthreads();
-    for (int i = 0; i < kLpWarps; ++i) if (s_cand[i] > best) best = s_cand[i];
-    __syncthreads();
-    below = best;
-    if (tid == 0) {
-      const unsigned v = 0xffffffffu - (unsigned)best;
-      a.top_id[row * a.top + r] = v;
-      a.top_lp[row * a.top + r] = log_prob(to_f(z[v]), ml);
+    const float2 ml = s_ml;
+    const int n = s_n;
+    if (n <= kCand) {
+      // rank: number of candidates before this one; all are different
+      for (int i = tid; i < n; i += kLpThreads) {
+        const unsigned long long c = s_cand[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += s_cand[j] > c;
+        if (rank < a.top) {
+          const unsigned v = cand_index(c);
+          a.top_id[row * a.top + rank] = v;
+          a.top_lp[row * a.top + rank] = log_prob(to_f(z[v]), ml);
+        }
+      }
+      return;
+    }
+    // Many equal logits (a row of constants): a round for each alternative, the next one below the last. No list, exact.
+    unsigned long long below = ~0ull;
+    for (int r = 0; r < a.top; ++r) {
+      unsigned long long best = 0;
+      for (int q = tid; q < want * VPG; q += kLpThreads) {
+        const int v = s_pick[q / VPG] * GR + q % VPG * 8;
+        Vec8<T> x;
+        load_vec(base, skew, a.V, v, x);
+        float f[8];
+        x.get(f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const unsigned long long c = cand_of(order_key(f[j]), v + j - skew);
+          if (v + j >= skew && v + j < span && c < below && c > best) best = c;
+        }
+      }
+      for (int d = 16; d; d >>= 1) {
+        const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, d);
+        if (o > best) best = o;
+      }
+      __syncthreads();
+      if (lane == 0) s_cand[w] = best;
+      __syncthreads();
+      for (int i = 0; i < kLpWarps; ++i)
+        if (s_cand[i] > best) best = s_cand[i];
+      below = best;
+      if (tid == 0) {
+        const unsigned v = cand_index(best);
+        a.top_id[row * a.top + r] = v;
+        a.top_lp[row * a.top + r] = log_prob(to_f(z[v]), ml);
+      }
     }
   }
 }
@@ -281,7 +401,7 @@ template <typename T> __global__ void __launch_bounds__(kGradThreads) token_logp
   const long long row = blockIdx.x;
   const T* z = (const T*)a.z + row * a.ld;
   T* dz = (T*)a.dz + row * a.V;
-  const int skew = (int)(((uintptr_t)z & 15) / sizeof(T)) & 7;
+  const int skew = (int)(((uintptr_t)z & 15) / sizeof(T));
   const bool aligned = (((uintptr_t)z ^ (uintptr_t)dz) & 15) == 0;
   const T* base = z - skew;
   const float2 ml = a.stat[row];
@@ -294,8 +414,10 @@ template <typename T> __global__ void __launch_bounds__(kGradThreads) token_logp
   for (int u = 0; u < kGradVecs; ++u) {
     const int v = blockIdx.y * kGradChunk + u * kGradThreads * 8 + threadIdx.x * 8;
     if (v >= skew + a.V) continue;
+    Vec8<T> x;
+    load_vec(base, skew, a.V, v, x);
     float f[8];
-    load_row8(base, skew, a.V, v, f);
+    x.get(f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float d = (f[i] - ml.x) - ml.y, p = empty ? 0.f : lp_ex2(d * kL2e);
@@ -310,7 +432,11 @@ template <typename T> __global__ void __launch_bounds__(kGradThreads) token_logp
   }
 }
 
-template <typename T> int launch_logprobs(const LpArgs& a, int parts, cudaStream_t st) {
+template <typename T, int GR> int launch_granule(const LpArgs& a, int parts, cudaStream_t st) {
+  if (parts == 1) {
+    token_logprobs_kernel<T, GR><<<(unsigned)a.rows, kLpThreads, 0, st>>>(a);
+    return (int)cudaGetLastError();
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * parts));
   cfg.blockDim = dim3(kLpThreads);
@@ -321,7 +447,17 @@ template <typename T> int launch_logprobs(const LpArgs& a, int parts, cudaStream
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a);
+  return (int)cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, GR>, a);
+}
+template <typename T> int launch_logprobs(const LpArgs& a, cudaStream_t st) {
+  // parts of a row: while the card holds them all at once (4 blocks a multiprocessor) and every warp has a segment
+  int parts = 1;
+  while (parts < 8 && a.rows * parts * 2 <= 4ll * sm_count() && a.V >= parts * 2 * kLpWarps * kSeg) parts *= 2;
+  if (a.top == 0) return launch_granule<T, 0>(a, parts, st);
+  // granules: enough of them that the ones read again are few, few enough for one warp to pick from
+  if (a.V <= 4096) return launch_granule<T, 8>(a, parts, st);
+  if (a.V <= 16384) return launch_granule<T, 64>(a, parts, st);
+  return launch_granule<T, 512>(a, parts, st);
 }
 template <typename T> int launch_grad(const LpGradArgs& a, cudaStream_t st) {
   const dim3 grid((unsigned)a.rows, (unsigned)((a.V + 7 + kGradChunk - 1) / kGradChunk));
@@ -332,32 +468,37 @@ template <typename T> int launch_grad(const LpGradArgs& a, cudaStream_t st) {
 
 using namespace hippo;
 
-// logits [rows][V] (row pitch ld elements), dtype 0 bf16, 1 fp16, 2 fp32; out fp32 [rows] logprob, entropy, [rows][2] stat; with top > 0
-// top_lp [rows][top], top_id [rows][top].
-extern "C" int hippo_token_logprobs(const void* z, int dtype, long long ld, long long rows, int V, const long long* ids, int top,
-                                    float* logprob, float* entropy, float* stat, float* top_lp, long long* top_id, void* stream) {
-  if (rows <= 0) return 0;
-  if (V < 1 || V > (kMaxSegs - 1) * kSeg || top < 0 || top > kMaxTop || top > V || rows > 0x0fffffffll) return -1;
-  LpArgs a{z, ld, rows, V, ids, top, logprob, entropy, (float2*)stat, top_lp, top_id};
-  // parts of a row: as many CTAs as fill the card once, but no part below one segment a warp
-  int parts = 1;
-  while (parts < 8 && rows * parts * 2 <= 2 * sm_count() && V >= parts * 2 * kLpWarps * kSeg) parts *= 2;
-  cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == 0) return launch_logprobs<__nv_bfloat16>(a, parts, st);
-  if (dtype == 1) return launch_logprobs<__half>(a, parts, st);
-  if (dtype == 2) return launch_logprobs<float>(a, parts, st);
+// logits [rows][V] (row pitch ld elements), dtype 0 bf16, 1 fp16, 2 fp32; out fp32 [rows] logprob, entropy, [rows][2] stat (or null);
+// with top > 0 top_lp [rows][top], top_id [rows][top]. One block of arguments, as in kv8.cu.
+struct LpCall {
+  const void* z; const long long* ids; float *logprob, *entropy, *stat, *top_lp; long long* top_id; void* stream;
+  long long ld, rows;
+  int V, top, dtype;
+};
+extern "C" int hippo_token_logprobs(const LpCall* c) {
+  if (c->rows <= 0) return 0;
+  if (c->V < 1 || c->V > (kMaxGranules - 1) * kSeg || c->top < 0 || c->top > kMaxTop || c->top > c->V || c->rows > 0x0fffffffll) return -1;
+  LpArgs a{c->z, c->ld, c->rows, c->V, c->ids, c->top, c->logprob, c->entropy, (float2*)c->stat, c->top_lp, c->top_id};
+  cudaStream_t st = (cudaStream_t)c->stream;
+  if (c->dtype == 0) return launch_logprobs<__nv_bfloat16>(a, st);
+  if (c->dtype == 1) return launch_logprobs<__half>(a, st);
+  if (c->dtype == 2) return launch_logprobs<float>(a, st);
   return -1;
 }
 
-extern "C" int hippo_token_logprobs_grad(const void* z, int dtype, long long ld, long long rows, int V, const long long* ids,
-                                         const float* stat, const float* entropy, const float* g_lp, const float* g_h, void* dz,
-                                         void* stream) {
-  if (rows <= 0) return 0;
-  if (V < 1 || rows > 0x7fffffffll) return -1;
-  LpGradArgs a{z, ld, rows, V, ids, (const float2*)stat, entropy, g_lp, g_h, dz};
-  cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == 0) return launch_grad<__nv_bfloat16>(a, st);
-  if (dtype == 1) return launch_grad<__half>(a, st);
-  if (dtype == 2) return launch_grad<float>(a, st);
+// dz [rows][V] from the gradients of logprob and entropy (either may be null)
+struct LpGradCall {
+  const void* z; const long long* ids; const float *stat, *entropy, *g_lp, *g_h; void *dz, *stream;
+  long long ld, rows;
+  int V, dtype;
+};
+extern "C" int hippo_token_logprobs_grad(const LpGradCall* c) {
+  if (c->rows <= 0) return 0;
+  if (c->V < 1 || c->rows > 0x7fffffffll) return -1;
+  LpGradArgs a{c->z, c->ld, c->rows, c->V, c->ids, (const float2*)c->stat, c->entropy, c->g_lp, c->g_h, c->dz};
+  cudaStream_t st = (cudaStream_t)c->stream;
+  if (c->dtype == 0) return launch_grad<__nv_bfloat16>(a, st);
+  if (c->dtype == 1) return launch_grad<__half>(a, st);
+  if (c->dtype == 2) return launch_grad<float>(a, st);
   return -1;
 }

@@ -15,6 +15,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from ..ref import kv8 as _ref
+from . import kv8_cuda
 
 BLOCK_SIZES = (16, 32, 64)
 CODE_TYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
@@ -34,12 +35,6 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _same_device(first: torch.Tensor, *rest: torch.Tensor) -> None:
-    for t in rest:
-        if t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}")
-
-
 def kv8_empty(blocks: int, heads: int, head_dim: int, block_size: int = 64, dtype="e4m3", device=None
               ) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(codes, scales)`` of an empty cache. ``dtype``: "e4m3" (relative steps: keys or values of very different sizes in one block)
@@ -51,7 +46,22 @@ def kv8_empty(blocks: int, heads: int, head_dim: int, block_size: int = 64, dtyp
     return codes, torch.ones((2, blocks, heads), dtype=torch.float32, device=device)
 
 
-def _check_cache(codes: torch.Tensor, scales: torch.Tensor) -> None:
+# The operators check their arguments in one expression and call these only to say what is wrong: a decoding step makes these
+# calls for every layer, and its time is the host's.
+def _cache_ok(codes, scales) -> bool:
+    c = codes.shape
+    return (len(c) == 5 and c[0] == 2 and c[1] > 0 and c[2] > 0 and c[3] in BLOCK_SIZES
+            and (codes.dtype == torch.float8_e4m3fn or codes.dtype == torch.int8) and codes.is_contiguous()
+            and codes.data_ptr() % 16 == 0 and scales.dtype == torch.float32 and scales.is_contiguous() and scales.shape == c[:3])
+
+
+def _table_ok(table, lens) -> bool:
+    t = table.shape
+    return (len(t) == 2 and t[1] > 0 and table.dtype == torch.int32 and table.stride(1) == 1 and lens.dtype == torch.int32
+            and lens.is_contiguous() and lens.shape == t[:1])
+
+
+def _refuse_cache(codes, scales) -> None:
     _need(codes.dim() == 5 and codes.shape[0] == 2 and codes.is_contiguous() and codes.dtype in CODE_TYPES.values(),
           "codes: contiguous int8 or float8_e4m3fn [2, blocks, heads, block_size, head_dim]")
     _need(scales.dtype == torch.float32 and scales.is_contiguous() and scales.shape == codes.shape[:3],
@@ -61,10 +71,14 @@ def _check_cache(codes: torch.Tensor, scales: torch.Tensor) -> None:
     _need(codes.data_ptr() % 16 == 0, "codes: a start on 16 bytes")
 
 
-def _check_table(table: torch.Tensor, lens: torch.Tensor) -> None:
+def _refuse_table(table, lens) -> None:
     _need(table.dim() == 2 and table.dtype == torch.int32 and table.stride(1) == 1 and table.shape[1] > 0,
           "table: int32 [requests, width > 0], unit stride along the width")
     _need(lens.dtype == torch.int32 and lens.is_contiguous() and lens.shape == table.shape[:1], "lens: contiguous int32 [requests]")
+
+
+def _refuse_devices(*tensors) -> None:
+    raise ValueError("tensors on different devices: " + ", ".join(str(t.device) for t in tensors))
 
 
 def kv8_plan(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, free_list: torch.Tensor, free_count: torch.Tensor,
@@ -82,32 +96,36 @@ def kv8_plan(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, fr
     ``table`` gets the new blocks and ``free_list`` the released ones, in place; lengths and the stack's height are returned new
     (``plan.lens``, ``plan.free_count``), so a repeated call with the same lengths gives the same plan. Lengths below 0 count as 0,
     lengths beyond the table's width as the width."""
-    _check_table(table, lens)
-    _need(table.shape[0] <= 1 or table.stride(0) >= table.shape[1], "table: rows that do not overlap")
-    _need(new_lens.dtype == torch.int32 and new_lens.is_contiguous() and new_lens.shape == lens.shape,
-          "new_lens: contiguous int32 [requests]")
-    _need(free_list.dim() == 1 and free_list.dtype == torch.int32 and free_list.is_contiguous() and free_list.numel() > 0,
-          "free_list: contiguous int32 [capacity > 0]")
-    _need(free_count.dtype == torch.int32 and free_count.numel() == 1, "free_count: int32 [1]")
-    _need(block_size in BLOCK_SIZES, f"block_size {block_size}: one of {BLOCK_SIZES}")
-    _need(0 <= num_tokens < 1 << 31, "num_tokens: 0 .. 2^31 - 1")
-    _need(table.shape[1] * block_size < 1 << 31, "table: at most 2^31 - 1 tokens a row")
-    _same_device(table, lens, new_lens, free_list, free_count)
-    if release is not None:
-        _need(release.dtype == torch.bool and release.is_contiguous() and release.shape == lens.shape,
-              "release: contiguous bool [requests]")
-        _same_device(table, release)
+    if not (_table_ok(table, lens) and (table.shape[0] <= 1 or table.stride(0) >= table.shape[1])
+            and new_lens.dtype == torch.int32 and new_lens.is_contiguous() and new_lens.shape == lens.shape
+            and free_list.dtype == torch.int32 and free_list.is_contiguous() and free_list.dim() == 1 and free_list.numel() > 0
+            and free_count.dtype == torch.int32 and free_count.numel() == 1 and block_size in BLOCK_SIZES
+            and 0 <= num_tokens < 1 << 31 and table.shape[1] * block_size < 1 << 31
+            and (release is None or (release.dtype == torch.bool and release.is_contiguous() and release.shape == lens.shape))):
+        _refuse_table(table, lens)
+        _need(table.shape[0] <= 1 or table.stride(0) >= table.shape[1], "table: rows that do not overlap")
+        _need(new_lens.dtype == torch.int32 and new_lens.is_contiguous() and new_lens.shape == lens.shape,
+              "new_lens: contiguous int32 [requests]")
+        _need(free_list.dim() == 1 and free_list.dtype == torch.int32 and free_list.is_contiguous() and free_list.numel() > 0,
+              "free_list: contiguous int32 [capacity > 0]")
+        _need(free_count.dtype == torch.int32 and free_count.numel() == 1, "free_count: int32 [1]")
+        _need(block_size in BLOCK_SIZES, f"block_size {block_size}: one of {BLOCK_SIZES}")
+        _need(0 <= num_tokens < 1 << 31, "num_tokens: 0 .. 2^31 - 1")
+        _need(table.shape[1] * block_size < 1 << 31, "table: at most 2^31 - 1 tokens a row")
+        _need(False, "release: contiguous bool [requests]")
+    dev = table.get_device()
+    if not (dev == lens.get_device() == new_lens.get_device() == free_list.get_device() == free_count.get_device()) or (
+            release is not None and release.get_device() != dev):
+        _refuse_devices(table, lens, new_lens, free_list, free_count, *([] if release is None else [release]))
     if table.shape[0] == 0:
         d = table.device
         return KV8Plan(torch.full((num_tokens,), -1, dtype=torch.int64, device=d), lens.clone(), free_count.reshape(1).clone(),
                        torch.empty(0, dtype=torch.bool, device=d), torch.zeros(1, dtype=torch.int32, device=d))
-    if table.is_cuda:
-        from . import kv8_cuda
-        return KV8Plan(*kv8_cuda.plan(table, lens, new_lens, free_list, free_count, block_size, num_tokens, release))
+    if dev >= 0:
+        return KV8Plan(*kv8_cuda.plan(table, lens, new_lens, free_list, free_count, block_size, num_tokens, release, dev))
     return KV8Plan(*_ref.kv8_plan(table, lens, new_lens, free_list, free_count, block_size, num_tokens, release))
 
 
-@torch.no_grad()
 def kv8_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
     """Stores the keys and values [tokens, heads, head_dim] of new tokens at their ``slots``, in place.
 
@@ -116,40 +134,49 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, codes: torc
     one block stand next to each other, at ascending slots without gaps (as ``kv8_plan`` lays them out), and no slot appears twice.
     Slots outside the cache are skipped. A key or value that is not finite makes the scale of its (block, head) NaN, so that what
     attends to it is NaN. Not differentiable (the cache belongs to inference)."""
-    _check_cache(codes, scales)
-    _need(k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype and k.dtype in FLOAT_TYPES,
-          "k, v: [tokens, heads, head_dim], both bf16, fp16 or fp32")
-    _need(k.shape[1] == codes.shape[2] and k.shape[2] == codes.shape[4], "k, v and codes: heads and head_dim differ")
-    _need(slots.dtype == torch.int64 and slots.is_contiguous() and slots.shape == k.shape[:1], "slots: contiguous int64 [tokens]")
-    _same_device(codes, scales, k, v, slots)
-    if k.shape[0] == 0:
+    ks, c = k.shape, codes.shape
+    if not (_cache_ok(codes, scales) and len(ks) == 3 and ks == v.shape and k.dtype == v.dtype and k.dtype in FLOAT_TYPES
+            and ks[1] == c[2] and ks[2] == c[4] and slots.dtype == torch.int64 and slots.is_contiguous() and slots.shape == ks[:1]):
+        _refuse_cache(codes, scales)
+        _need(k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype and k.dtype in FLOAT_TYPES,
+              "k, v: [tokens, heads, head_dim], both bf16, fp16 or fp32")
+        _need(ks[1] == c[2] and ks[2] == c[4], "k, v and codes: heads and head_dim differ")
+        _need(False, "slots: contiguous int64 [tokens]")
+    dev = codes.get_device()
+    if not (dev == scales.get_device() == k.get_device() == v.get_device() == slots.get_device()):
+        _refuse_devices(codes, scales, k, v, slots)
+    if ks[0] == 0:
         return
-    if k.is_cuda:
-        from . import kv8_cuda
-        kv8_cuda.write(k, v, slots, codes, scales)
+    if dev >= 0:
+        kv8_cuda.write(k, v, slots, codes, scales, dev)
     else:
-        _ref.kv8_write(k, v, slots, codes, scales)
+        with torch.no_grad():
+            _ref.kv8_write(k, v, slots, codes, scales)
 
 
-@torch.no_grad()
 def attention_decode_kv8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
                          scale: Optional[float] = None) -> torch.Tensor:
     """One query token per request against its ``lens[n]`` cached tokens (its own included): q [requests, q heads, head_dim] (bf16,
     fp16 or fp32) -> the same shape and type, contiguous. Query head i reads kv head i // (q heads / kv heads). A request without
     tokens gives zeros; bytes behind the last token are not looked at; a block outside the cache counts as not there. ``scale``
     defaults to head_dim ** -0.5. Inference only (no gradient)."""
-    _check_cache(codes, scales)
-    _check_table(table, lens)
-    _need(q.dim() == 3 and q.dtype in FLOAT_TYPES, "q: bf16, fp16 or fp32 [requests, heads, head_dim]")
-    _need(q.shape[0] == table.shape[0] and q.shape[2] == codes.shape[4], "q, table and codes: requests or head_dim differ")
-    _need(q.shape[1] > 0 and q.shape[1] % codes.shape[2] == 0, "q heads: a multiple of the kv heads")
-    _need(table.shape[1] * codes.shape[3] < 1 << 31, "table: at most 2^31 - 1 tokens a row")
-    _same_device(codes, scales, q, table, lens)
+    qs, c = q.shape, codes.shape
+    if not (_cache_ok(codes, scales) and _table_ok(table, lens) and len(qs) == 3 and q.dtype in FLOAT_TYPES
+            and qs[0] == table.shape[0] and qs[2] == c[4] and qs[1] > 0 and qs[1] % c[2] == 0 and table.shape[1] * c[3] < 1 << 31):
+        _refuse_cache(codes, scales)
+        _refuse_table(table, lens)
+        _need(q.dim() == 3 and q.dtype in FLOAT_TYPES, "q: bf16, fp16 or fp32 [requests, heads, head_dim]")
+        _need(qs[0] == table.shape[0] and qs[2] == c[4], "q, table and codes: requests or head_dim differ")
+        _need(qs[1] > 0 and qs[1] % c[2] == 0, "q heads: a multiple of the kv heads")
+        _need(False, "table: at most 2^31 - 1 tokens a row")
+    dev = codes.get_device()
+    if not (dev == scales.get_device() == q.get_device() == table.get_device() == lens.get_device()):
+        _refuse_devices(codes, scales, q, table, lens)
     if scale is None:
-        scale = q.shape[2] ** -0.5
-    if q.shape[0] == 0:
+        scale = qs[2] ** -0.5
+    if qs[0] == 0:
         return torch.empty_like(q)
-    if q.is_cuda:
-        from . import kv8_cuda
-        return kv8_cuda.attention_decode(q, codes, scales, table, lens, float(scale))
-    return _ref.attention_decode_kv8(q, codes, scales, table, lens, float(scale))
+    if dev >= 0:
+        return kv8_cuda.attention_decode(q, codes, scales, table, lens, scale, dev)
+    with torch.no_grad():
+        return _ref.attention_decode_kv8(q, codes, scales, table, lens, scale)
