@@ -13,8 +13,10 @@ namespace hippo {
 
 // ------------------------------------------------------------------------------------------------ planning
 // One CTA of 1024 threads walks the requests 1024 at a time: a thread owns a request, prefix sums over the CTA give the
-// positions in the stack of free blocks, in the packed tokens, and decide who still fits. Released requests push first. The work
-// is a few dependent loads and five barriers (latency-bound); more CTAs would need a grid-wide order between pushes and pops.
+// positions in the stack of free blocks, in the packed tokens, and decide who still fits. Blocks pushed, blocks popped and slots are
+// then dealt out one by one to all threads, which find their request by bisection of the sums in shared memory (a request may
+// own one block or hundreds). Released requests push first. The work is a few dependent loads and barriers (latency-bound); more
+// CTAs would need a grid-wide order between pushes and pops.
 constexpr int kPlanThreads = 1024;
 
 __device__ __forceinline__ long long block_inclusive_scan(long long v, long long* warp_sum, long long& total) {
@@ -49,14 +51,26 @@ __device__ __forceinline__ long long slot_of(const int* row, int pos, int sh) {
   return b < 0 ? -1ll : ((long long)b << sh) + (pos & ((1 << sh) - 1));
 }
 
+// first index whose sum is above p (the sums ascend, the last one is above p)
+__device__ __forceinline__ int owner_of(const int* sum, int p) {
+  int lo = 0, hi = kPlanThreads - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (sum[mid] > p) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
+
 __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(
     int* table, long long table_ld, int M, const int* __restrict__ lens, const int* __restrict__ new_lens, int N,
     int* free_list, int cap, const int* __restrict__ free_count, const unsigned char* __restrict__ release, int sh,
     long long num_tokens, long long* __restrict__ slots, int* __restrict__ lens_out, int* __restrict__ count_out,
     unsigned char* __restrict__ served, int* __restrict__ cu, int write_slots) {
   __shared__ long long warp_sum[32];
-  __shared__ int s_end[kPlanThreads], s_pos[kPlanThreads];      // packed end of a request's tokens, position of its first one
-  const int tid = threadIdx.x, lane = tid & 31;
+  __shared__ int s_sum[kPlanThreads];                // blocks pushed or popped up to and with this request of the chunk
+  __shared__ int s_have[kPlanThreads];               // blocks it had
+  __shared__ int s_end[kPlanThreads], s_pos[kPlanThreads];      // packed end of its tokens, position of its first one (-1: not served)
+  const int tid = threadIdx.x;
   const int bs1 = (1 << sh) - 1;
   const long long room = (long long)M << sh;
   long long count = min(max(*free_count, 0), cap), total;
@@ -66,18 +80,18 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(
       const int n = base + tid;
       int back = 0;
       if (n < N && release[n]) back = (int)((min((long long)max(lens[n], 0), room) + bs1) >> sh);
-      const long long at = count + block_inclusive_scan(back, warp_sum, total) - back;
-      for (unsigned todo = __ballot_sync(0xffffffffu, back > 0); todo; todo &= todo - 1) {
-        const int src = __ffs(todo) - 1;
-        const int cnt = __shfl_sync(0xffffffffu, back, src);
-        const long long a = __shfl_sync(0xffffffffu, at, src);
-        const int* row = table + (long long)(n - lane + src) * table_ld;
-        for (int j = lane; j < cnt; j += 32)
-          if (a + j < cap) free_list[a + j] = row[j];
+      const long long sum = block_inclusive_scan(back, warp_sum, total);
+      s_sum[tid] = (int)min(sum, (long long)0x7fffffff);
+      __syncthreads();
+      // what does not fit the list any more (more blocks than it holds: a table that is not ours) is dropped
+      const int push = (int)min(total, cap - count);
+      for (int p = tid; p < push; p += kPlanThreads) {
+        const int r = owner_of(s_sum, p);
+        free_list[count + p] = table[(long long)(base + r) * table_ld + p - (r ? s_sum[r - 1] : 0)];
       }
-      count = min(count + total, (long long)cap);
+      count += push;
+      __syncthreads();                               // pushes are visible to the pops of every thread; s_sum is free
     }
-    __syncthreads();                                 // pushes are visible to the pops of every thread
   }
 
   long long tokens = 0, asked = 0, used = 0;         // packed tokens, blocks asked for, blocks handed out so far
@@ -95,42 +109,32 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(
     const long long top = asked + block_inclusive_scan(need, warp_sum, total);
     asked += total;
     const bool ok = want == 0 || (fits && (need == 0 || top <= count));
-    const long long at = count - 1 - (top - need);   // first pop; the rows that get blocks are a prefix of those that ask
-    if (!ok) need = 0;
-    if (need == 1) table[(long long)n * table_ld + have] = free_list[at];
-    for (unsigned todo = __ballot_sync(0xffffffffu, need > 1); todo; todo &= todo - 1) {
-      const int src = __ffs(todo) - 1;
-      const int cnt = __shfl_sync(0xffffffffu, need, src), h0 = __shfl_sync(0xffffffffu, have, src);
-      const long long a = __shfl_sync(0xffffffffu, at, src);
-      int* row = table + (long long)(n - lane + src) * table_ld;
-      for (int j = lane; j < cnt; j += 32) row[h0 + j] = free_list[a - j];
-    }
-    block_inclusive_scan(need, warp_sum, total);
-    used += total;
+    // the requests that get blocks are a prefix of those that ask: their sums without the refused ones are the same
+    const long long mine = block_inclusive_scan(ok ? need : 0, warp_sum, total);
+    s_sum[tid] = (int)mine;
+    s_have[tid] = have;
+    s_end[tid] = (int)min(end, num_tokens);
+    s_pos[tid] = ok && in ? (int)len : -1;
     if (in) {
       lens_out[n] = (int)(ok ? len + want : len);
       served[n] = ok;
       cu[n + 1] = (int)min(end, (long long)0x7fffffff);
     }
-    if (write_slots) {
-      s_end[tid] = (int)min(end, num_tokens);
-      s_pos[tid] = ok ? (int)len : -1;
-      __syncthreads();
-      const long long last = min(tokens, num_tokens);
-      for (long long t = chunk_begin + tid; t < last; t += kPlanThreads) {
-        int lo = 0, hi = kPlanThreads - 1;           // first request of the chunk whose tokens end behind t
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (s_end[mid] > t) hi = mid; else lo = mid + 1;
-        }
-        const int first = lo ? s_end[lo - 1] : (int)chunk_begin;
-        long long slot = -1;
-        if (s_pos[lo] >= 0 && base + lo < N)
-          slot = slot_of(table + (long long)(base + lo) * table_ld, s_pos[lo] + (int)t - first, sh);
-        slots[t] = slot;
-      }
-      __syncthreads();
+    __syncthreads();
+    for (int p = tid; p < (int)total; p += kPlanThreads) {
+      const int r = owner_of(s_sum, p);
+      table[(long long)(base + r) * table_ld + s_have[r] + p - (r ? s_sum[r - 1] : 0)] = free_list[count - 1 - used - p];
     }
+    used += total;
+    if (write_slots) {
+      __syncthreads();                               // the popped blocks are in the table
+      const int last = (int)min(tokens, num_tokens);
+      for (int t = (int)min(chunk_begin, num_tokens) + tid; t < last; t += kPlanThreads) {
+        const int r = owner_of(s_end, t), first = r ? s_end[r - 1] : (int)chunk_begin;
+        slots[t] = s_pos[r] < 0 ? -1ll : slot_of(table + (long long)(base + r) * table_ld, s_pos[r] + t - first, sh);
+      }
+    }
+    __syncthreads();
   }
   if (write_slots)
     for (long long t = min(tokens, num_tokens) + tid; t < num_tokens; t += kPlanThreads) slots[t] = -1;

@@ -1,16 +1,17 @@
 // One query token per sequence against the 8-bit paged cache: o = sum_j softmax_j(scale q.k_j) v_j with k_j = s_K code, v_j = s_V code
 // and one (s_K, s_V) per (block, kv head).
 //
-// Bound by HBM: a token and kv head costs 2 D bytes of codes, read once for all query heads that share the kv head. Work is cut in
-// tiles of 32 tokens; the tiles of all (sequence, kv head, group of 8 query heads) form one list that is divided evenly over all
-// warps of one resident wave, whatever the lengths. A warp streams its tiles through its own TMA ring (no block-wide barrier in the
-// loop) and carries the running maximum and sum; a unit that spans several warps leaves partial (m, l, o) rows that a second, small
-// kernel joins in the order of the tokens, so results do not depend on timing.
+// Bound by HBM: a token and kv head costs 2 D bytes of codes, read once for the query heads that share the kv head (up to 8 of them
+// together). Work is cut in tiles of 32 tokens; the tiles of all (sequence, kv head, group of query heads) form one list that is
+// divided evenly over all warps of one resident wave, whatever the lengths. A warp streams its tiles through its own TMA ring (no
+// block-wide barrier in the loop) and carries the running maximum and sum; a unit that spans several warps leaves partial (m, l, o)
+// rows that a second, small kernel joins in a fixed order, so results do not depend on timing.
 //
-// Arithmetic: codes are exact in fp16, so mma.m16n8k16 (fp16 operands, fp32 accumulators) is exact for them; the query and the
-// probabilities are split in two fp16 terms that sit in rows 0-7 and 8-15 of the A operand (one thread holds both sums), which keeps
-// 21 bits or more of each. Legacy mma is deliberate: with 1 to 8 live rows a 128-row tcgen05 tile would multiply zeros, and the
-// kernel waits for memory, not for the tensor pipe.
+// Arithmetic: codes are exact in fp16, so mma.m16n8k16 (fp16 operands, fp32 accumulators) is exact for them. They are the 16-row
+// operand of both products (S^T = K q^T, O^T = V^T P^T); the 8 columns are 4 query heads, each as two fp16 terms of the query and of
+// the probabilities (21 bits or more), whose two sums meet in one thread. P^T comes from the scores' fragments by movmatrix. The
+// converted codes, not the tensor pipe, set the instruction count, so the narrow side of the product is the query's. Legacy mma is
+// deliberate: with 1 to 8 live columns a 128-row tcgen05 tile would multiply zeros, and the kernel waits for memory.
 // In the reference a decoding step re-runs the whole forward (src/models/model.py:180-219).
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
@@ -28,7 +29,7 @@ struct KvAttnArgs {
   const float* scales; long long half_scales;
   const int* table; long long table_ld; int M;
   const int* lens;
-  int N, H, G, QG, sh, blocks, dtype;                // kv heads, query heads a kv head, groups of 8 of them
+  int N, H, G, QG, sh, blocks, dtype;                // kv heads, query heads a kv head, groups of 4 or 8 of them
   long long half_rows;                               // cache rows (of D bytes) of the key half
   float scale;
   float* part; float* part_ml; int4* desc; int NW, rows;   // parts of `rows` query rows each, two a worker
@@ -43,33 +44,34 @@ template <int D> struct KvShape {
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {       // 8 x 8 fp16, a pair a lane
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 
-// two codes (bytes 0,1 or 2,3 of w) -> two fp16, exactly. int8 goes through 1024 + (code + 128), whose low byte is the biased code.
-template <int E4M3> __device__ __forceinline__ uint32_t codes2(uint32_t w, bool upper) {
-  uint32_t r;
+// four codes -> four fp16, exactly: bytes 0, 1 in `lo`, bytes 2, 3 in `hi`. int8 goes through 1024 + (code + 128), whose low byte is
+// the biased code.
+template <int E4M3> __device__ __forceinline__ void codes4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if (E4M3) {
-    const uint16_t p = upper ? (uint16_t)(w >> 16) : (uint16_t)w;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(p));
-    return r;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+    return;
   }
-  r = __byte_perm(w ^ 0x80808080u, 0x64646464u, upper ? 0x4342 : 0x4140);
-  const __half2 h = __hsub2(*(__half2*)&r, __half2half2(__ushort_as_half(0x6480)));          // 1152
-  return *(const uint32_t*)&h;
+  w ^= 0x80808080u;
+  const uint32_t l = __byte_perm(w, 0x64646464u, 0x4140), h = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 bias = __half2half2(__ushort_as_half(0x6480));       // 1152
+  const __half2 x = __hsub2(*(const __half2*)&l, bias), y = __hsub2(*(const __half2*)&h, bias);
+  lo = *(const uint32_t*)&x;
+  hi = *(const uint32_t*)&y;
 }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *(const uint32_t*)&h;
-}
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(a, b);
-  const float2 f = __half22float2(h);
-  hi = *(const uint32_t*)&h;
-  lo = pack2(a - f.x, b - f.y);
 }
 
 __device__ __forceinline__ float load_q(const KvAttnArgs& a, long long i) {
@@ -87,43 +89,40 @@ __device__ __forceinline__ int cached_len(const KvAttnArgs& a, int n) {
   return (int)min((long long)max(a.lens[n], 0), (long long)a.M << a.sh);
 }
 
-// Where a warp stands in the list of tiles: sequence, unit = (kv head, group of 8 query heads), tile of the unit.
+// Where a warp stands in the list of tiles: sequence, kv head, group of query heads, tile.
 struct Cursor {
-  int n, unit, tile, len, tiles;
-  long long left;                                    // tiles of the warp's range that are still ahead, this one included
-  __device__ void next_sequence(const KvAttnArgs& a) {
+  int n, h, grp, tile, len, tiles, left;             // left: tiles of the warp's range that are still ahead, this one included
+  __device__ void advance(const KvAttnArgs& a) {
+    if (--left <= 0 || ++tile < tiles) return;
+    tile = 0;
+    if (++grp < a.QG) return;
+    grp = 0;
+    if (++h < a.H) return;
+    h = 0;
     do { ++n; len = n < a.N ? cached_len(a, n) : 0; } while (n < a.N && len == 0);
     tiles = (len + kTile - 1) / kTile;
   }
-  __device__ void advance(const KvAttnArgs& a) {
-    --left;
-    if (left <= 0) return;
-    if (++tile < tiles) return;
-    tile = 0;
-    if (++unit < a.H * a.QG) return;
-    unit = 0;
-    next_sequence(a);
-  }
 };
 
-template <int D, int E4M3>
+// SETS: groups of 4 query heads that one pass over the codes serves
+template <int D, int E4M3, int SETS>
 __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid_constant__ CUtensorMap codes_map, KvAttnArgs a) {
   using S = KvShape<D>;
-  constexpr int KS = D / 16, NT = D / 8;             // k steps of q.k, n tiles of p.v
+  constexpr int KS = D / 16, MT = D / 16, DL = D / 8;        // k steps of K q, row tiles of V^T P, output columns a lane
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kWarps][S::kStages];
-  __shared__ float s_scale[kWarps][S::kStages][4];   // K, V scale of the tile's first 16 tokens, K, V of the others
+  __shared__ float4 s_scale[kWarps][S::kStages];     // K, V scale of the tile's first 16 tokens, K, V of the others
   __shared__ int s_there[kWarps][S::kStages];        // which 16-token groups of the tile lie in a block of the pool
   __shared__ long long s_pre[kThreads + 1];
   __shared__ long long s_warp[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int units = a.H * a.QG;
+  asm volatile("griddepcontrol.launch_dependents;");
 
   // rows of empty sequences
-  for (long long i = (long long)blockIdx.x * kThreads + tid; i < (long long)a.N * a.H * a.G * (D / 2); i += (long long)gridDim.x * kThreads) {
-    const int n = (int)(i / (a.H * a.G * (D / 2)));
-    if (a.lens[n] <= 0) store_out(a, i * 2, 0.f, 0.f);
-  }
+  for (int n = blockIdx.x; n < a.N; n += gridDim.x)
+    if (a.lens[n] <= 0)
+      for (int i = tid; i < a.H * a.G * (D / 2); i += kThreads) store_out(a, (long long)n * a.H * a.G * D + i * 2, 0.f, 0.f);
 
   // tiles before every thread's share of the sequences
   const int share = (a.N + kThreads - 1) / kThreads;
@@ -169,14 +168,17 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
         at += c; ++n;
       }
       put.n = n;
-      put.unit = (int)((begin - at) / put.tiles);
-      put.tile = (int)((begin - at) - (long long)put.unit * put.tiles);
-      put.left = end - begin;
+      const int unit = (int)((begin - at) / put.tiles);
+      put.tile = (int)((begin - at) - (long long)unit * put.tiles);
+      put.h = unit / a.QG;
+      put.grp = unit - put.h * a.QG;
+      put.left = (int)(end - begin);
     }
     Cursor get = put;
     // fetching: lanes hold 32 entries of the table row
     int held_n = -1, held_base = 0, held = -1;
     const int box = min(kTile, 1 << a.sh);           // rows of one TMA box
+    const int half_rows = (int)a.half_rows;
     auto fetch = [&](int stage) {
       const int tok = put.tile * kTile, blk = tok >> a.sh;
       const int base = blk & ~31;                    // a tile never spans two batches of 32 entries (at most 2 blocks, even start)
@@ -186,147 +188,154 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
         held = j < a.M && ((long long)j << a.sh) < put.len ? a.table[(long long)put.n * a.table_ld + j] : -1;
         if (held >= a.blocks) held = -1;
       }
-      const int h = put.unit / a.QG;
-      const int b0 = __shfl_sync(0xffffffffu, held, blk - base);
-      const int b1 = a.sh == 4 ? __shfl_sync(0xffffffffu, held, (blk + 1 - base) & 31) : b0;
-      const bool second = a.sh == 4 && tok + 16 < put.len;          // the tile's second block holds tokens
-      const int there = a.sh == 4 ? (b0 >= 0 ? 1 : 0) | (second && b1 >= 0 ? 2 : 0) : (b0 >= 0 ? 3 : 0);
+      const int b0 = __shfl_sync(0xffffffffu, held, blk & 31);
+      const int b1 = a.sh == 4 ? __shfl_sync(0xffffffffu, held, (blk + 1) & 31) : b0;
+      int there = b0 >= 0 ? 3 : 0;
+      if (a.sh == 4) there = (b0 >= 0 ? 1 : 0) | (tok + 16 < put.len && b1 >= 0 ? 2 : 0);
       uint64_t* bar = &full[w][stage];
-      uint8_t* dst = ring + stage * S::kStageBytes;
-      if (lane == 0) {
-        s_there[w][stage] = there;
-        const int boxes = a.sh == 4 ? __popc(there) : (there ? 1 : 0);
-        mbar_expect_tx(bar, (uint32_t)(boxes * 2 * box * D));
-        const int in = tok & ((1 << a.sh) - 1);
-        if (there & 1) {
-          const int y = (int)((((long long)b0 * a.H + h) << a.sh) + in);
-          tma_load_2d(dst, &codes_map, bar, 0, y);
-          tma_load_2d(dst + kTile * D, &codes_map, bar, 0, (int)(y + a.half_rows));
-        }
-        if (a.sh == 4 && (there & 2)) {
-          const int y = (int)(((long long)b1 * a.H + h) << a.sh);
-          tma_load_2d(dst + 16 * D, &codes_map, bar, 0, y);
-          tma_load_2d(dst + kTile * D + 16 * D, &codes_map, bar, 0, (int)(y + a.half_rows));
-        }
-      }
       if (lane < 4) {
-        const int b = lane < 2 ? b0 : b1;
+        const int bh = (lane < 2 ? b0 : b1) * a.H + put.h;           // below 2^31 with the rows of all blocks
         if (there & (lane < 2 ? 1 : 2)) {
-          const float* src = a.scales + (lane & 1) * a.half_scales + (long long)b * a.H + h;
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&s_scale[w][stage][lane])), "l"(src) : "memory");
+          const float* src = a.scales + (lane & 1 ? a.half_scales : 0) + bh;
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32((float*)&s_scale[w][stage] + lane)), "l"(src) : "memory");
+        }
+        if (lane == 0) {
+          uint8_t* dst = ring + stage * S::kStageBytes;
+          s_there[w][stage] = there;
+          const int boxes = a.sh == 4 ? __popc(there) : there & 1;
+          mbar_expect_tx(bar, (uint32_t)(boxes * 2 * box * D));
+          if (there & 1) {
+            const int y = (bh << a.sh) + (tok & ((1 << a.sh) - 1));
+            tma_load_2d(dst, &codes_map, bar, 0, y);
+            tma_load_2d(dst + kTile * D, &codes_map, bar, 0, y + half_rows);
+          }
+          if (a.sh == 4 && (there & 2)) {
+            const int y = (b1 * a.H + put.h) << 4;
+            tma_load_2d(dst + 16 * D, &codes_map, bar, 0, y);
+            tma_load_2d(dst + kTile * D + 16 * D, &codes_map, bar, 0, y + half_rows);
+          }
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
       }
       put.advance(a);
     };
-    const int g = lane >> 2, c = lane & 3;           // row of the fragments (query head), column pair
+    const int g = lane >> 2, c = lane & 3;           // fragments: row (token, output column group) / column of the query side; query head
 #pragma unroll 1
     for (int i = 0; i < S::kStages; ++i)
       if (put.left > 0) fetch(i);
     __syncwarp();
 
-    uint32_t qf[KS][4];
-    float o[NT][4];
-    float m = -INFINITY, mv = -INFINITY, l = 0.f, f = 0.f;
+    uint32_t qf[SETS][KS][2];
+    float o[SETS][MT][4];
+    float m[SETS], mv[SETS], l[SETS], f[SETS];       // maximum of the scores, of scores + log2 of the value scale; sum; factor of the scores
     bool alive = true, fresh = true, whole = true, first = true;
-    int stage = 0, phase = 0, tile0 = 0;
-    long long unit_tile0 = 0;
-    while (get.left > 0 && alive) {
-      const int n = get.n, unit = get.unit, h = unit / a.QG, g0 = (unit - h * a.QG) * 8;
+    int stage = 0, phase = 0;
+    // smem offsets of this lane: K rows g (+ 8), 16 bytes at chunk 2c (D 128) or c (D 64); V rows 2c (+ 1, 8, 9), D / 8 bytes at column g
+    const uint32_t k_at = g * D + (D == 128 ? ((2 * c) ^ g) * 16 : (c ^ ((g >> 1) & 3)) * 16);
+    while (get.left > 0) {
+      const int n = get.n, h = get.h, g0 = get.grp * 4 * SETS;
       if (fresh) {                                   // a new unit: its query rows, normalised to [1, 2) and split in two fp16
         fresh = false;
-        tile0 = get.tile;
-        unit_tile0 = end - get.left - get.tile;
         whole = get.tile == 0;
-        float x[D / 4];
-        float top = 0.f;
-        const bool row = g0 + g < a.G;
-        const long long qi = (long long)n * a.q_n + (long long)(h * a.G + g0 + g) * a.q_h + c * (D / 4);
 #pragma unroll
-        for (int i = 0; i < D / 4; ++i) x[i] = row ? load_q(a, qi + i) : 0.f;
+        for (int t = 0; t < SETS; ++t) {
+          const int qh = g0 + t * 4 + (g >> 1);      // column g of the query side: head g / 2, its high (even) or low term
+          const bool row = qh < a.G;
+          const long long qi = (long long)n * a.q_n + (long long)(h * a.G + qh) * a.q_h + c * (D / 4);
+          float x[D / 4], top = 0.f;
 #pragma unroll
-        for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 126);
-        const float down = pow2f(-e);
-        f = pow2f(e) * a.scale * kLog2e;
+          for (int i = 0; i < D / 4; ++i) x[i] = row ? load_q(a, qi + i) : 0.f;
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          split2(x[4 * i] * down, x[4 * i + 1] * down, qf[i][0], qf[i][1]);
-          split2(x[4 * i + 2] * down, x[4 * i + 3] * down, qf[i][2], qf[i][3]);
+          for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 126);
+          const float down = pow2f(-e);
+          f[t] = __shfl_sync(0xffffffffu, pow2f(e), c * 8) * a.scale * kLog2e;       // of head c: its column 2c is lane 8c's
+#pragma unroll
+          for (int i = 0; i < D / 4; ++i) {
+            x[i] *= down;
+            if (g & 1) x[i] -= __half2float(__float2half_rn(x[i]));
+          }
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            qf[t][i][0] = pack2(x[4 * i], x[4 * i + 1]);
+            qf[t][i][1] = pack2(x[4 * i + 2], x[4 * i + 3]);
+          }
+#pragma unroll
+          for (int i = 0; i < MT; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+          m[t] = mv[t] = -INFINITY; l[t] = 0.f;
         }
-#pragma unroll
-        for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        m = mv = -INFINITY; l = 0.f;
       }
       if (!mbar_wait(&full[w][stage], phase, kWaitTmaFull, worker)) { alive = false; break; }
       const uint8_t* kt = ring + stage * S::kStageBytes;
       const uint8_t* vt = kt + kTile * D;
-      const int there = s_there[w][stage];
-      const int valid = min(kTile, get.len - get.tile * kTile);
+      const int valid = min(kTile, get.len - get.tile * kTile), there = s_there[w][stage];
       const bool ragged = valid < kTile || there != 3;
-      float s[4][4];
+      const float4 sc = s_scale[w][stage];
+      const float lv0 = log2f(sc.y), lv1 = log2f(sc.w);
+      uint32_t pb[SETS][4];                          // P^T as the second operand: two k steps of 16 tokens
+      {
+        float s[SETS][2][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-        const int r = j * 8 + g;
+        for (int t = 0; t < SETS; ++t)
 #pragma unroll
-        for (int q4 = 0; q4 < D / 64; ++q4) {
-          const int chunk = D == 128 ? (2 * c + q4) ^ (r & 7) : c ^ ((r >> 1) & 3);
-          const uint4 x = *(const uint4*)(kt + r * D + chunk * 16);
-          const uint32_t word[4] = {x.x, x.y, x.z, x.w};
+          for (int j = 0; j < 2; ++j) s[t][j][0] = s[t][j][1] = s[t][j][2] = s[t][j][3] = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            mma16816(s[j], qf[q4 * 4 + i], codes2<E4M3>(word[i], false), codes2<E4M3>(word[i], true));
+        for (int q4 = 0; q4 < D / 64; ++q4)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint4 x = *(const uint4*)(kt + j * 16 * D + (k_at ^ (q4 * 16)));           // row 16j + g
+            const uint4 y = *(const uint4*)(kt + j * 16 * D + 8 * D + (k_at ^ (q4 * 16)));   // row 16j + g + 8
+            const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t a0, a1, a2, a3;
+              codes4<E4M3>(xw[i], a0, a2);
+              codes4<E4M3>(yw[i], a1, a3);
+#pragma unroll
+              for (int t = 0; t < SETS; ++t) mma16816(s[t][j], a0, a1, a2, a3, qf[t][q4 * 4 + i][0], qf[t][q4 * 4 + i][1]);
+            }
+          }
+#pragma unroll
+        for (int t = 0; t < SETS; ++t) {
+          // tokens 16j + g and 16j + g + 8 of query head c
+          float y[4], z[4];
+          const float f0 = f[t] * sc.x, f1 = f[t] * sc.z;
+          y[0] = (s[t][0][0] + s[t][0][1]) * f0; y[1] = (s[t][0][2] + s[t][0][3]) * f0;
+          y[2] = (s[t][1][0] + s[t][1][1]) * f1; y[3] = (s[t][1][2] + s[t][1][3]) * f1;
+          z[0] = y[0] + lv0; z[1] = y[1] + lv0; z[2] = y[2] + lv1; z[3] = y[3] + lv1;
+          if (ragged) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (i * 8 + g >= valid || !(there >> (i >> 1) & 1)) y[i] = z[i] = -INFINITY;
+          }
+          float mx = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), mz = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            mz = fmaxf(mz, __shfl_xor_sync(0xffffffffu, mz, d));
+          }
+          mx = fmaxf(mx, m[t]); mz = fmaxf(mz, mv[t]);
+          const float mu = mx == -INFINITY ? 0.f : mx, mzu = mz == -INFINITY ? 0.f : mz;
+          const float alpha = ex2(mv[t] - mzu);
+          l[t] *= ex2(m[t] - mu);
+          m[t] = mx; mv[t] = mz;
+          if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) { o[t][i][0] *= alpha; o[t][i][1] *= alpha; o[t][i][2] *= alpha; o[t][i][3] *= alpha; }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            l[t] += ex2(y[i] - mu);
+            const float p = ex2(z[i] - mzu);
+            pb[t][i] = transpose8x8(pack2(p, p - __half2float(__float2half_rn(p))));
+          }
         }
       }
-      const float ks0 = s_scale[w][stage][0], vs0 = s_scale[w][stage][1], ks1 = s_scale[w][stage][2], vs1 = s_scale[w][stage][3];
-      // log2 of the value scale: whole part and a factor in [1, 2) (1 for the powers of two that the write kernel stores)
-      const float ev0 = (float)((int)((__float_as_uint(vs0) >> 23) & 255) - 127), ev1 = (float)((int)((__float_as_uint(vs1) >> 23) & 255) - 127);
-      const float fv0 = isnan_bits(vs0) ? vs0 : __uint_as_float((__float_as_uint(vs0) & 0x807fffffu) | 0x3f800000u);
-      const float fv1 = isnan_bits(vs1) ? vs1 : __uint_as_float((__float_as_uint(vs1) & 0x807fffffu) | 0x3f800000u);
-      float x[8], mx = -INFINITY, mxv = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float y = (s[j][i] + s[j][i + 2]) * (f * (j < 2 ? ks0 : ks1));
-          if (ragged && (j * 8 + 2 * c + i >= valid || !(there >> (j >> 1) & 1))) y = -INFINITY;
-          x[2 * j + i] = y;
-          mx = fmaxf(mx, y);
-          mxv = fmaxf(mxv, y + (j < 2 ? ev0 : ev1));
-        }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mxv = fmaxf(mxv, __shfl_xor_sync(0xffffffffu, mxv, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      mxv = fmaxf(mxv, __shfl_xor_sync(0xffffffffu, mxv, 2));
-      const float m1 = fmaxf(m, mx), mv1 = fmaxf(mv, mxv);
-      const float mu = m1 == -INFINITY ? 0.f : m1, mvu = mv1 == -INFINITY ? 0.f : mv1;
-      l *= ex2(m - mu);
-      const float alpha = ex2(mv - mvu);
-      if (__any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) { o[i][0] *= alpha; o[i][1] *= alpha; o[i][2] *= alpha; o[i][3] *= alpha; }
-      }
-      m = m1; mv = mv1;
-      float p[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float y = x[2 * j + i];
-          l += ex2(y - mu);
-          float pv = ex2(y + (j < 2 ? ev0 : ev1) - mvu) * (j < 2 ? fv0 : fv1);
-          if (y == -INFINITY) pv = 0.f;              // a group outside the pool leaves its scales unset
-          p[2 * j + i] = pv;
-        }
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
-        uint32_t pa[4];
-        split2(p[4 * kk], p[4 * kk + 1], pa[0], pa[1]);
-        split2(p[4 * kk + 2], p[4 * kk + 3], pa[2], pa[3]);
-        constexpr int W = D / 32;                    // 32-bit words a lane reads of a row: D / 8 bytes at column g
+        constexpr int W = D / 32;                    // 32-bit words a lane reads of a row
         uint32_t v[4][W];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -338,60 +347,65 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
             const uint2 y = *(const uint2*)(vt + r * D + (((g >> 1) ^ ((r >> 1) & 3)) * 16) + (g & 1) * 8);
             v[i][0] = y.x; v[i][1] = y.y;
           }
-          if (ragged && (r >= valid || !(there >> kk & 1))) {       // bytes behind the last token may be NaN codes
+        }
+        if (ragged) {                                // bytes behind the last token may be NaN codes
 #pragma unroll
-            for (int j = 0; j < W; ++j) v[i][j] = 0;
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t keep = kk * 16 + 2 * c + (i & 1) + (i >> 1) * 8 < valid && (there >> kk & 1) ? 0xffffffffu : 0u;
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[i][j] &= keep;
           }
         }
 #pragma unroll
         for (int j = 0; j < W; ++j) {
-          const uint32_t a01 = __byte_perm(v[0][j], v[1][j], 0x5140), a23 = __byte_perm(v[0][j], v[1][j], 0x7362);
-          const uint32_t b01 = __byte_perm(v[2][j], v[3][j], 0x5140), b23 = __byte_perm(v[2][j], v[3][j], 0x7362);
-          mma16816(o[4 * j], pa, codes2<E4M3>(a01, false), codes2<E4M3>(b01, false));
-          mma16816(o[4 * j + 1], pa, codes2<E4M3>(a01, true), codes2<E4M3>(b01, true));
-          mma16816(o[4 * j + 2], pa, codes2<E4M3>(a23, false), codes2<E4M3>(b23, false));
-          mma16816(o[4 * j + 3], pa, codes2<E4M3>(a23, true), codes2<E4M3>(b23, true));
+          // bytes 4j .. 4j + 3 of the four rows: pairs of tokens for each output column
+          uint32_t x0, x1, x2, x3, y0, y1, y2, y3;
+          codes4<E4M3>(__byte_perm(v[0][j], v[1][j], 0x5140), x0, x1);
+          codes4<E4M3>(__byte_perm(v[2][j], v[3][j], 0x5140), y0, y1);
+          codes4<E4M3>(__byte_perm(v[0][j], v[1][j], 0x7362), x2, x3);
+          codes4<E4M3>(__byte_perm(v[2][j], v[3][j], 0x7362), y2, y3);
+#pragma unroll
+          for (int t = 0; t < SETS; ++t) {
+            mma16816(o[t][2 * j], x0, x1, y0, y1, pb[t][2 * kk], pb[t][2 * kk + 1]);
+            mma16816(o[t][2 * j + 1], x2, x3, y2, y3, pb[t][2 * kk], pb[t][2 * kk + 1]);
+          }
         }
       }
       __syncwarp();                                  // every lane has read the stage
       if (put.left > 0) fetch(stage);
       if (++stage == S::kStages) { stage = 0; phase ^= 1; }
 
-      const bool last_of_unit = get.tile + 1 == get.tiles;
-      const int tiles = get.tiles;
+      const int tile = get.tile, tiles = get.tiles, left = get.left;
       get.advance(a);
-      if (last_of_unit || get.left <= 0) {           // the unit, or this warp's part of it, is done
-        float lt = l + __shfl_xor_sync(0xffffffffu, l, 1);
-        lt += __shfl_xor_sync(0xffffffffu, lt, 2);
-        const bool row = g0 + g < a.G;
-        const float back = lt == 0.f ? 0.f : ex2(mv - m);           // o is held relative to the maximum of p s_V, l to that of p
-        if (whole && last_of_unit) {
-          const float r = lt == 0.f ? 0.f : back / lt;
-          const long long oi = ((long long)n * a.H * a.G + h * a.G + g0 + g) * D + c * (D / 4);
-          if (row) {
+      if (tile + 1 == tiles || left == 1) {          // the unit, or this warp's part of it, is done
+        // a worker has at most two parts: of the unit at its start (slot 0), and of one that begins inside it (slot 1)
+        const bool done = whole && tile + 1 == tiles;
+        const int sl = worker * 2 + (first ? 0 : 1);
 #pragma unroll
-            for (int i = 0; i < NT; i += 2) store_out(a, oi + i, (o[i][0] + o[i][2]) * r, (o[i + 1][0] + o[i + 1][2]) * r);
+        for (int t = 0; t < SETS; ++t) {
+          float lt = l[t];
 #pragma unroll
-            for (int i = 0; i < NT; i += 2) store_out(a, oi + NT + i, (o[i][1] + o[i][3]) * r, (o[i + 1][1] + o[i + 1][3]) * r);
-          }
-        } else {
-          // a worker has at most two parts: of the unit at its start (slot 0), and of one that begins inside it (slot 1)
-          const int sl = worker * 2 + (first ? 0 : 1);
-          if (row) {
-            float* dst = a.part + ((long long)sl * a.rows + g) * D + c * (D / 4);
+          for (int d = 4; d < 32; d <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, d);
+          // o is held relative to the maximum of p s_V, l to that of p
+          const float back = lt == 0.f ? 0.f : ex2(mv[t] - m[t]), r = done ? (lt == 0.f ? 0.f : back / lt) : back;
+          const int row = t * 4 + c;                 // this lane: query head c of the set, output columns DL g ...
+          if (g0 + row >= a.G) continue;
+          if (done) {
+            const long long oi = ((long long)n * a.H * a.G + h * a.G + g0 + row) * D + g * DL;
 #pragma unroll
-            for (int i = 0; i < NT; i += 2) {
-              *(float2*)(dst + i) = make_float2((o[i][0] + o[i][2]) * back, (o[i + 1][0] + o[i + 1][2]) * back);
-              *(float2*)(dst + NT + i) = make_float2((o[i][1] + o[i][3]) * back, (o[i + 1][1] + o[i + 1][3]) * back);
-            }
-            if (c == 0) *(float2*)(a.part_ml + ((long long)sl * a.rows + g) * 2) = make_float2(m, lt);
+            for (int i = 0; i < MT; ++i) store_out(a, oi + 2 * i, (o[t][i][0] + o[t][i][1]) * r, (o[t][i][2] + o[t][i][3]) * r);
+          } else {
+            float* dst = a.part + ((long long)sl * a.rows + row) * D + g * DL;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) *(float2*)(dst + 2 * i) = make_float2((o[t][i][0] + o[t][i][1]) * r, (o[t][i][2] + o[t][i][3]) * r);
+            if (g == 0) *(float2*)(a.part_ml + ((long long)sl * a.rows + row) * 2) = make_float2(m[t], lt);
           }
-          if (whole) {                               // begins here, goes on: this worker's unit to join
-            const long long last = unit_tile0 + tiles - 1;
-            found = make_int4(n, unit, sl, (int)(last * nw / total));   // the last worker, but for the rounding down of the ranges
-            while (total * (found.w + 1) / nw <= last) ++found.w;
-            while (total * found.w / nw > last) --found.w;
-          }
+        }
+        if (whole && !done) {                        // begins here, goes on: this worker's unit to join
+          const long long last = end - left - tile + tiles - 1;
+          found = make_int4(n, h * a.QG + g0 / (4 * SETS), sl, (int)(last * nw / total));   // the last worker, but for the rounding down
+          while (total * (found.w + 1) / nw <= last) ++found.w;
+          while (total * found.w / nw > last) --found.w;
         }
         fresh = true;
         first = false;
@@ -405,44 +419,80 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
   if (lane == 0) a.desc[worker] = found;
 }
 
-// Joins the parts of the unit that begins in worker blockIdx.x: parts in order, weights 2^(m_i - m).
-template <int D> __global__ void __launch_bounds__(128) kv8_join_kernel(KvAttnArgs a) {
+// Joins the parts of the unit that begins in worker blockIdx.x: warps take parts in turn and carry (m, l, o), then warp 0 joins the
+// warps in order.
+constexpr int kJoinWarps = 8;
+template <int D, int SETS> __global__ void __launch_bounds__(kJoinWarps * 32) kv8_join_kernel(KvAttnArgs a) {
+  constexpr int C = D / 32;                          // columns a lane
+  __shared__ float s_o[kJoinWarps][D], s_m[kJoinWarps], s_l[kJoinWarps];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 d = a.desc[blockIdx.x];
   if (d.x < 0) return;
-  const int w0 = blockIdx.x, w1 = min(d.w, a.NW - 1), h = d.y / a.QG, g0 = (d.y - h * a.QG) * 8;
-  constexpr int TPR = D / 2, ROWS = 128 / TPR;       // two columns a thread
-  const int col = (threadIdx.x % TPR) * 2;
-  for (int g = threadIdx.x / TPR; g < 8 && g0 + g < a.G; g += ROWS) {
-    float m = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
-    for (int i = w0; i <= w1; ++i) {
-      const long long sl = (long long)(i == w0 ? d.z : 2 * i) * a.rows + g;
+  const int w0 = blockIdx.x, parts = min(d.w, a.NW - 1) - w0 + 1, h = d.y / a.QG, g0 = (d.y - h * a.QG) * 4 * SETS;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  for (int row = blockIdx.y; row < 4 * SETS && g0 + row < a.G; row += gridDim.y) {
+    float m = -INFINITY, l = 0.f, o[C] = {};
+#pragma unroll 4
+    for (int i = w; i < parts; i += kJoinWarps) {
+      const long long sl = (long long)(i == 0 ? d.z : 2 * (w0 + i)) * a.rows + row;
       const float2 ml = *(const float2*)(a.part_ml + sl * 2);
-      const float2 v = *(const float2*)(a.part + sl * D + col);
+      float v[C];
+      if (C == 4) { const float4 x = *(const float4*)(a.part + sl * D + lane * 4); v[0] = x.x; v[1] = x.y; v[C - 2] = x.z; v[C - 1] = x.w; }
+      else { const float2 x = *(const float2*)(a.part + sl * D + lane * 2); v[0] = x.x; v[1] = x.y; }
       const float m1 = fmaxf(m, ml.x), mu = m1 == -INFINITY ? 0.f : m1;
       const float p = ex2(m - mu), r = ex2(ml.x - mu);
       l = l * p + ml.y * r;
-      x = x * p + v.x * r;
-      y = y * p + v.y * r;
+#pragma unroll
+      for (int j = 0; j < C; ++j) o[j] = o[j] * p + v[j] * r;
       m = m1;
     }
-    const float r = l == 0.f ? 0.f : 1.f / l;
-    store_out(a, ((long long)d.x * a.H * a.G + h * a.G + g0 + g) * D + col, x * r, y * r);
+#pragma unroll
+    for (int j = 0; j < C; ++j) s_o[w][lane * C + j] = o[j];
+    if (lane == 0) { s_m[w] = m; s_l[w] = l; }
+    __syncthreads();
+    if (w == 0) {
+      for (int i = 1; i < min(parts, kJoinWarps); ++i) {
+        const float m1 = fmaxf(m, s_m[i]), mu = m1 == -INFINITY ? 0.f : m1;
+        const float p = ex2(m - mu), r = ex2(s_m[i] - mu);
+        l = l * p + s_l[i] * r;
+#pragma unroll
+        for (int j = 0; j < C; ++j) o[j] = o[j] * p + s_o[i][lane * C + j] * r;
+        m = m1;
+      }
+      const float r = l == 0.f ? 0.f : 1.f / l;
+      const long long oi = ((long long)d.x * a.H * a.G + h * a.G + g0 + row) * D + lane * C;
+#pragma unroll
+      for (int j = 0; j < C; j += 2) store_out(a, oi + j, o[j] * r, o[j + 1] * r);
+    }
+    __syncthreads();
   }
 }
 
-template <int D, int E4M3> int launch_kv8_attention(const KvAttnArgs& a, const CUtensorMap& map, int grid, cudaStream_t st) {
+template <int D, int E4M3, int SETS> int launch_sets(const KvAttnArgs& a, const CUtensorMap& map, int grid, cudaStream_t st) {
   using S = KvShape<D>;
   static bool set[16] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 16 || !set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kv8_attention_kernel<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(kv8_attention_kernel<D, E4M3, SETS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return (int)e;
     if (dev >= 0 && dev < 16) set[dev] = true;
   }
-  kv8_attention_kernel<D, E4M3><<<grid, kThreads, S::kSmem, st>>>(map, a);
-  kv8_join_kernel<D><<<a.NW, 128, 0, st>>>(a);
-  return (int)cudaGetLastError();
+  kv8_attention_kernel<D, E4M3, SETS><<<grid, kThreads, S::kSmem, st>>>(map, a);
+  // the joining kernel is launched while the first one runs and waits for its end on the device
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.NW, (unsigned)a.rows);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, kv8_join_kernel<D, SETS>, a);
+}
+template <int D, int E4M3> int launch_kv8_attention(const KvAttnArgs& a, const CUtensorMap& map, int grid, cudaStream_t st) {
+  return a.G <= 4 ? launch_sets<D, E4M3, 1>(a, map, grid, st) : launch_sets<D, E4M3, 2>(a, map, grid, st);
 }
 }  // namespace hippo
 
@@ -478,7 +528,7 @@ extern "C" int hippo_kv8_attention(const KvAttendCall* c) {
   const int G = c->Hq / c->H, rows = G < 8 ? G : 8;
   const long long parts = 2ll * c->workers * rows;
   KvAttnArgs a{c->q, c->out, c->q_n, c->q_h, c->scales, c->blocks * c->H, c->table, c->table_ld, c->M, c->lens, c->N, c->H, G,
-               (G + 7) / 8, sh, (int)c->blocks, c->dtype, half_rows, c->scale, c->ws, c->ws + parts * D,
+               G <= 4 ? 1 : (G + 7) / 8, sh, (int)c->blocks, c->dtype, half_rows, c->scale, c->ws, c->ws + parts * D,
                (int4*)(c->ws + parts * (D + 2)), c->workers, rows};
   cudaStream_t st = (cudaStream_t)c->stream;
   const int grid = c->workers / kWarps;
