@@ -3,7 +3,8 @@
 //
 // Bound by HBM: a token and kv head costs 2 D bytes of codes, read once for the query heads that share the kv head (up to 8 of them
 // together). Work is cut in tiles of 32 tokens; the tiles of all (sequence, kv head, group of query heads) form one list that is
-// divided evenly over all warps of one resident wave, whatever the lengths. A warp streams its tiles through its own TMA ring (no
+// divided evenly over all warps of one resident wave, whatever the lengths (the start of a unit counts as one more tile: its query
+// rows and its result cost about as much). A warp streams its tiles through its own TMA ring (no
 // block-wide barrier in the loop) and carries the running maximum and sum; a unit that spans several warps leaves partial (m, l, o)
 // rows that a second, small kernel joins in a fixed order, so results do not depend on timing.
 //
@@ -91,11 +92,11 @@ __device__ __forceinline__ int cached_len(const KvAttnArgs& a, int n) {
 
 // Where a warp stands in the list of tiles: sequence, kv head, group of query heads, tile.
 struct Cursor {
-  int n, h, grp, tile, len, tiles, left;             // left: tiles of the warp's range that are still ahead, this one included
+  int n, h, grp, tile, len, tiles, left;             // left: places of the warp's range that are still ahead, this tile's included
   __device__ void advance(const KvAttnArgs& a) {
     if (--left <= 0 || ++tile < tiles) return;
     tile = 0;
-    if (++grp < a.QG) return;
+    if (--left <= 0 || ++grp < a.QG) return;         // the next unit's first place has no tile
     grp = 0;
     if (++h < a.H) return;
     h = 0;
@@ -124,10 +125,13 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
     if (a.lens[n] <= 0)
       for (int i = tid; i < a.H * a.G * (D / 2); i += kThreads) store_out(a, (long long)n * a.H * a.G * D + i * 2, 0.f, 0.f);
 
-  // tiles before every thread's share of the sequences
+  // places before every thread's share of the sequences: a unit has one more than tiles
   const int share = (a.N + kThreads - 1) / kThreads;
   long long mine = 0;
-  for (int n = tid * share; n < min(a.N, (tid + 1) * share); ++n) mine += (long long)((cached_len(a, n) + kTile - 1) / kTile) * units;
+  for (int n = tid * share; n < min(a.N, (tid + 1) * share); ++n) {
+    const int len = cached_len(a, n);
+    if (len > 0) mine += (long long)((len + kTile - 1) / kTile + 1) * units;
+  }
   long long inc = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -147,9 +151,11 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
   __syncthreads();
   const long long total = s_pre[kThreads];
 
-  // no more workers than tiles: every part between a unit's first and last worker is then written
-  const int worker = blockIdx.x * kWarps + w, nw = (int)min((long long)a.NW, total);
-  const long long begin = worker < nw ? total * worker / nw : 0, end = worker < nw ? total * (worker + 1) / nw : 0;
+  // no more workers than half the places: each has two at least, so one tile or more of every unit between its ends
+  const int worker = blockIdx.x * kWarps + w, nw = (int)min((long long)a.NW, total >> 1);
+  const long long each = nw ? total / nw : 0, odd = total - each * nw;         // the first `odd` workers have one place more
+  const long long begin = worker < nw ? each * worker + min((long long)worker, odd) : 0;
+  const long long end = worker < nw ? begin + each + (worker < odd) : 0;
   int4 found = make_int4(-1, 0, 0, 0);               // unit that begins here and ends in a later worker
   uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023) + w * S::kWarpBytes;
 
@@ -163,16 +169,17 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
       for (;;) {                                     // the sequence of the share that holds `begin`
         put.len = cached_len(a, n);
         put.tiles = (put.len + kTile - 1) / kTile;
-        const long long c = (long long)put.tiles * units;
+        const long long c = put.len > 0 ? (long long)(put.tiles + 1) * units : 0;
         if (at + c > begin) break;
         at += c; ++n;
       }
       put.n = n;
-      const int unit = (int)((begin - at) / put.tiles);
-      put.tile = (int)((begin - at) - (long long)unit * put.tiles);
+      const int unit = (int)((begin - at) / (put.tiles + 1));
+      put.tile = (int)((begin - at) - (long long)unit * (put.tiles + 1)) - 1;
+      put.left = (int)(end - begin);
+      if (put.tile < 0) { put.tile = 0; --put.left; }
       put.h = unit / a.QG;
       put.grp = unit - put.h * a.QG;
-      put.left = (int)(end - begin);
     }
     Cursor get = put;
     // fetching: lanes hold 32 entries of the table row
@@ -377,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
 
       const int tile = get.tile, tiles = get.tiles, left = get.left;
       get.advance(a);
-      if (tile + 1 == tiles || left == 1) {          // the unit, or this warp's part of it, is done
+      if (tile + 1 == tiles || get.left <= 0) {      // the unit, or this warp's part of it, is done
         // a worker has at most two parts: of the unit at its start (slot 0), and of one that begins inside it (slot 1)
         const bool done = whole && tile + 1 == tiles;
         const int sl = worker * 2 + (first ? 0 : 1);
@@ -402,10 +409,8 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
           }
         }
         if (whole && !done) {                        // begins here, goes on: this worker's unit to join
-          const long long last = end - left - tile + tiles - 1;
-          found = make_int4(n, h * a.QG + g0 / (4 * SETS), sl, (int)(last * nw / total));   // the last worker, but for the rounding down
-          while (total * (found.w + 1) / nw <= last) ++found.w;
-          while (total * found.w / nw > last) --found.w;
+          const long long last = end - left - tile + tiles - 1, wide = (each + 1) * odd;     // place of its last tile
+          found = make_int4(n, h * a.QG + g0 / (4 * SETS), sl, (int)(last < wide ? last / (each + 1) : odd + (last - wide) / each));
         }
         fresh = true;
         first = false;
@@ -419,8 +424,8 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
   if (lane == 0) a.desc[worker] = found;
 }
 
-// Joins the parts of the unit that begins in worker blockIdx.x: warps take parts in turn and carry (m, l, o), then warp 0 joins the
-// warps in order.
+// Joins the parts of the unit that begins in worker blockIdx.x, a query row at a time: the maximum over all parts first, then their
+// sums with weights 2^(m_i - m), every warp over its share of the parts (independent loads) and warp 0 over the warps, in order.
 constexpr int kJoinWarps = 8;
 template <int D, int SETS> __global__ void __launch_bounds__(kJoinWarps * 32) kv8_join_kernel(KvAttnArgs a) {
   constexpr int C = D / 32;                          // columns a lane
@@ -431,33 +436,41 @@ template <int D, int SETS> __global__ void __launch_bounds__(kJoinWarps * 32) kv
   const int w0 = blockIdx.x, parts = min(d.w, a.NW - 1) - w0 + 1, h = d.y / a.QG, g0 = (d.y - h * a.QG) * 4 * SETS;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   for (int row = blockIdx.y; row < 4 * SETS && g0 + row < a.G; row += gridDim.y) {
-    float m = -INFINITY, l = 0.f, o[C] = {};
-#pragma unroll 4
-    for (int i = w; i < parts; i += kJoinWarps) {
-      const long long sl = (long long)(i == 0 ? d.z : 2 * (w0 + i)) * a.rows + row;
-      const float2 ml = *(const float2*)(a.part_ml + sl * 2);
-      float v[C];
-      if (C == 4) { const float4 x = *(const float4*)(a.part + sl * D + lane * 4); v[0] = x.x; v[1] = x.y; v[C - 2] = x.z; v[C - 1] = x.w; }
-      else { const float2 x = *(const float2*)(a.part + sl * D + lane * 2); v[0] = x.x; v[1] = x.y; }
-      const float m1 = fmaxf(m, ml.x), mu = m1 == -INFINITY ? 0.f : m1;
-      const float p = ex2(m - mu), r = ex2(ml.x - mu);
-      l = l * p + ml.y * r;
+    auto slot = [&](int i) { return (long long)(i == 0 ? d.z : 2 * (w0 + i)) * a.rows + row; };
+    float m = -INFINITY;
+    for (int i = threadIdx.x; i < parts; i += kJoinWarps * 32) m = fmaxf(m, a.part_ml[slot(i) * 2]);
 #pragma unroll
-      for (int j = 0; j < C; ++j) o[j] = o[j] * p + v[j] * r;
-      m = m1;
+    for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    if (lane == 0) s_m[w] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i) m = fmaxf(m, s_m[i]);
+    if (m == -INFINITY) m = 0.f;
+    float l = 0.f, o[C] = {};
+#pragma unroll 8
+    for (int i = w; i < parts; i += kJoinWarps) {
+      const long long sl = slot(i);
+      const float2 ml = *(const float2*)(a.part_ml + sl * 2);
+      const float r = ex2(ml.x - m);
+      l += ml.y * r;
+      if (C == 4) {
+        const float4 x = *(const float4*)(a.part + sl * D + lane * 4);
+        o[0] += x.x * r; o[1] += x.y * r; o[C - 2] += x.z * r; o[C - 1] += x.w * r;
+      } else {
+        const float2 x = *(const float2*)(a.part + sl * D + lane * 2);
+        o[0] += x.x * r; o[1] += x.y * r;
+      }
     }
 #pragma unroll
     for (int j = 0; j < C; ++j) s_o[w][lane * C + j] = o[j];
-    if (lane == 0) { s_m[w] = m; s_l[w] = l; }
+    if (lane == 0) s_l[w] = l;
     __syncthreads();
     if (w == 0) {
-      for (int i = 1; i < min(parts, kJoinWarps); ++i) {
-        const float m1 = fmaxf(m, s_m[i]), mu = m1 == -INFINITY ? 0.f : m1;
-        const float p = ex2(m - mu), r = ex2(s_m[i] - mu);
-        l = l * p + s_l[i] * r;
 #pragma unroll
-        for (int j = 0; j < C; ++j) o[j] = o[j] * p + s_o[i][lane * C + j] * r;
-        m = m1;
+      for (int i = 1; i < kJoinWarps; ++i) {
+        l += s_l[i];
+#pragma unroll
+        for (int j = 0; j < C; ++j) o[j] += s_o[i][lane * C + j];
       }
       const float r = l == 0.f ? 0.f : 1.f / l;
       const long long oi = ((long long)d.x * a.H * a.G + h * a.G + g0 + row) * D + lane * C;
