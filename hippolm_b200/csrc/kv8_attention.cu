@@ -75,10 +75,30 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *(const uint32_t*)&h;
 }
 
-__device__ __forceinline__ float load_q(const KvAttnArgs& a, long long i) {
-  if (a.dtype == 0) return __bfloat162float(((const __nv_bfloat16*)a.q)[i]);
-  if (a.dtype == 1) return __half2float(((const __half*)a.q)[i]);
-  return ((const float*)a.q)[i];
+// N consecutive query values (16-byte aligned) as fp32
+template <int N> __device__ __forceinline__ void load_q(const KvAttnArgs& a, long long i, float (&x)[N]) {
+  if (a.dtype == 2) {
+    const float4* p = (const float4*)((const float*)a.q + i);
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+      const float4 v = __ldg(p + j);
+      x[4 * j] = v.x; x[4 * j + 1] = v.y; x[4 * j + 2] = v.z; x[4 * j + 3] = v.w;
+    }
+    return;
+  }
+  uint4 v[N / 8];
+#pragma unroll
+  for (int j = 0; j < N / 8; ++j) v[j] = __ldg((const uint4*)((const __half*)a.q + i) + j);
+#pragma unroll
+  for (int j = 0; j < N / 8; ++j) {
+    const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = a.dtype == 0 ? make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u))
+                                    : __half22float2(*(const __half2*)&w[k]);
+      x[8 * j + 2 * k] = f.x; x[8 * j + 2 * k + 1] = f.y;
+    }
+  }
 }
 __device__ __forceinline__ void store_out(const KvAttnArgs& a, long long i, float x, float y) {      // elements i, i + 1
   if (a.dtype == 0) ((__nv_bfloat162*)a.out)[i >> 1] = __floats2bfloat162_rn(x, y);
@@ -114,8 +134,8 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
   __shared__ uint64_t full[kWarps][S::kStages];
   __shared__ float4 s_scale[kWarps][S::kStages];     // K, V scale of the tile's first 16 tokens, K, V of the others
   __shared__ int s_there[kWarps][S::kStages];        // which 16-token groups of the tile lie in a block of the pool
-  __shared__ long long s_pre[kThreads + 1];
-  __shared__ long long s_warp[kWarps];
+  __shared__ int s_pre[kThreads + 1];
+  __shared__ int s_warp[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int units = a.H * a.QG;
   asm volatile("griddepcontrol.launch_dependents;");
@@ -127,15 +147,15 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
 
   // places before every thread's share of the sequences: a unit has one more than tiles
   const int share = (a.N + kThreads - 1) / kThreads;
-  long long mine = 0;
+  int mine = 0;                                      // (the host has seen to it that all places are below 2^31)
   for (int n = tid * share; n < min(a.N, (tid + 1) * share); ++n) {
     const int len = cached_len(a, n);
-    if (len > 0) mine += (long long)((len + kTile - 1) / kTile + 1) * units;
+    if (len > 0) mine += ((len + kTile - 1) / kTile + 1) * units;
   }
-  long long inc = mine;
+  int inc = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, inc, d);
+    const int y = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += y;
   }
   if (lane == 31) s_warp[w] = inc;
@@ -149,13 +169,13 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
   s_pre[tid + 1] = inc;
   if (tid == 0) s_pre[0] = 0;
   __syncthreads();
-  const long long total = s_pre[kThreads];
+  const int total = s_pre[kThreads];
 
   // no more workers than half the places: each has two at least, so one tile or more of every unit between its ends
-  const int worker = blockIdx.x * kWarps + w, nw = (int)min((long long)a.NW, total >> 1);
-  const long long each = nw ? total / nw : 0, odd = total - each * nw;         // the first `odd` workers have one place more
-  const long long begin = worker < nw ? each * worker + min((long long)worker, odd) : 0;
-  const long long end = worker < nw ? begin + each + (worker < odd) : 0;
+  const int worker = blockIdx.x * kWarps + w, nw = min(a.NW, total >> 1);
+  const int each = nw ? total / nw : 0, odd = total - each * nw;         // the first `odd` workers have one place more
+  const int begin = worker < nw ? each * worker + min(worker, odd) : 0;
+  const int end = worker < nw ? begin + each + (worker < odd) : 0;
   int4 found = make_int4(-1, 0, 0, 0);               // unit that begins here and ends in a later worker
   uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023) + w * S::kWarpBytes;
 
@@ -164,19 +184,19 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
     {
       int lo = 0, hi = kThreads - 1;
       while (lo < hi) { const int mid = (lo + hi) >> 1; if (s_pre[mid + 1] > begin) hi = mid; else lo = mid + 1; }
-      long long at = s_pre[lo];
+      int at = s_pre[lo];
       int n = lo * share;
       for (;;) {                                     // the sequence of the share that holds `begin`
         put.len = cached_len(a, n);
         put.tiles = (put.len + kTile - 1) / kTile;
-        const long long c = put.len > 0 ? (long long)(put.tiles + 1) * units : 0;
+        const int c = put.len > 0 ? (put.tiles + 1) * units : 0;
         if (at + c > begin) break;
         at += c; ++n;
       }
       put.n = n;
-      const int unit = (int)((begin - at) / (put.tiles + 1));
-      put.tile = (int)((begin - at) - (long long)unit * (put.tiles + 1)) - 1;
-      put.left = (int)(end - begin);
+      const int unit = (begin - at) / (put.tiles + 1);
+      put.tile = begin - at - unit * (put.tiles + 1) - 1;
+      put.left = end - begin;
       if (put.tile < 0) { put.tile = 0; --put.left; }
       put.h = unit / a.QG;
       put.grp = unit - put.h * a.QG;
@@ -249,9 +269,8 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
           const int qh = g0 + t * 4 + (g >> 1);      // column g of the query side: head g / 2, its high (even) or low term
           const bool row = qh < a.G;
           const long long qi = (long long)n * a.q_n + (long long)(h * a.G + qh) * a.q_h + c * (D / 4);
-          float x[D / 4], top = 0.f;
-#pragma unroll
-          for (int i = 0; i < D / 4; ++i) x[i] = row ? load_q(a, qi + i) : 0.f;
+          float x[D / 4] = {}, top = 0.f;
+          if (row) load_q(a, qi, x);
 #pragma unroll
           for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -409,8 +428,8 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
           }
         }
         if (whole && !done) {                        // begins here, goes on: this worker's unit to join
-          const long long last = end - left - tile + tiles - 1, wide = (each + 1) * odd;     // place of its last tile
-          found = make_int4(n, h * a.QG + g0 / (4 * SETS), sl, (int)(last < wide ? last / (each + 1) : odd + (last - wide) / each));
+          const int last = end - left - tile + tiles - 1, wide = (each + 1) * odd;     // place of its last tile
+          found = make_int4(n, h * a.QG + g0 / (4 * SETS), sl, last < wide ? last / (each + 1) : odd + (last - wide) / each);
         }
         fresh = true;
         first = false;
@@ -424,17 +443,22 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
   if (lane == 0) a.desc[worker] = found;
 }
 
-// Joins the parts of the unit that begins in worker blockIdx.x, a query row at a time: the maximum over all parts first, then their
+// Joins the parts of the units that begin in the workers of a block of the first kernel, a query row at a time: the maximum over all parts first, then their
 // sums with weights 2^(m_i - m), every warp over its share of the parts (independent loads) and warp 0 over the warps, in order.
 constexpr int kJoinWarps = 8;
 template <int D, int SETS> __global__ void __launch_bounds__(kJoinWarps * 32) kv8_join_kernel(KvAttnArgs a) {
   constexpr int C = D / 32;                          // columns a lane
   __shared__ float s_o[kJoinWarps][D], s_m[kJoinWarps], s_l[kJoinWarps];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 d = a.desc[blockIdx.x];
-  if (d.x < 0) return;
-  const int w0 = blockIdx.x, parts = min(d.w, a.NW - 1) - w0 + 1, h = d.y / a.QG, g0 = (d.y - h * a.QG) * 4 * SETS;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int4 all[kWarps];
+#pragma unroll
+  for (int k = 0; k < kWarps; ++k) all[k] = a.desc[blockIdx.x * kWarps + k];
+#pragma unroll 1
+  for (int k = 0; k < kWarps; ++k) {
+  const int4 d = k == 0 ? all[0] : k == 1 ? all[1] : k == 2 ? all[2] : all[3];
+  if (d.x < 0) continue;
+  const int w0 = blockIdx.x * kWarps + k, parts = min(d.w, a.NW - 1) - w0 + 1, h = d.y / a.QG, g0 = (d.y - h * a.QG) * 4 * SETS;
   for (int row = blockIdx.y; row < 4 * SETS && g0 + row < a.G; row += gridDim.y) {
     auto slot = [&](int i) { return (long long)(i == 0 ? d.z : 2 * (w0 + i)) * a.rows + row; };
     float m = -INFINITY;
@@ -479,6 +503,7 @@ template <int D, int SETS> __global__ void __launch_bounds__(kJoinWarps * 32) kv
     }
     __syncthreads();
   }
+  }
 }
 
 template <int D, int E4M3, int SETS> int launch_sets(const KvAttnArgs& a, const CUtensorMap& map, int grid, cudaStream_t st) {
@@ -494,7 +519,7 @@ template <int D, int E4M3, int SETS> int launch_sets(const KvAttnArgs& a, const 
   kv8_attention_kernel<D, E4M3, SETS><<<grid, kThreads, S::kSmem, st>>>(map, a);
   // the joining kernel is launched while the first one runs and waits for its end on the device
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.NW, (unsigned)a.rows);
+  cfg.gridDim = dim3((unsigned)grid, (unsigned)a.rows);
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -528,6 +553,9 @@ extern "C" int hippo_kv8_attention(const KvAttendCall* c) {
   const int D = c->D;
   const long long half_rows = (c->blocks * c->H) << sh;
   if (2 * half_rows > 0x7fffffffll) return -2;       // TMA coordinates are 32-bit
+  const long long groups = (long long)c->N * c->H * ((c->Hq / c->H + 7) / 8);
+  if (groups * ((((long long)c->M << sh) + kTile - 1) / kTile + 1) > 0x7fffffffll) return -3;
+  if (((uintptr_t)c->q & 15) || c->q_n * (c->dtype == 2 ? 4 : 2) % 16 || c->q_h * (c->dtype == 2 ? 4 : 2) % 16) return -4;
   auto fn = get_encode_fn();
   if (!fn) return -100;
   CUtensorMap map;

@@ -77,18 +77,19 @@ def attention_decode(q, codes, scales, table, lens, scale: float, dev: int):
         raise ValueError(f"head_dim {D}: the CUDA cache supports 64 and 128")
     if 2 * blocks * H * bs >= 1 << 31:
         raise ValueError("the cache has 2^31 rows or more")
-    qn, qh, qd = q.stride()
-    if qd != 1:
-        q = q.contiguous()
-        qn, qh, _ = q.stride()
+    q = _rows(q)
+    qn, qh, _ = q.stride()
     ld, _ = table.stride()
     M = table.shape[1]
     G = Hq // H
+    groups, tiles = N * H * (-(-G // 8)), -(-M * bs // 32)
+    if groups * (tiles + 1) >= 1 << 31:
+        raise ValueError(f"{N} requests of up to {M * bs} tokens and {H} heads: 2^31 tiles of 32 tokens or more")
     sms = _SMS.get(dev)
     if sms is None:
         sms = _SMS[dev] = torch.cuda.get_device_properties(dev).multi_processor_count
     # a warp takes tiles of 32 tokens; three blocks of four warps fill a multiprocessor
-    workers = 4 * min(3 * sms, -(-(N * H * (-(-G // 8)) * (-(-M * bs // 32))) // 4))
+    workers = 4 * min(3 * sms, -(-(groups * tiles) // 4))
     ws = torch.empty(workers * (2 * min(G, 8) * (D + 2) + 4), dtype=torch.float32, device=q.device)
     out = torch.empty((N, Hq, D), dtype=q.dtype, device=q.device)
     launch("kv8_attention", dev, _ATTEND.pack(
