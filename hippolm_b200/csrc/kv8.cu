@@ -165,42 +165,53 @@ __global__ void __launch_bounds__(256) kv8_slots_kernel(
 }
 
 // ------------------------------------------------------------------------------------------------ write
-template <typename T> struct Row8;                   // 8 consecutive values as they are loaded, and as fp32
+// 8 consecutive values as they are loaded, and as fp32. amax() joins their sizes to a running maximum of absolute bits (integer order
+// keeps infinities and NaN on top; two 16-bit fields for the 16-bit types); bits() makes fp32 bits of it.
+template <typename T> struct Row8;
 template <> struct Row8<float> {
   float4 a, b;
   __device__ void load(const float* p) { a = __ldg((const float4*)p); b = __ldg((const float4*)p + 1); }
   __device__ void zero() { a = b = make_float4(0, 0, 0, 0); }
   __device__ void get(float* f) const { f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w; }
+  __device__ uint32_t amax(uint32_t m) const {
+    float f[8];
+    get(f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+    return m;
+  }
+  static __device__ uint32_t bits(uint32_t m) { return m; }
 };
-template <> struct Row8<__nv_bfloat16> {
+struct Row8h {
   uint4 a;
-  __device__ void load(const __nv_bfloat16* p) { a = __ldg((const uint4*)p); }
   __device__ void zero() { a = make_uint4(0, 0, 0, 0); }
+  __device__ uint32_t amax(uint32_t m) const {
+    m = __vmaxu2(m, a.x & 0x7fff7fffu);
+    m = __vmaxu2(m, a.y & 0x7fff7fffu);
+    m = __vmaxu2(m, a.z & 0x7fff7fffu);
+    return __vmaxu2(m, a.w & 0x7fff7fffu);
+  }
+};
+template <> struct Row8<__nv_bfloat16> : Row8h {
+  __device__ void load(const __nv_bfloat16* p) { a = __ldg((const uint4*)p); }
   __device__ void get(float* f) const {
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
   }
+  static __device__ uint32_t bits(uint32_t m) { return max(m & 0xffffu, m >> 16) << 16; }
 };
-template <> struct Row8<__half> {
-  uint4 a;
+template <> struct Row8<__half> : Row8h {
   __device__ void load(const __half* p) { a = __ldg((const uint4*)p); }
-  __device__ void zero() { a = make_uint4(0, 0, 0, 0); }
   __device__ void get(float* f) const {
     const __half2* h = (const __half2*)&a;
 #pragma unroll
     for (int i = 0; i < 4; ++i) { const float2 v = __half22float2(h[i]); f[2 * i] = v.x; f[2 * i + 1] = v.y; }
   }
+  static __device__ uint32_t bits(uint32_t m) {
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16))));
+  }
 };
-
-// largest |x| of the 8 values as bits (integer order keeps infinities and NaN on top)
-template <typename R> __device__ __forceinline__ uint32_t amax_bits(const R& r, uint32_t m) {
-  float f[8];
-  r.get(f);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
-  return m;
-}
 
 // What a run of new tokens does to its (block, head): the exponent of the scale, how far older codes shift, poison.
 struct RunScale { int e, down; bool bad; };
@@ -232,11 +243,9 @@ template <int E4M3> __device__ __forceinline__ void shift_codes(uint8_t* codes, 
 template <int E4M3, typename R> __device__ __forceinline__ uint2 encode_row(const R& r, float inv, bool bad) {
   float f[8];
   r.get(f);
-  uint2 o;
-  uint8_t* c = (uint8_t*)&o;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = bad ? 0 : encode1<E4M3>(f[i] * inv);
-  return o;
+  for (int i = 0; i < 8; ++i) f[i] = bad ? 0.f : f[i] * inv;
+  return encode8<E4M3>(f);
 }
 
 struct WriteArgs {
@@ -295,13 +304,13 @@ __global__ void __launch_bounds__(256) kv8_write_rows_kernel(WriteArgs a) {
     if (r < L) keep[i].load(x + r * ld + col); else keep[i].zero();
   }
 #pragma unroll
-  for (int i = 0; i < U; ++i) m = amax_bits(keep[i], m);
+  for (int i = 0; i < U; ++i) m = keep[i].amax(m);
   for (int r = r0 + U * RPW; r < L; r += RPW) {
     Row8<T> row;
     row.load(x + r * ld + col);
-    m = amax_bits(row, m);
+    m = row.amax(m);
   }
-  m = __reduce_max_sync(0xffffffffu, m);
+  m = __reduce_max_sync(0xffffffffu, Row8<T>::bits(m));
   const RunScale rs = run_scale<E4M3>(m, old, off > 0);
   if (rs.down < 0) shift_codes<E4M3>(codes, off * D, rs.down, lane, 32);
   const float inv = pow2f(-rs.e);
@@ -318,22 +327,24 @@ __global__ void __launch_bounds__(256) kv8_write_rows_kernel(WriteArgs a) {
   if (lane == 0) *scale = rs.bad ? __uint_as_float(0x7fffffffu) : pow2f(rs.e);
 }
 
-// One CTA for the runs that start in a window of bs tokens, of one head and half: the form for prompts. A run (at most bs rows) is
-// read once into registers, reduced over the CTA and stored: HBM-bound, bytes = T * H * D * (element + 1) a half.
+// One CTA for the runs that start in a window of bs tokens, of a group of (head, half) pairs: the form for prompts. The run is found
+// once; then the pairs follow each other, the next one's rows (at most bs) in flight while this one's are reduced over the CTA and
+// stored from registers. HBM-bound, bytes = T * H * D * (element + 1) a half.
+constexpr int kPairs = 8;
 template <typename T, int D, int E4M3, int BS>
 __global__ void __launch_bounds__(128) kv8_write_blocks_kernel(WriteArgs a) {
   constexpr int LPR = D / 8, RPP = 128 / LPR, P = (BS + RPP - 1) / RPP;   // lanes a row, rows a pass, passes
   __shared__ unsigned s_cont[4];                     // bit i: token w0 + i continues the run of the token before it
   __shared__ unsigned s_ok[4];
-  __shared__ uint32_t s_max[4];
+  __shared__ uint32_t s_max[2][4];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const int h = blockIdx.y >> 1, half = blockIdx.y & 1;
+  const int first = blockIdx.y * kPairs, last = min(first + kPairs, 2 * a.H);
   const long long w0 = (long long)blockIdx.x * BS;
   bool ok = false, cont = false;
   if (tid < 2 * BS && w0 + tid < a.T) {
-    const long long s = a.slots[w0 + tid];
+    const long long s = a.slots[w0 + tid], prev = w0 + tid > 0 ? a.slots[w0 + tid - 1] : -1;
     ok = slot_ok(a, s);
-    cont = ok && w0 + tid > 0 && continues(a, a.slots[w0 + tid - 1], s);
+    cont = ok && continues(a, prev, s);
   }
   const unsigned bc = __ballot_sync(0xffffffffu, cont), bo = __ballot_sync(0xffffffffu, ok);
   if (lane == 0) { s_cont[w] = bc; s_ok[w] = bo; }
@@ -342,8 +353,6 @@ __global__ void __launch_bounds__(128) kv8_write_blocks_kernel(WriteArgs a) {
   unsigned long long heads = (s_ok[0] | ((unsigned long long)s_ok[1] << 32)) & ~c0;
   if (BS < 64) heads &= (1ull << (BS & 63)) - 1;
   const int r0 = tid / LPR, col = (tid % LPR) * 8;
-  const T* base = (const T*)(half ? a.v : a.k) + h * (half ? a.v_h : a.k_h) + col;
-  const long long ld = half ? a.v_t : a.k_t;
   for (; heads; heads &= heads - 1) {
     const int i0 = __ffsll(heads) - 1;
     // consecutive "continues" bits behind i0
@@ -351,32 +360,47 @@ __global__ void __launch_bounds__(128) kv8_write_blocks_kernel(WriteArgs a) {
     const int L = min(~rest ? __ffsll(~rest) : 64, BS);
     const long long t = w0 + i0, s = a.slots[t];
     const int off = (int)(s & (BS - 1));
-    const long long bh = (s >> a.sh) * a.H + h;
-    float* scale = a.scales + half * a.half_scales + bh;
-    uint8_t* codes = a.codes + half * a.half_codes + bh * BS * D;
-    const float old = off ? *scale : 0.f;
-    Row8<T> row[P];
-    uint32_t m = 0;
+    const long long block = (s >> a.sh) * a.H;
+    Row8<T> next[P];
+    float next_old = 0.f;
+    auto load = [&](int pair) {
+      const int h = pair >> 1, half = pair & 1;
+      const T* x = (const T*)(half ? a.v : a.k) + t * (half ? a.v_t : a.k_t) + h * (half ? a.v_h : a.k_h) + col;
+      const long long ld = half ? a.v_t : a.k_t;
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const int r = r0 + p * RPP;
-      if (r < L) row[p].load(base + (t + r) * ld); else row[p].zero();
+      for (int p = 0; p < P; ++p) {
+        const int r = r0 + p * RPP;
+        if (r < L) next[p].load(x + r * ld); else next[p].zero();
+      }
+      if (off) next_old = a.scales[half * a.half_scales + block + h];
+    };
+    load(first);
+    for (int pair = first; pair < last; ++pair) {
+      Row8<T> row[P];
+#pragma unroll
+      for (int p = 0; p < P; ++p) row[p] = next[p];
+      const float old = next_old;
+      if (pair + 1 < last) load(pair + 1);
+      const int h = pair >> 1, half = pair & 1;
+      uint8_t* codes = a.codes + half * a.half_codes + (block + h) * BS * D;
+      uint32_t m = 0;
+#pragma unroll
+      for (int p = 0; p < P; ++p) m = row[p].amax(m);
+      m = __reduce_max_sync(0xffffffffu, Row8<T>::bits(m));
+      uint32_t* sm = s_max[pair & 1];                // a warp is at most one pair ahead of the others
+      if (lane == 0) sm[w] = m;
+      __syncthreads();                               // also: every thread has read the old scale
+      m = max(max(sm[0], sm[1]), max(sm[2], sm[3]));
+      const RunScale rs = run_scale<E4M3>(m, old, off > 0);
+      if (rs.down < 0) shift_codes<E4M3>(codes, off * D, rs.down, tid, 128);
+      const float inv = pow2f(-rs.e);
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const int r = r0 + p * RPP;
+        if (r < L) *(uint2*)(codes + (off + r) * D + col) = encode_row<E4M3>(row[p], inv, rs.bad);
+      }
+      if (tid == 0) a.scales[half * a.half_scales + block + h] = rs.bad ? __uint_as_float(0x7fffffffu) : pow2f(rs.e);
     }
-#pragma unroll
-    for (int p = 0; p < P; ++p) m = amax_bits(row[p], m);
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) s_max[w] = m;
-    __syncthreads();                                 // also: every thread has read the old scale
-    m = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
-    const RunScale rs = run_scale<E4M3>(m, old, off > 0);
-    if (rs.down < 0) shift_codes<E4M3>(codes, off * D, rs.down, tid, 128);
-    const float inv = pow2f(-rs.e);
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const int r = r0 + p * RPP;
-      if (r < L) *(uint2*)(codes + (off + r) * D + col) = encode_row<E4M3>(row[p], inv, rs.bad);
-    }
-    if (tid == 0) *scale = rs.bad ? __uint_as_float(0x7fffffffu) : pow2f(rs.e);
     __syncthreads();                                 // s_max is free for the next run
   }
 }
@@ -392,7 +416,7 @@ template <typename T, int D, int E4M3> int launch_write(const WriteArgs& a, int 
     kv8_write_rows_kernel<T, D, E4M3><<<dim3((unsigned)g, 2), 256, 0, st>>>(a);
     return (int)cudaGetLastError();
   }
-  const dim3 grid((unsigned)((a.T + (1 << a.sh) - 1) >> a.sh), (unsigned)(2 * a.H));
+  const dim3 grid((unsigned)((a.T + (1 << a.sh) - 1) >> a.sh), (unsigned)((2 * a.H + kPairs - 1) / kPairs));
   if (a.sh == 4) kv8_write_blocks_kernel<T, D, E4M3, 16><<<grid, 128, 0, st>>>(a);
   else if (a.sh == 5) kv8_write_blocks_kernel<T, D, E4M3, 32><<<grid, 128, 0, st>>>(a);
   else kv8_write_blocks_kernel<T, D, E4M3, 64><<<grid, 128, 0, st>>>(a);

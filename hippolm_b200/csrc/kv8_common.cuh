@@ -23,6 +23,19 @@ template <int E4M3> __device__ __forceinline__ uint8_t encode1(float x) {       
   if (E4M3) return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
   return (uint8_t)(int8_t)__float2int_rn(x);
 }
+// eight values at once: e4m3 two a conversion; int8 by adding 1.5 * 2^23, which leaves the nearest whole number in the low byte
+template <int E4M3> __device__ __forceinline__ uint2 encode8(const float* f) {
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (E4M3) {
+      h[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i], f[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+    } else {
+      h[i] = __byte_perm(__float_as_uint(f[2 * i] + 12582912.f), __float_as_uint(f[2 * i + 1] + 12582912.f), 0x0040);
+    }
+  }
+  return make_uint2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
+}
 template <int E4M3> __device__ __forceinline__ float decode1(uint8_t c) {
   if (E4M3) return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
   return (float)(int8_t)c;

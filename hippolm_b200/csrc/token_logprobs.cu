@@ -3,16 +3,20 @@
 //   l = sum e^(z - m),  logprob = (z_y - m) - log l,  entropy = log l - sum (z - m) e^(z - m) / l      (m: the row's maximum)
 //   dz_v = g_lp (1[v = y] - p_v) - g_H p_v (log p_v + H)
 //
-// Forward is one pass over the logits: a warp takes segments of 512 consecutive logits, the next one in flight while it works; every
-// lane carries its own (m, l, sum) and rescales them when a segment brings a larger maximum. Besides HBM the exponentials are the
-// bound (one a logit: 11.6 of the 16 a clock that a multiprocessor has, at the card's copy rate in 16 bits), so the rest is kept to
-// four instructions a logit: maximum and clamp on packed pairs, sums and products as fp32 pairs. For the alternatives the maximum
-// of every granule (8, 64 or 512 consecutive logits, by the vocabulary) is kept: the k largest logits lie in the k granules that
-// come first by (maximum, lowest index), so only those are read again (from L2). With few rows a cluster of up to 8 CTAs shares a
-// row and joins its parts through distributed shared memory.
+// Forward is one pass over the logits: a warp takes segments of 1024 consecutive logits (512 in fp32), the next one in flight while
+// it works; every lane carries its own (m, l, sum) and rescales them when a segment brings a larger maximum. With 16-bit logits
+// instructions are as near a bound as HBM (an exponential a logit is 11.6 of the 16 a clock that a multiprocessor has, at the
+// card's copy rate), so maximum and clamp work on packed pairs, sums and products on fp32 pairs, and the row's ragged ends have a
+// path of their own. For the alternatives the maximum of every granule (8, 64 or 512 consecutive logits, by the vocabulary) is
+// kept: the k largest logits lie in the k granules that come first by (maximum, lowest index), so only those are read again (from
+// L2). One warp finds the k-th largest maximum bit by bit (a count over its lanes each; 16-bit logits have 16 or 19 bits to
+// find). With few rows a cluster of up to 8 blocks shares a row and joins its parts through distributed shared memory. (Blocks that
+// stay, with a warp of their own for the alternatives of the row before, were slower: 359 against 242 us for 4096 x 128256 and
+// k = 20, as that warp shares its multiprocessor's issue slots.)
 // The backward pass reads the logits once more and writes their gradient: HBM-bound.
 // The reference computes losses only (fla/modules/fused_linear_cross_entropy.py:516-679); it has no per-token scores.
 #include <cooperative_groups.h>
+#include <type_traits>
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include "sm100.cuh"
@@ -21,7 +25,7 @@
 namespace cg = cooperative_groups;
 
 namespace hippo {
-constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kSeg = 512;
+constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;          // at most; a row of few segments gets fewer
 constexpr int kMaxGranules = 1024, kCand = 1024, kMaxTop = 32;
 constexpr float kL2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -45,6 +49,8 @@ __device__ __forceinline__ int order_key(float x) {
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+
+__device__ __forceinline__ float key_value(int k) { return __int_as_float(k < 0 ? k ^ 0x7fffffff : k); }
 
 // 8 consecutive logits as they are loaded. max(): the largest, NaN if there is one. clamp(lo): what is below lo (far below the
 // maximum: its exponential is 0) or NaN becomes lo. kLow: maxima above it leave room for such a lo.
@@ -149,221 +155,317 @@ template <typename T> __device__ __forceinline__ void load_vec(const T* base, in
     if (v + i >= skew && v + i < skew + V) x.set(i, base[v + i]);
 }
 
+// Joins NV vectors with maximum mx (NaN if one is NaN) to a lane's statistics.
+template <typename T, int NV> __device__ __forceinline__ void lp_add(LpStat& st, Vec8<T> (&x)[NV], float mx) {
+  if (mx > st.m || mx != mx) {
+    const float d = (st.m - mx) * kL2e, p = lp_ex2(d);
+    st.m = mx;
+    st.s = p == 0.f ? 0.f : p * (st.s + d * st.l);
+    st.l *= p;
+  }
+  if (!(st.m > Vec8<T>::kLow)) {                     // masked by the type's lowest values, or nothing yet, or NaN: one at a time
+    if (st.m == -INFINITY) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float f[8];
+      x[i].get(f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = fmaxf((f[j] - st.m) * kL2e, -200.f), p = lp_ex2(d);
+        st.l += p;
+        st.s += p * d;
+      }
+    }
+    return;
+  }
+  // below the clamp (z - m) log2(e) stays finite and its exponential is 0 all the same
+  const float lo = st.m - fmaxf(104.f, fabsf(st.m) * 0.015625f);
+  const uint64_t off = pack(-st.m, -st.m), l2e = pack(kL2e, kL2e);
+  uint64_t l2[2] = {0, 0}, s2[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    x[i].clamp(lo);
+    float f[8];
+    x[i].get(f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint64_t d = mul2(add2(pack(f[2 * j], f[2 * j + 1]), off), l2e);
+      float d0, d1;
+      unpack(d, d0, d1);
+      const uint64_t p = pack(lp_ex2(d0), lp_ex2(d1));
+      l2[j & 1] = add2(l2[j & 1], p);
+      s2[j & 1] = fma2(p, d, s2[j & 1]);
+    }
+  }
+  float u, v;
+  unpack(add2(l2[0], l2[1]), u, v);
+  st.l += u + v;
+  unpack(add2(s2[0], s2[1]), u, v);
+  st.s += u + v;
+}
+
 // candidates are ordered by (value, lowest index) as one whole number
 __device__ __forceinline__ unsigned long long cand_of(int key, int index) {
   return ((unsigned long long)((unsigned)key ^ 0x80000000u) << 32) | (0xffffffffu - (unsigned)index);
 }
 __device__ __forceinline__ unsigned cand_index(unsigned long long c) { return 0xffffffffu - (unsigned)c; }
 
-// GR: logits a granule (0: no alternatives are asked for)
-template <typename T, int GR>
-__global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(LpArgs a) {
-  cg::cluster_group cl = cg::this_cluster();
-  const int part = (int)cl.block_rank(), parts = (int)cl.num_blocks();
-  const long long row = blockIdx.x / parts;
-  __shared__ int s_gran[GR ? kMaxGranules : 1];      // order keys of the granules' maxima (of all parts, in part 0)
-  __shared__ LpStat s_stat[kLpWarps], s_part[8];
-  __shared__ int s_pick[kMaxTop];
-  __shared__ unsigned long long s_cand[GR ? kCand : 1];
-  __shared__ int s_n, s_floor;
-  __shared__ float2 s_ml;
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const T* z = (const T*)a.z + row * a.ld;
-  const int skew = (int)(((uintptr_t)z & 15) / sizeof(T));
-  const T* base = z - skew;
-  const int span = skew + a.V, segs = (span + kSeg - 1) / kSeg;
-  int* gran0 = GR ? cl.map_shared_rank(s_gran, 0) : nullptr;
-  if (parts > 1) cl.sync();                          // part 0 runs: its shared memory may be written
+// A row of logits as its readers see it.
+template <typename T> struct LpRow {
+  const T *z, *base;
+  int skew, span, segs, inner0, inner1;              // segments; those from inner0 up to inner1 lie inside the row
+  static constexpr int NV = sizeof(T) == 2 ? 4 : 2, kSeg = NV * 256;       // vectors a lane, logits a segment
+  __device__ LpRow(const LpArgs& a, long long row) {
+    z = (const T*)a.z + row * a.ld;
+    skew = (int)(((uintptr_t)z & 15) / sizeof(T));
+    base = z - skew;
+    span = skew + a.V;
+    segs = (span + kSeg - 1) / kSeg;
+    inner0 = skew ? 1 : 0;
+    inner1 = span / kSeg;
+  }
+  __device__ void load(int g, Vec8<T> (&x)[NV]) const {
+    const int v = g * kSeg + (threadIdx.x & 31) * 8;
+    if (g >= inner0 && g < inner1) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) x[i].load(base + v + i * 256);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) load_vec(base, skew, span - skew, v + i * 256, x[i]);
+    }
+  }
+};
 
-  LpStat st{-INFINITY, 0.f, 0.f};
-  const int step = parts * kLpWarps;
-  int g = part * kLpWarps + w;
-  Vec8<T> next[2];
-  if (g < segs) {
+// One segment: statistics of the lane, keys of the granules' maxima. GR: logits a granule (0: no alternatives are asked for).
+template <typename T, int GR> __device__ __forceinline__ void lp_segment(const LpRow<T>& r, int g, Vec8<T> (&x)[LpRow<T>::NV], LpStat& st, int* gran) {
+  constexpr int NV = LpRow<T>::NV, kSeg = LpRow<T>::kSeg;
+  const int lane = threadIdx.x & 31;
+  float m[NV], mx;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) load_vec(base, skew, a.V, g * kSeg + i * 256 + lane * 8, next[i]);
+  for (int i = 0; i < NV; ++i) m[i] = x[i].max();
+  mx = m[0];
+#pragma unroll
+  for (int i = 1; i < NV; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(mx) : "f"(m[i]));
+  if constexpr (GR == 512) {
+#pragma unroll
+    for (int i = 0; i < NV; i += 2) {
+      const int k = __reduce_max_sync(0xffffffffu, max(order_key(m[i]), order_key(m[i + 1])));
+      const int at = g * (kSeg / 512) + i / 2;
+      if (lane == 0 && at * 512 < r.span) gran[at] = k;
+    }
+  } else if constexpr (GR > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      int k = order_key(m[i]);
+      if (GR == 64)
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, d));
+      const int at = g * (kSeg / GR) + (i * 256 + lane * 8) / GR;
+      if (lane % (GR / 8) == 0 && at * GR < r.span) gran[at] = k;
+    }
   }
-  for (; g < segs; g += step) {
-    Vec8<T> x[2] = {next[0], next[1]};
-    if (g + step < segs) {
+  lp_add<T, NV>(st, x, mx);
+}
+
+template <int N = 32> __device__ __forceinline__ LpStat lp_warp_join(LpStat st) {      // over N neighbouring lanes
 #pragma unroll
-      for (int i = 0; i < 2; ++i) load_vec(base, skew, a.V, (g + step) * kSeg + i * 256 + lane * 8, next[i]);
-    }
-    const float m0 = x[0].max(), m1 = x[1].max();
-    float mx;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(mx) : "f"(m0), "f"(m1));
-    if constexpr (GR == 512) {
-      const int k = __reduce_max_sync(0xffffffffu, order_key(mx));
-      if (lane == 0) gran0[g] = k;
-    } else if constexpr (GR > 0) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        int k = order_key(i ? m1 : m0);
-        if (GR == 64)
-#pragma unroll
-          for (int d = 1; d < 8; d <<= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, d));
-        const int at = g * (kSeg / GR) + (i * 256 + lane * 8) / GR;
-        if (lane % (GR / 8) == 0 && at * GR < span) gran0[at] = k;
-      }
-    }
-    if (mx > st.m || mx != mx) {
-      const float d = (st.m - mx) * kL2e, p = lp_ex2(d);
-      st.m = mx;
-      st.s = p == 0.f ? 0.f : p * (st.s + d * st.l);
-      st.l *= p;
-    }
-    if (st.m == -INFINITY) continue;
-    uint64_t l2[2] = {0, 0}, s2[2] = {0, 0};
-    const uint64_t off = pack(-st.m, -st.m), l2e = pack(kL2e, kL2e);
-    const bool safe = st.m > Vec8<T>::kLow;
-    if (safe) {                                      // from here on (z - m) log2(e) is finite and its exponential 0 where it should be
-      const float lo = st.m - fmaxf(104.f, fabsf(st.m) * 0.015625f);
-      x[0].clamp(lo);
-      x[1].clamp(lo);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float f[8];
-      x[i].get(f);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint64_t d = mul2(add2(pack(f[2 * j], f[2 * j + 1]), off), l2e);
-        float d0, d1;
-        unpack(d, d0, d1);
-        if (!safe) { d0 = fmaxf(d0, -200.f); d1 = fmaxf(d1, -200.f); d = pack(d0, d1); }
-        const uint64_t p = pack(lp_ex2(d0), lp_ex2(d1));
-        l2[j & 1] = add2(l2[j & 1], p);
-        s2[j & 1] = fma2(p, d, s2[j & 1]);
-      }
-    }
-    float u, v;
-    unpack(add2(l2[0], l2[1]), u, v);
-    st.l += u + v;
-    unpack(add2(s2[0], s2[1]), u, v);
-    st.s += u + v;
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
+  for (int d = N / 2; d; d >>= 1) {
     LpStat o;
     o.m = __shfl_xor_sync(0xffffffffu, st.m, d);
     o.l = __shfl_xor_sync(0xffffffffu, st.l, d);
     o.s = __shfl_xor_sync(0xffffffffu, st.s, d);
     st = lp_join(st, o);
   }
-  if (lane == 0) s_stat[w] = st;
-  if (tid == 0) s_n = 0;
+  return st;
+}
+
+// What a row gets from its statistics and the logit of its token; returns (m, log l).
+__device__ __forceinline__ float2 lp_finish(const LpArgs& a, long long row, bool scored, float zy, LpStat st) {
+  const float2 ml = make_float2(st.m, lp_lg2(st.l) * kLn2);
+  a.logprob[row] = scored ? log_prob(zy, ml) : 0.f;
+  a.entropy[row] = st.m == -INFINITY ? 0.f : ml.y - st.s / st.l * kLn2;
+  if (a.stat) a.stat[row] = ml;
+  return ml;
+}
+
+struct LpSelect {
+  int pick[kMaxTop];
+  unsigned long long cand[kCand];
+  int n;
+  unsigned floor;
+};
+
+// The alternatives of a row from the keys of its granules, by the whole block.
+template <typename T, int GR>
+__device__ __forceinline__ void lp_select(const LpArgs& a, long long row, const LpRow<T>& r, const int* gran, LpSelect& s, const float2& s_ml) {
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, w = tid >> 5, warps = threads >> 5;
+  const int grans = (r.span + GR - 1) / GR, want = min(a.top, grans);
+  // keys as unsigned integers without the low bits that this type's values never differ in
+  constexpr int kShift = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16;
+  if (w == 0) {
+    auto pick = [&](auto count) {
+      constexpr int K = decltype(count)::value;
+      unsigned key[K], t = 0;                        // of granules lane, lane + 32, ...; 0 is below every key
+#pragma unroll
+      for (int i = 0; i < K; ++i) key[i] = i * 32 + lane < grans ? ((unsigned)gran[i * 32 + lane] ^ 0x80000000u) >> kShift : 0u;
+      // t: the largest number that `want` keys reach, or a smaller one that exactly `want` keys reach
+      int reach = grans;
+      for (int bit = 31 - kShift; bit >= 0 && reach != want; --bit) {
+        const unsigned c = t | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < K; ++i) n += key[i] >= c;
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (n >= want) { t = c; reach = n; }
+      }
+      // keys above t, then those equal to it by lowest index as long as there is room
+      int above = 0, have = 0, ties = 0;
+      const unsigned need = reach == want ? t : t + 1;
+#pragma unroll
+      for (int i = 0; i < K; ++i) above += key[i] >= need;
+      above = __reduce_add_sync(0xffffffffu, above);
+#pragma unroll
+      for (int i = 0; i < K; ++i) {
+        const bool in = key[i] >= need, tie = !in && key[i] == t && i * 32 + lane < grans;
+        const unsigned m = __ballot_sync(0xffffffffu, in), e = __ballot_sync(0xffffffffu, tie), low = (1u << lane) - 1;
+        if (in) s.pick[have + __popc(m & low)] = i * 32 + lane;
+        const int at = above + ties + __popc(e & low);
+        if (tie && at < want) s.pick[at] = i * 32 + lane;
+        have += __popc(m);
+        ties += __popc(e);
+      }
+      if (lane == 0) { s.n = 0; s.floor = t; }
+    };
+    if (grans <= 256) pick(std::integral_constant<int, 8>()); else pick(std::integral_constant<int, 32>());
+  }
   __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < kLpWarps; ++i) st = lp_join(st, s_stat[i]);
-    *cl.map_shared_rank(&s_part[part], 0) = st;
+  // candidates: logits of those granules that reach the smallest of their maxima (fewer granules than `top`: all logits)
+  const int floor_key = want < a.top ? (int)0x80000000 : (int)((s.floor << kShift) ^ 0x80000000u);
+  constexpr int VPG = GR / 8, U = 5;                 // vectors a granule, vectors a thread has in flight
+  for (int q0 = 0; q0 < want * VPG; q0 += U * threads) {
+    Vec8<T> x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int q = q0 + u * threads + tid;
+      if (q < want * VPG) load_vec(r.base, r.skew, a.V, s.pick[q / VPG] * GR + q % VPG * 8, x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int q = q0 + u * threads + tid;
+      if (q >= want * VPG || order_key(x[u].max()) < floor_key) continue;
+      const int v = s.pick[q / VPG] * GR + q % VPG * 8;
+      float f[8];
+      x[u].get(f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int k = order_key(f[j]);
+        if (v + j >= r.skew && v + j < r.span && k >= floor_key) {
+          const int at = atomicAdd(&s.n, 1);         // the order of arrival does not matter: candidates are ranked below
+          if (at < kCand) s.cand[at] = cand_of(k, v + j - r.skew);
+        }
+      }
+    }
   }
-  if (parts > 1) cl.sync(); else __syncthreads();
-  if (part) return;                                  // part 0 has everything and reads no other block's memory from here on
-  if (tid == kLpThreads - 1) {
-    st = s_part[0];
-    for (int i = 1; i < parts; ++i) st = lp_join(st, s_part[i]);
-    const float2 ml = make_float2(st.m, lp_lg2(st.l) * kLn2);
+  __syncthreads();
+  const float2 ml = s_ml;
+  auto put = [&](int rank, unsigned long long c) {
+    const unsigned v = cand_index(c);
+    a.top_id[row * a.top + rank] = v;
+    a.top_lp[row * a.top + rank] = log_prob(key_value((int)((unsigned)(c >> 32) ^ 0x80000000u)), ml);
+  };
+  const int n = s.n;
+  if (n <= kCand) {
+    // rank: number of candidates before this one; all are different
+    for (int i = tid; i < n; i += threads) {
+      const unsigned long long c = s.cand[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += s.cand[j] > c;
+      if (rank < a.top) put(rank, c);
+    }
+    return;
+  }
+  // Many equal logits (a row of constants): a round for each alternative, the next one below the last. No list, exact.
+  unsigned long long below = ~0ull;
+  for (int q = 0; q < a.top; ++q) {
+    unsigned long long best = 0;
+    for (int i = tid; i < want * VPG; i += threads) {
+      const int v = s.pick[i / VPG] * GR + i % VPG * 8;
+      Vec8<T> x;
+      load_vec(r.base, r.skew, a.V, v, x);
+      float f[8];
+      x.get(f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const unsigned long long c = cand_of(order_key(f[j]), v + j - r.skew);
+        if (v + j >= r.skew && v + j < r.span && c < below && c > best) best = c;
+      }
+    }
+    for (int d = 16; d; d >>= 1) {
+      const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, d);
+      if (o > best) best = o;
+    }
+    __syncthreads();
+    if (lane == 0) s.cand[w] = best;
+    __syncthreads();
+    for (int i = 0; i < warps; ++i)
+      if (s.cand[i] > best) best = s.cand[i];
+    below = best;
+    if (tid == 0) put(q, best);
+  }
+}
+
+// gridDim.x = rows * blocks of a cluster.
+template <typename T, int GR>
+__global__ void __launch_bounds__(kLpThreads, sizeof(T) == 2 ? 3 : 4) token_logprobs_kernel(LpArgs a) {
+  cg::cluster_group cl = cg::this_cluster();
+  const int part = (int)cl.block_rank(), parts = (int)cl.num_blocks();
+  const long long row = blockIdx.x / parts;
+  __shared__ int s_gran[GR ? kMaxGranules : 1];      // order keys of the granules' maxima (of all parts, in part 0)
+  __shared__ LpStat s_stat[kLpWarps], s_part[8];
+  __shared__ LpSelect s_sel[1];
+  __shared__ float2 s_ml;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, warps = blockDim.x >> 5;
+  const LpRow<T> r(a, row);
+  int* gran0 = GR ? cl.map_shared_rank(s_gran, 0) : nullptr;
+  if (parts > 1) cl.sync();                          // part 0 runs: its shared memory may be written
+  bool scored = false;
+  float zy = 0.f;
+  if (part == 0 && w == warps - 1 && lane == 0) {    // the last warp finishes the row; its token's logit is under way from here on
     const long long y = a.ids[row];
-    a.logprob[row] = y >= 0 && y < a.V ? log_prob(to_f(z[y]), ml) : 0.f;
-    a.entropy[row] = st.m == -INFINITY ? 0.f : ml.y - st.s / st.l * kLn2;
-    if (a.stat) a.stat[row] = ml;
-    s_ml = ml;
+    scored = y >= 0 && y < a.V;
+    if (scored) zy = to_f(r.z[y]);
   }
-  if constexpr (GR > 0) {
-    // the first `top` granules by (maximum, lowest index): one warp, a round each
-    const int grans = (span + GR - 1) / GR, want = min(a.top, grans);
-    if (w == 0) {
-      for (int r = 0; r < want; ++r) {
-        int best = (int)0x80000000, at = 0x7fffffff;                 // a key is never the smallest integer: that marks the taken ones
-        for (int i = lane; i < grans; i += 32) {
-          const int k = s_gran[i];
-          if (k > best) { best = k; at = i; }
-        }
-        const int top = __reduce_max_sync(0xffffffffu, best);
-        const int win = __reduce_min_sync(0xffffffffu, best == top ? at : 0x7fffffff);
-        if (lane == 0) { s_gran[win] = (int)0x80000000; s_pick[r] = win; s_floor = top; }
-        __syncwarp();
-      }
-    }
-    __syncthreads();
-    // candidates: logits of those granules that reach the smallest of their maxima (fewer granules than `top`: all logits)
-    const int floor_key = want < a.top ? (int)0x80000000 : s_floor;
-    constexpr int VPG = GR / 8;                      // vectors a granule
-    for (int q0 = 0; q0 < want * VPG; q0 += 4 * kLpThreads) {
-      Vec8<T> x[4];
+
+  LpStat st{-INFINITY, 0.f, 0.f};
+  const int step = parts * warps;
+  int g = part * warps + w;
+  Vec8<T> next[LpRow<T>::NV];
+  if (g < r.segs) r.load(g, next);
+  for (; g < r.segs; g += step) {
+    Vec8<T> x[LpRow<T>::NV];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int q = q0 + u * kLpThreads + tid;
-        if (q < want * VPG) load_vec(base, skew, a.V, s_pick[q / VPG] * GR + q % VPG * 8, x[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int q = q0 + u * kLpThreads + tid;
-        if (q >= want * VPG) break;
-        const int v = s_pick[q / VPG] * GR + q % VPG * 8;
-        if (order_key(x[u].max()) < floor_key) continue;
-        float f[8];
-        x[u].get(f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int k = order_key(f[j]);
-          if (v + j >= skew && v + j < span && k >= floor_key) {
-            const int at = atomicAdd(&s_n, 1);       // the order of arrival does not matter: candidates are ranked below
-            if (at < kCand) s_cand[at] = cand_of(k, v + j - skew);
-          }
-        }
-      }
-    }
-    __syncthreads();
-    const float2 ml = s_ml;
-    const int n = s_n;
-    if (n <= kCand) {
-      // rank: number of candidates before this one; all are different
-      for (int i = tid; i < n; i += kLpThreads) {
-        const unsigned long long c = s_cand[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += s_cand[j] > c;
-        if (rank < a.top) {
-          const unsigned v = cand_index(c);
-          a.top_id[row * a.top + rank] = v;
-          a.top_lp[row * a.top + rank] = log_prob(to_f(z[v]), ml);
-        }
-      }
-      return;
-    }
-    // Many equal logits (a row of constants): a round for each alternative, the next one below the last. No list, exact.
-    unsigned long long below = ~0ull;
-    for (int r = 0; r < a.top; ++r) {
-      unsigned long long best = 0;
-      for (int q = tid; q < want * VPG; q += kLpThreads) {
-        const int v = s_pick[q / VPG] * GR + q % VPG * 8;
-        Vec8<T> x;
-        load_vec(base, skew, a.V, v, x);
-        float f[8];
-        x.get(f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const unsigned long long c = cand_of(order_key(f[j]), v + j - skew);
-          if (v + j >= skew && v + j < span && c < below && c > best) best = c;
-        }
-      }
-      for (int d = 16; d; d >>= 1) {
-        const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, d);
-        if (o > best) best = o;
-      }
-      __syncthreads();
-      if (lane == 0) s_cand[w] = best;
-      __syncthreads();
-      for (int i = 0; i < kLpWarps; ++i)
-        if (s_cand[i] > best) best = s_cand[i];
-      below = best;
-      if (tid == 0) {
-        const unsigned v = cand_index(best);
-        a.top_id[row * a.top + r] = v;
-        a.top_lp[row * a.top + r] = log_prob(to_f(z[v]), ml);
-      }
+    for (int i = 0; i < LpRow<T>::NV; ++i) x[i] = next[i];
+    if (g + step < r.segs) r.load(g + step, next);
+    lp_segment<T, GR>(r, g, x, st, gran0);
+  }
+  st = lp_warp_join(st);
+  if (lane == 0) s_stat[w] = st;
+  __syncthreads();
+  if (w == warps - 1) {
+    st = lane < warps ? s_stat[lane] : LpStat{-INFINITY, 0.f, 0.f};
+    st = lp_warp_join<kLpWarps>(st);
+    if (parts > 1 && lane == 0) *cl.map_shared_rank(&s_part[part], 0) = st;
+  }
+  if (parts > 1) {
+    cl.sync();
+    if (part) return;                                // part 0 has everything and reads no other block's memory from here on
+    if (w == warps - 1) {
+      st = lane < parts ? s_part[lane] : LpStat{-INFINITY, 0.f, 0.f};
+      st = lp_warp_join<8>(st);
     }
   }
+  if (w == warps - 1 && lane == 0) s_ml = lp_finish(a, row, scored, zy, st);
+  if constexpr (GR > 0) lp_select<T, GR>(a, row, r, s_gran, s_sel[0], s_ml);
 }
 
 struct LpGradArgs {
@@ -432,14 +534,20 @@ template <typename T> __global__ void __launch_bounds__(kGradThreads) token_logp
   }
 }
 
-template <typename T, int GR> int launch_granule(const LpArgs& a, int parts, cudaStream_t st) {
+template <typename T, int GR> int launch_granule(const LpArgs& a, cudaStream_t st) {
+  const int resident = sizeof(T) == 2 ? 3 : 4;
+  // parts of a row: while the card holds them all at once and every warp has 512 logits
+  int parts = 1;
+  while (parts < 8 && a.rows * parts * 2 <= (long long)resident * sm_count() && a.V >= parts * 2 * kLpWarps * 512) parts *= 2;
+  // a warp for each segment, 8 at most
+  const int per = a.V / parts / LpRow<T>::kSeg, threads = 32 * (per < 1 ? 1 : per < kLpWarps ? per : kLpWarps);
   if (parts == 1) {
-    token_logprobs_kernel<T, GR><<<(unsigned)a.rows, kLpThreads, 0, st>>>(a);
+    token_logprobs_kernel<T, GR><<<(unsigned)a.rows, threads, 0, st>>>(a);
     return (int)cudaGetLastError();
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * parts));
-  cfg.blockDim = dim3(kLpThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -450,14 +558,11 @@ template <typename T, int GR> int launch_granule(const LpArgs& a, int parts, cud
   return (int)cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, GR>, a);
 }
 template <typename T> int launch_logprobs(const LpArgs& a, cudaStream_t st) {
-  // parts of a row: while the card holds them all at once (4 blocks a multiprocessor) and every warp has a segment
-  int parts = 1;
-  while (parts < 8 && a.rows * parts * 2 <= 4ll * sm_count() && a.V >= parts * 2 * kLpWarps * kSeg) parts *= 2;
-  if (a.top == 0) return launch_granule<T, 0>(a, parts, st);
-  // granules: enough of them that the ones read again are few, few enough for one warp to pick from
-  if (a.V <= 4096) return launch_granule<T, 8>(a, parts, st);
-  if (a.V <= 16384) return launch_granule<T, 64>(a, parts, st);
-  return launch_granule<T, 512>(a, parts, st);
+  // granules: as large as leaves two for every alternative
+  if (a.top == 0) return launch_granule<T, 0>(a, st);
+  if (a.V >= 1024 * a.top) return launch_granule<T, 512>(a, st);
+  if (a.V >= 128 * a.top) return launch_granule<T, 64>(a, st);
+  return launch_granule<T, 8>(a, st);
 }
 template <typename T> int launch_grad(const LpGradArgs& a, cudaStream_t st) {
   const dim3 grid((unsigned)a.rows, (unsigned)((a.V + 7 + kGradChunk - 1) / kGradChunk));
@@ -477,7 +582,7 @@ struct LpCall {
 };
 extern "C" int hippo_token_logprobs(const LpCall* c) {
   if (c->rows <= 0) return 0;
-  if (c->V < 1 || c->V > (kMaxGranules - 1) * kSeg || c->top < 0 || c->top > kMaxTop || c->top > c->V || c->rows > 0x0fffffffll) return -1;
+  if (c->V < 1 || c->V > (kMaxGranules - 1) * 512 || c->top < 0 || c->top > kMaxTop || c->top > c->V || c->rows > 0x0fffffffll) return -1;
   LpArgs a{c->z, c->ld, c->rows, c->V, c->ids, c->top, c->logprob, c->entropy, (float2*)c->stat, c->top_lp, c->top_id};
   cudaStream_t st = (cudaStream_t)c->stream;
   if (c->dtype == 0) return launch_logprobs<__nv_bfloat16>(a, st);

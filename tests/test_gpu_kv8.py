@@ -205,7 +205,8 @@ def score_bound(z, dtype):
 
 
 @pytest.mark.parametrize("T,V,top", [(1, 1, 1), (3, 2, 2), (5, 33, 20), (2, 600, 5), (4, 1031, 32), (1, 9000, 20), (3, 32000, 1),
-                                     (2, 128256, 20), (700, 515, 3), (1, 523776, 32)])
+                                     (2, 128256, 20), (700, 515, 3), (1, 523776, 32),
+                                     (1300, 9001, 20), (5000, 700, 3), (9500, 130, 8), (1000, 1024, 1)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_scores_match_64_bits(T, V, top, dtype):
     g = torch.Generator().manual_seed(V)
