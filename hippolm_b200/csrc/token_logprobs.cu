@@ -416,7 +416,7 @@ __device__ __forceinline__ void lp_select(const LpArgs& a, long long row, const 
 
 // gridDim.x = rows * blocks of a cluster.
 template <typename T, int GR>
-__global__ void __launch_bounds__(kLpThreads, sizeof(T) == 2 ? 3 : 4) token_logprobs_kernel(LpArgs a) {
+__global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(LpArgs a) {
   cg::cluster_group cl = cg::this_cluster();
   const int part = (int)cl.block_rank(), parts = (int)cl.num_blocks();
   const long long row = blockIdx.x / parts;
@@ -535,7 +535,7 @@ template <typename T> __global__ void __launch_bounds__(kGradThreads) token_logp
 }
 
 template <typename T, int GR> int launch_granule(const LpArgs& a, cudaStream_t st) {
-  const int resident = sizeof(T) == 2 ? 3 : 4;
+  const int resident = 4;
   // parts of a row: while the card holds them all at once and every warp has 512 logits
   int parts = 1;
   while (parts < 8 && a.rows * parts * 2 <= (long long)resident * sm_count() && a.V >= parts * 2 * kLpWarps * 512) parts *= 2;
