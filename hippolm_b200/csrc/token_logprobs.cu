@@ -133,18 +133,6 @@ struct LpArgs {
 __device__ __forceinline__ float log_prob(float z, float2 ml) { return ml.x == -INFINITY ? -INFINITY : (z - ml.x) - ml.y; }
 
 struct LpStat { float m, l, s; };                    // maximum, sum of e^(z - m), sum of (z - m) log2(e) e^(z - m)
-__device__ __forceinline__ LpStat lp_join(LpStat a, LpStat b) {
-  LpStat r;
-  r.m = (a.m != a.m || b.m != b.m) ? __int_as_float(0x7fffffff) : fmaxf(a.m, b.m);
-  if (r.m == -INFINITY) { r.l = r.s = 0.f; return r; }
-  const float da = (a.m - r.m) * kL2e, db = (b.m - r.m) * kL2e;
-  const float pa = lp_ex2(da), pb = lp_ex2(db);
-  r.l = a.l * pa + b.l * pb;
-  // a part of weight 0 leaves nothing (its distance may be infinite)
-  r.s = (pa == 0.f ? 0.f : pa * (a.s + da * a.l)) + (pb == 0.f ? 0.f : pb * (b.s + db * b.l));
-  return r;
-}
-
 // A row is cut in vectors of 8 from the aligned address at or before its start: index v of that grid is logit v - skew. What lies
 // outside [0, V) is not read and counts as -inf.
 template <typename T> __device__ __forceinline__ void load_vec(const T* base, int skew, int V, int v, Vec8<T>& x) {
@@ -267,16 +255,17 @@ template <typename T, int GR> __device__ __forceinline__ void lp_segment(const L
   lp_add<T, NV>(st, x, mx);
 }
 
-template <int N = 32> __device__ __forceinline__ LpStat lp_warp_join(LpStat st) {      // over N neighbouring lanes
+__device__ __forceinline__ LpStat lp_warp_join(LpStat st) {
+  const float m = key_value(__reduce_max_sync(0xffffffffu, order_key(st.m)));
+  const float d = (st.m - m) * kL2e, p = m == -INFINITY ? 0.f : lp_ex2(d);
+  // a part of weight 0 leaves nothing (its distance may be infinite)
+  float l = st.l * p, s = p == 0.f ? 0.f : p * (st.s + d * st.l);
 #pragma unroll
-  for (int d = N / 2; d; d >>= 1) {
-    LpStat o;
-    o.m = __shfl_xor_sync(0xffffffffu, st.m, d);
-    o.l = __shfl_xor_sync(0xffffffffu, st.l, d);
-    o.s = __shfl_xor_sync(0xffffffffu, st.s, d);
-    st = lp_join(st, o);
+  for (int k = 16; k; k >>= 1) {
+    l += __shfl_xor_sync(0xffffffffu, l, k);
+    s += __shfl_xor_sync(0xffffffffu, s, k);
   }
-  return st;
+  return {m, l, s};
 }
 
 // What a row gets from its statistics and the logit of its token; returns (m, log l).
@@ -308,25 +297,34 @@ __device__ __forceinline__ void lp_select(const LpArgs& a, long long row, const 
       unsigned key[K], t = 0;                        // of granules lane, lane + 32, ...; 0 is below every key
 #pragma unroll
       for (int i = 0; i < K; ++i) key[i] = i * 32 + lane < grans ? ((unsigned)gran[i * 32 + lane] ^ 0x80000000u) >> kShift : 0u;
-      // t: the largest number that `want` keys reach, or a smaller one that exactly `want` keys reach
-      int reach = grans;
-      for (int bit = 31 - kShift; bit >= 0 && reach != want; --bit) {
-        const unsigned c = t | 1u << bit;
-        int n = 0;
+      // t: the largest number that `want` keys reach, or a smaller one that exactly `want` keys reach; it begins like all keys do
+      unsigned most = key[0], least = 0xffffffffu;
 #pragma unroll
-        for (int i = 0; i < K; ++i) n += key[i] >= c;
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (n >= want) { t = c; reach = n; }
+      for (int i = 0; i < K; ++i) {
+        most = max(most, key[i]);
+        least = min(least, i * 32 + lane < grans ? key[i] : 0xffffffffu);
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      least = __reduce_min_sync(0xffffffffu, least);
+      int reach = grans, bit = 31 - __clz(most ^ least);               // -1 where all are equal
+      t = bit < 0 ? most : most & ~((2u << bit) - 1);
+      for (; bit >= 0 && reach != want; --bit) {
+        const unsigned c = t | 1u << bit;
+        int n[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < K; ++i) n[i & 3] += key[i] >= c;
+        const int all = __reduce_add_sync(0xffffffffu, n[0] + n[1] + n[2] + n[3]);
+        if (all >= want) { t = c; reach = all; }
       }
       // keys above t, then those equal to it by lowest index as long as there is room
       int above = 0, have = 0, ties = 0;
-      const unsigned need = reach == want ? t : t + 1;
+      const bool all_in = reach == want;
 #pragma unroll
-      for (int i = 0; i < K; ++i) above += key[i] >= need;
+      for (int i = 0; i < K; ++i) above += key[i] > t || (all_in && key[i] == t);
       above = __reduce_add_sync(0xffffffffu, above);
 #pragma unroll
       for (int i = 0; i < K; ++i) {
-        const bool in = key[i] >= need, tie = !in && key[i] == t && i * 32 + lane < grans;
+        const bool in = key[i] > t || (all_in && key[i] == t), tie = !in && key[i] == t && i * 32 + lane < grans;
         const unsigned m = __ballot_sync(0xffffffffu, in), e = __ballot_sync(0xffffffffu, tie), low = (1u << lane) - 1;
         if (in) s.pick[have + __popc(m & low)] = i * 32 + lane;
         const int at = above + ties + __popc(e & low);
@@ -340,7 +338,12 @@ __device__ __forceinline__ void lp_select(const LpArgs& a, long long row, const 
   }
   __syncthreads();
   // candidates: logits of those granules that reach the smallest of their maxima (fewer granules than `top`: all logits)
-  const int floor_key = want < a.top ? (int)0x80000000 : (int)((s.floor << kShift) ^ 0x80000000u);
+  float floor = -INFINITY;
+  if (want == a.top) {
+    const int k = (int)((s.floor << kShift) ^ 0x80000000u);          // (a bit pattern between two values is as good a bound)
+    floor = key_value(k);
+    if (floor != floor) floor = k > 0 ? INFINITY : -INFINITY;        // beyond the infinities
+  }
   constexpr int VPG = GR / 8, U = 5;                 // vectors a granule, vectors a thread has in flight
   for (int q0 = 0; q0 < want * VPG; q0 += U * threads) {
     Vec8<T> x[U];
@@ -352,17 +355,18 @@ __device__ __forceinline__ void lp_select(const LpArgs& a, long long row, const 
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int q = q0 + u * threads + tid;
-      if (q >= want * VPG || order_key(x[u].max()) < floor_key) continue;
+      if (q >= want * VPG || x[u].max() < floor) continue;           // (NaN is not below)
       const int v = s.pick[q / VPG] * GR + q % VPG * 8;
       float f[8];
       x[u].get(f);
+      unsigned hit = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int k = order_key(f[j]);
-        if (v + j >= r.skew && v + j < r.span && k >= floor_key) {
-          const int at = atomicAdd(&s.n, 1);         // the order of arrival does not matter: candidates are ranked below
-          if (at < kCand) s.cand[at] = cand_of(k, v + j - r.skew);
-        }
+      for (int j = 0; j < 8; ++j) hit |= (f[j] < floor ? 0u : 1u) << j;
+      for (; hit; hit &= hit - 1) {
+        const int i = v + __ffs(hit) - 1 - r.skew;
+        if (i < 0 || i >= a.V) continue;
+        const int at = atomicAdd(&s.n, 1);           // the order of arrival does not matter: candidates are ranked below
+        if (at < kCand) s.cand[at] = cand_of(order_key(to_f(r.z[i])), i);
       }
     }
   }
@@ -379,6 +383,7 @@ __device__ __forceinline__ void lp_select(const LpArgs& a, long long row, const 
     for (int i = tid; i < n; i += threads) {
       const unsigned long long c = s.cand[i];
       int rank = 0;
+#pragma unroll 8
       for (int j = 0; j < n; ++j) rank += s.cand[j] > c;
       if (rank < a.top) put(rank, c);
     }
@@ -453,7 +458,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(LpArgs a)
   __syncthreads();
   if (w == warps - 1) {
     st = lane < warps ? s_stat[lane] : LpStat{-INFINITY, 0.f, 0.f};
-    st = lp_warp_join<kLpWarps>(st);
+    st = lp_warp_join(st);
     if (parts > 1 && lane == 0) *cl.map_shared_rank(&s_part[part], 0) = st;
   }
   if (parts > 1) {
@@ -461,7 +466,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(LpArgs a)
     if (part) return;                                // part 0 has everything and reads no other block's memory from here on
     if (w == warps - 1) {
       st = lane < parts ? s_part[lane] : LpStat{-INFINITY, 0.f, 0.f};
-      st = lp_warp_join<8>(st);
+      st = lp_warp_join(st);
     }
   }
   if (w == warps - 1 && lane == 0) s_ml = lp_finish(a, row, scored, zy, st);

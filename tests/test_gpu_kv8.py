@@ -236,14 +236,29 @@ def test_scores_of_masked_and_broken_rows():
     check_special(DEV)
 
 
-@pytest.mark.parametrize("V,top", [(4096, 20), (20000, 32), (128256, 7)])
-def test_alternatives_among_equal_logits(V, top):
-    z = torch.zeros(3, V, device=DEV, dtype=torch.bfloat16)
+@pytest.mark.parametrize("V,top", [(4096, 20), (20000, 32), (128256, 7), (1000, 3)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_alternatives_among_equal_logits(V, top, dtype):
+    z = torch.zeros(10, V, device=DEV, dtype=dtype)
     z[1, V - 5:] = 1.0
     z[2, ::3] = 2.0
-    got = ops.token_logprobs(z, torch.zeros(3, dtype=torch.int64, device=DEV), top_k=top)
-    order = torch.sort(z.float().cpu(), dim=-1, descending=True, stable=True).indices[:, :top]
+    z[3] = -math.inf
+    z[4, V // 2:] = math.nan
+    z[5, 5:] = -math.inf
+    z[6] = torch.finfo(dtype).min
+    z[6, V // 3] = -3.0
+    z[7] = -1.5 - torch.arange(V, device=DEV) % 7
+    z[8, 100:900:90] = math.inf
+    z[9, ::2] = -0.0
+    got = ops.token_logprobs(z, torch.zeros(10, dtype=torch.int64, device=DEV), top_k=top)
+    order = torch.sort(z.float().cpu() + 0.0, dim=-1, descending=True, stable=True).indices[:, :top]
     assert torch.equal(got.top_ids.cpu(), order)
+    want = torch.log_softmax(z.double().cpu(), -1).gather(1, order)
+    for t in (0, 1, 2, 5, 6, 7, 9):
+        w = want[t].clamp(min=torch.finfo(torch.float32).min)
+        g = got.top_logprobs[t].cpu().double().clamp(min=torch.finfo(torch.float32).min)
+        assert bool(((g - w).abs() <= 1e-5 + 1e-6 * w.abs()).all()), t
+    assert torch.isneginf(got.top_logprobs[3]).all() and torch.isnan(got.top_logprobs[[4, 8]]).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
