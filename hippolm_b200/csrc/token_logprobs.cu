@@ -308,29 +308,51 @@ __device__ __forceinline__ void lp_select(const LpArgs& a, long long row, const 
       least = __reduce_min_sync(0xffffffffu, least);
       int reach = grans, bit = 31 - __clz(most ^ least);               // -1 where all are equal
       t = bit < 0 ? most : most & ~((2u << bit) - 1);
-      for (; bit >= 0 && reach != want; --bit) {
-        const unsigned c = t | 1u << bit;
-        int n[4] = {0, 0, 0, 0};
+      while (bit >= 0 && reach != want) {            // two bits a round: three numbers to try, their counts side by side
+        const int low = bit ? bit - 1 : 0;
+        const unsigned c1 = t | 1u << low, c2 = bit ? t | 1u << bit : 0xffffffffu, c3 = c2 | 1u << low;
+        unsigned n1 = 0, n23 = 0;
 #pragma unroll
-        for (int i = 0; i < K; ++i) n[i & 3] += key[i] >= c;
-        const int all = __reduce_add_sync(0xffffffffu, n[0] + n[1] + n[2] + n[3]);
-        if (all >= want) { t = c; reach = all; }
+        for (int i = 0; i < K; ++i) {
+          n1 += key[i] >= c1;
+          n23 += (key[i] >= c2 ? 1u : 0u) + (key[i] >= c3 ? 0x10000u : 0u);
+        }
+        n1 = __reduce_add_sync(0xffffffffu, n1);
+        n23 = __reduce_add_sync(0xffffffffu, n23);
+        const int r3 = bit ? (int)(n23 >> 16) : 0, r2 = bit ? (int)(n23 & 0xffffu) : 0, r1 = (int)n1;
+        if (r3 >= want) { t = c3; reach = r3; }
+        else if (r2 >= want) { t = c2; reach = r2; }
+        else if (r1 >= want) { t = c1; reach = r1; }
+        bit -= 2;
       }
-      // keys above t, then those equal to it by lowest index as long as there is room
-      int above = 0, have = 0, ties = 0;
-      const bool all_in = reach == want;
+      // keys above t (where exactly `want` reach it: from t on), lane by lane
+      const bool exact = reach == want;
+      int mine = 0;
 #pragma unroll
-      for (int i = 0; i < K; ++i) above += key[i] > t || (all_in && key[i] == t);
-      above = __reduce_add_sync(0xffffffffu, above);
+      for (int i = 0; i < K; ++i) mine += key[i] > t || (exact && key[i] == t && i * 32 + lane < grans);
+      int at = mine;
 #pragma unroll
-      for (int i = 0; i < K; ++i) {
-        const bool in = key[i] > t || (all_in && key[i] == t), tie = !in && key[i] == t && i * 32 + lane < grans;
-        const unsigned m = __ballot_sync(0xffffffffu, in), e = __ballot_sync(0xffffffffu, tie), low = (1u << lane) - 1;
-        if (in) s.pick[have + __popc(m & low)] = i * 32 + lane;
-        const int at = above + ties + __popc(e & low);
-        if (tie && at < want) s.pick[at] = i * 32 + lane;
-        have += __popc(m);
-        ties += __popc(e);
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, at, d);
+        if (lane >= d) at += y;
+      }
+      const int above = __shfl_sync(0xffffffffu, at, 31);
+      at -= mine;
+#pragma unroll
+      for (int i = 0; i < K; ++i)
+        if (key[i] > t || (exact && key[i] == t && i * 32 + lane < grans)) s.pick[at++] = i * 32 + lane;
+      // then those equal to t by lowest index as long as there is room
+      if (!exact) {
+        int have = above;
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+          const bool tie = key[i] == t && i * 32 + lane < grans;
+          const unsigned e = __ballot_sync(0xffffffffu, tie);
+          const int p = have + __popc(e & ((1u << lane) - 1));
+          if (tie && p < want) s.pick[p] = i * 32 + lane;
+          have += __popc(e);
+          if (have >= want) break;
+        }
       }
       if (lane == 0) { s.n = 0; s.floor = t; }
     };
@@ -352,22 +374,22 @@ __device__ __forceinline__ void lp_select(const LpArgs& a, long long row, const 
       const int q = q0 + u * threads + tid;
       if (q < want * VPG) load_vec(r.base, r.skew, a.V, s.pick[q / VPG] * GR + q % VPG * 8, x[u]);
     }
+    unsigned long long hits = 0;                     // bit 8u + j: logit j of vector u
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int q = q0 + u * threads + tid;
-      if (q >= want * VPG || x[u].max() < floor) continue;           // (NaN is not below)
-      const int v = s.pick[q / VPG] * GR + q % VPG * 8;
+      if (q0 + u * threads + tid >= want * VPG || x[u].max() < floor) continue;      // (NaN is not below)
       float f[8];
       x[u].get(f);
       unsigned hit = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) hit |= (f[j] < floor ? 0u : 1u) << j;
-      for (; hit; hit &= hit - 1) {
-        const int i = v + __ffs(hit) - 1 - r.skew;
-        if (i < 0 || i >= a.V) continue;
-        const int at = atomicAdd(&s.n, 1);           // the order of arrival does not matter: candidates are ranked below
-        if (at < kCand) s.cand[at] = cand_of(order_key(to_f(r.z[i])), i);
-      }
+      hits |= (unsigned long long)hit << (8 * u);
+    }
+    for (; hits; hits &= hits - 1) {
+      const int b = __ffsll(hits) - 1, q = q0 + (b >> 3) * threads + tid, i = s.pick[q / VPG] * GR + q % VPG * 8 + (b & 7) - r.skew;
+      if (i < 0 || i >= a.V) continue;
+      const int at = atomicAdd(&s.n, 1);             // the order of arrival does not matter: candidates are ranked below
+      if (at < kCand) s.cand[at] = cand_of(order_key(to_f(r.z[i])), i);
     }
   }
   __syncthreads();
@@ -379,13 +401,15 @@ __device__ __forceinline__ void lp_select(const LpArgs& a, long long row, const 
   };
   const int n = s.n;
   if (n <= kCand) {
-    // rank: number of candidates before this one; all are different
-    for (int i = tid; i < n; i += threads) {
-      const unsigned long long c = s.cand[i];
+    // rank: number of candidates before this one (all are different), counted by 8 threads a candidate
+    for (int i0 = 0; i0 < n; i0 += threads / 8) {
+      const int i = i0 + tid / 8;
+      const unsigned long long c = i < n ? s.cand[i] : 0ull;
       int rank = 0;
-#pragma unroll 8
-      for (int j = 0; j < n; ++j) rank += s.cand[j] > c;
-      if (rank < a.top) put(rank, c);
+      for (int j = tid & 7; j < n; j += 8) rank += s.cand[j] > c;
+#pragma unroll
+      for (int k = 1; k < 8; k <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, k);
+      if (i < n && rank < a.top && (tid & 7) == 0) put(rank, c);
     }
     return;
   }
