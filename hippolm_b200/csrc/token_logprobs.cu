@@ -237,9 +237,11 @@ template <typename T, int GR> __device__ __forceinline__ void lp_segment(const L
   if constexpr (GR == 512) {
 #pragma unroll
     for (int i = 0; i < NV; i += 2) {
-      const int k = __reduce_max_sync(0xffffffffu, max(order_key(m[i]), order_key(m[i + 1])));
+      float k;
+      asm("max.NaN.f32 %0, %1, %2;" : "=f"(k) : "f"(m[i]), "f"(m[i + 1]));
+      asm("redux.sync.max.NaN.f32 %0, %0, 0xffffffff;" : "+f"(k));
       const int at = g * (kSeg / 512) + i / 2;
-      if (lane == 0 && at * 512 < r.span) gran[at] = k;
+      if (lane == 0 && at * 512 < r.span) gran[at] = order_key(k);
     }
   } else if constexpr (GR > 0) {
 #pragma unroll
