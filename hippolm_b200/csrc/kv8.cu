@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(
     if (in) {
       lens_out[n] = (int)(ok ? len + want : len);
       served[n] = ok;
-      cu[n + 1] = (int)min(end, (long long)0x7fffffff);
+      if (cu) cu[n + 1] = (int)min(end, (long long)0x7fffffff);
     }
     __syncthreads();
     for (int p = tid; p < (int)total; p += kPlanThreads) {
@@ -138,7 +138,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(
   }
   if (write_slots)
     for (long long t = min(tokens, num_tokens) + tid; t < num_tokens; t += kPlanThreads) slots[t] = -1;
-  if (tid == 0) { cu[0] = 0; *count_out = (int)(count - used); }
+  if (tid == 0) {
+    if (cu) cu[0] = 0;
+    *count_out = (int)(count - used);
+  }
 }
 
 // Slot map of many tokens (prompts): 4 tokens a thread, the request of the first found in the packed ends, the table rows stay in
@@ -434,7 +437,8 @@ using namespace hippo;
 // Arguments come as one block (a packed struct costs the caller a fifth of converting twenty arguments one by one).
 
 // table [N][M] int32 (row pitch table_ld), lens / new_lens [N], free_list [cap], free_count [1], release [N] or null; out: slots
-// [num_tokens], lens_out [N], count_out [1], served [N], cu [N + 1].
+// [num_tokens], lens_out [N], count_out [1], served [N], cu [N + 1]
+// (ends of the packed tokens; null: the planning block writes the slots itself, which is the faster form up to some 16 thousand).
 struct KvPlanCall {
   int* table; const int *lens, *new_lens; int* free_list; const int* free_count; const unsigned char* release;
   long long* slots; int *lens_out, *count_out; unsigned char* served; int* cu; void* stream;
@@ -444,7 +448,7 @@ struct KvPlanCall {
 extern "C" int hippo_kv8_plan(const KvPlanCall* c) {
   const int sh = c->block_size == 16 ? 4 : c->block_size == 32 ? 5 : c->block_size == 64 ? 6 : -1;
   if (sh < 0 || c->N < 1 || c->M < 1 || c->cap < 1 || c->num_tokens < 0 || c->num_tokens > 0x7fffffffll) return -1;
-  const bool many = c->num_tokens > 16384;
+  const bool many = c->cu != nullptr;
   cudaStream_t st = (cudaStream_t)c->stream;
   kv8_plan_kernel<<<1, kPlanThreads, 0, st>>>(c->table, c->table_ld, c->M, c->lens, c->new_lens, c->N, c->free_list, c->cap,
                                               c->free_count, c->release, sh, c->num_tokens, c->slots, c->lens_out, c->count_out,

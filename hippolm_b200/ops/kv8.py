@@ -20,6 +20,7 @@ from . import kv8_cuda
 BLOCK_SIZES = (16, 32, 64)
 CODE_TYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 FLOAT_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_CODES = frozenset(CODE_TYPES.values())
 
 
 class KV8Plan(NamedTuple):
@@ -27,7 +28,6 @@ class KV8Plan(NamedTuple):
     lens: torch.Tensor          # int32 [requests]: lengths with the new tokens
     free_count: torch.Tensor    # int32 [1]: blocks left in the free list
     served: torch.Tensor        # bool [requests]: whether the request's new tokens have slots
-    cu_seqlens: torch.Tensor    # int32 [requests + 1]: ends of the requests' new tokens in the packed stream
 
 
 def _need(ok: bool, what: str) -> None:
@@ -48,17 +48,10 @@ def kv8_empty(blocks: int, heads: int, head_dim: int, block_size: int = 64, dtyp
 
 # The operators check their arguments in one expression and call these only to say what is wrong: a decoding step makes these
 # calls for every layer, and its time is the host's.
-def _cache_ok(codes, scales) -> bool:
-    c = codes.shape
-    return (len(c) == 5 and c[0] == 2 and c[1] > 0 and c[2] > 0 and c[3] in BLOCK_SIZES
-            and (codes.dtype == torch.float8_e4m3fn or codes.dtype == torch.int8) and codes.is_contiguous()
-            and codes.data_ptr() % 16 == 0 and scales.dtype == torch.float32 and scales.is_contiguous() and scales.shape == c[:3])
-
-
-def _table_ok(table, lens) -> bool:
-    t = table.shape
-    return (len(t) == 2 and t[1] > 0 and table.dtype == torch.int32 and table.stride(1) == 1 and lens.dtype == torch.int32
-            and lens.is_contiguous() and lens.shape == t[:1])
+def _cache_ok(codes, c, scales) -> bool:
+    return (len(c) == 5 and c[0] == 2 and c[1] > 0 and c[2] > 0 and c[3] in BLOCK_SIZES and codes.dtype in _CODES
+            and codes.is_contiguous() and codes.data_ptr() % 16 == 0 and scales.dtype == torch.float32 and scales.is_contiguous()
+            and scales.shape == c[:3])
 
 
 def _refuse_cache(codes, scales) -> None:
@@ -96,12 +89,13 @@ def kv8_plan(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, fr
     ``table`` gets the new blocks and ``free_list`` the released ones, in place; lengths and the stack's height are returned new
     (``plan.lens``, ``plan.free_count``), so a repeated call with the same lengths gives the same plan. Lengths below 0 count as 0,
     lengths beyond the table's width as the width."""
-    if not (_table_ok(table, lens) and (table.shape[0] <= 1 or table.stride(0) >= table.shape[1])
-            and new_lens.dtype == torch.int32 and new_lens.is_contiguous() and new_lens.shape == lens.shape
-            and free_list.dtype == torch.int32 and free_list.is_contiguous() and free_list.dim() == 1 and free_list.numel() > 0
-            and free_count.dtype == torch.int32 and free_count.numel() == 1 and block_size in BLOCK_SIZES
-            and 0 <= num_tokens < 1 << 31 and table.shape[1] * block_size < 1 << 31
-            and (release is None or (release.dtype == torch.bool and release.is_contiguous() and release.shape == lens.shape))):
+    ts, ls = table.shape, lens.shape
+    if not (len(ts) == 2 and ts[1] > 0 and table.dtype == lens.dtype == new_lens.dtype == free_list.dtype == free_count.dtype == torch.int32
+            and ls == ts[:1] == new_lens.shape and lens.is_contiguous() and new_lens.is_contiguous() and table.stride(1) == 1
+            and (ts[0] <= 1 or table.stride(0) >= ts[1]) and free_list.is_contiguous() and free_list.dim() == 1
+            and free_list.numel() > 0 and free_count.numel() == 1 and block_size in BLOCK_SIZES and 0 <= num_tokens < 1 << 31
+            and ts[1] * block_size < 1 << 31
+            and (release is None or (release.dtype == torch.bool and release.is_contiguous() and release.shape == ls))):
         _refuse_table(table, lens)
         _need(table.shape[0] <= 1 or table.stride(0) >= table.shape[1], "table: rows that do not overlap")
         _need(new_lens.dtype == torch.int32 and new_lens.is_contiguous() and new_lens.shape == lens.shape,
@@ -117,12 +111,12 @@ def kv8_plan(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, fr
     if not (dev == lens.get_device() == new_lens.get_device() == free_list.get_device() == free_count.get_device()) or (
             release is not None and release.get_device() != dev):
         _refuse_devices(table, lens, new_lens, free_list, free_count, *([] if release is None else [release]))
-    if table.shape[0] == 0:
+    if ts[0] == 0:
         d = table.device
-        return KV8Plan(torch.full((num_tokens,), -1, dtype=torch.int64, device=d), lens.clone(), free_count.reshape(1).clone(),
-                       torch.empty(0, dtype=torch.bool, device=d), torch.zeros(1, dtype=torch.int32, device=d))
+        return KV8Plan(torch.full((num_tokens,), -1, dtype=torch.int64, device=d), lens.clone(), free_count.clone(),
+                       torch.empty(0, dtype=torch.bool, device=d))
     if dev >= 0:
-        return KV8Plan(*kv8_cuda.plan(table, lens, new_lens, free_list, free_count, block_size, num_tokens, release, dev))
+        return KV8Plan._make(kv8_cuda.plan(table, lens, new_lens, free_list, free_count, block_size, num_tokens, release, dev, ts))
     return KV8Plan(*_ref.kv8_plan(table, lens, new_lens, free_list, free_count, block_size, num_tokens, release))
 
 
@@ -135,7 +129,7 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, codes: torc
     Slots outside the cache are skipped. A key or value that is not finite makes the scale of its (block, head) NaN, so that what
     attends to it is NaN. Not differentiable (the cache belongs to inference)."""
     ks, c = k.shape, codes.shape
-    if not (_cache_ok(codes, scales) and len(ks) == 3 and ks == v.shape and k.dtype == v.dtype and k.dtype in FLOAT_TYPES
+    if not (_cache_ok(codes, c, scales) and len(ks) == 3 and ks == v.shape and k.dtype == v.dtype and k.dtype in FLOAT_TYPES
             and ks[1] == c[2] and ks[2] == c[4] and slots.dtype == torch.int64 and slots.is_contiguous() and slots.shape == ks[:1]):
         _refuse_cache(codes, scales)
         _need(k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype and k.dtype in FLOAT_TYPES,
@@ -148,7 +142,7 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, codes: torc
     if ks[0] == 0:
         return
     if dev >= 0:
-        kv8_cuda.write(k, v, slots, codes, scales, dev)
+        kv8_cuda.write(k, v, slots, codes, scales, dev, ks, c)
     else:
         with torch.no_grad():
             _ref.kv8_write(k, v, slots, codes, scales)
@@ -160,9 +154,10 @@ def attention_decode_kv8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Ten
     fp16 or fp32) -> the same shape and type, contiguous. Query head i reads kv head i // (q heads / kv heads). A request without
     tokens gives zeros; bytes behind the last token are not looked at; a block outside the cache counts as not there. ``scale``
     defaults to head_dim ** -0.5. Inference only (no gradient)."""
-    qs, c = q.shape, codes.shape
-    if not (_cache_ok(codes, scales) and _table_ok(table, lens) and len(qs) == 3 and q.dtype in FLOAT_TYPES
-            and qs[0] == table.shape[0] and qs[2] == c[4] and qs[1] > 0 and qs[1] % c[2] == 0 and table.shape[1] * c[3] < 1 << 31):
+    qs, c, ts = q.shape, codes.shape, table.shape
+    if not (_cache_ok(codes, c, scales) and len(qs) == 3 and len(ts) == 2 and q.dtype in FLOAT_TYPES and qs[0] == ts[0] and ts[1] > 0
+            and table.dtype == lens.dtype == torch.int32 and table.stride(1) == 1 and lens.is_contiguous() and lens.shape == ts[:1]
+            and qs[2] == c[4] and qs[1] > 0 and qs[1] % c[2] == 0 and ts[1] * c[3] < 1 << 31):
         _refuse_cache(codes, scales)
         _refuse_table(table, lens)
         _need(q.dim() == 3 and q.dtype in FLOAT_TYPES, "q: bf16, fp16 or fp32 [requests, heads, head_dim]")
@@ -177,6 +172,6 @@ def attention_decode_kv8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Ten
     if qs[0] == 0:
         return torch.empty_like(q)
     if dev >= 0:
-        return kv8_cuda.attention_decode(q, codes, scales, table, lens, scale, dev)
+        return kv8_cuda.attention_decode(q, codes, scales, table, lens, scale, dev, qs, c, ts[1])
     with torch.no_grad():
         return _ref.attention_decode_kv8(q, codes, scales, table, lens, scale)

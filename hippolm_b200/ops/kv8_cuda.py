@@ -13,6 +13,7 @@ from ._ext import check, lib
 DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _stream = torch._C._cuda_getCurrentRawStream            # the handle of a device's current stream
 _current = torch.cuda.current_device
+ONE_BLOCK_TOKENS = 16384
 _FNS: dict = {}
 _SMS: dict = {}
 
@@ -35,17 +36,18 @@ def launch(name: str, dev: int, block: bytes) -> None:
         check(fn(block), name)
 
 
-def plan(table, lens, new_lens, free_list, free_count, block_size, num_tokens, release, dev: int):
-    N, M = table.shape
-    slots = torch.empty(num_tokens, dtype=torch.int64, device=table.device)
+def plan(table, lens, new_lens, free_list, free_count, block_size, num_tokens, release, dev: int, shape):
+    N, M = shape
+    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
     lens_out, count = torch.empty_like(lens), torch.empty_like(free_count)
-    served = torch.empty(N, dtype=torch.bool, device=table.device)
-    cu = torch.empty(N + 1, dtype=torch.int32, device=table.device)
+    served = torch.empty(N, dtype=torch.bool, device=dev) if release is None else torch.empty_like(release)
+    # prompts: the slots are laid out by a kernel of their own, which looks requests up by the ends of their tokens
+    cu = torch.empty(N + 1, dtype=torch.int32, device=dev) if num_tokens > ONE_BLOCK_TOKENS else None
     launch("kv8_plan", dev, _PLAN.pack(
         table.data_ptr(), lens.data_ptr(), new_lens.data_ptr(), free_list.data_ptr(), free_count.data_ptr(),
         0 if release is None else release.data_ptr(), slots.data_ptr(), lens_out.data_ptr(), count.data_ptr(), served.data_ptr(),
-        cu.data_ptr(), _stream(dev), table.stride(0), num_tokens, M, N, free_list.numel(), block_size))
-    return slots, lens_out, count, served, cu
+        0 if cu is None else cu.data_ptr(), _stream(dev), table.stride(0), num_tokens, M, N, free_list.numel(), block_size))
+    return slots, lens_out, count, served
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -57,30 +59,28 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x
 
 
-def write(k, v, slots, codes, scales, dev: int, form: int = 0):
+def write(k, v, slots, codes, scales, dev: int, ks, cs, form: int = 0):
     """``form``: 0 by size, 1 a warp for each run of tokens, 2 a block for each window of tokens (tests)."""
-    T, H, D = k.shape
+    T, H, D = ks
     if D != 128 and D != 64:
         raise ValueError(f"head_dim {D}: the CUDA cache supports 64 and 128")
     k, v = _rows(k), _rows(v)
     (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
-    _, blocks, _, bs, _ = codes.shape
+    _, blocks, _, bs, _ = cs
     launch("kv8_write", dev, _WRITE.pack(
         k.data_ptr(), v.data_ptr(), slots.data_ptr(), codes.data_ptr(), scales.data_ptr(), _stream(dev), kt, kh, vt, vh, T, blocks,
         H, D, bs, DTYPE[k.dtype], codes.dtype != torch.int8, form))
 
 
-def attention_decode(q, codes, scales, table, lens, scale: float, dev: int):
-    N, Hq, D = q.shape
-    _, blocks, H, bs, _ = codes.shape
+def attention_decode(q, codes, scales, table, lens, scale: float, dev: int, qs, cs, M: int):
+    N, Hq, D = qs
+    _, blocks, H, bs, _ = cs
     if D != 128 and D != 64:
         raise ValueError(f"head_dim {D}: the CUDA cache supports 64 and 128")
     if 2 * blocks * H * bs >= 1 << 31:
         raise ValueError("the cache has 2^31 rows or more")
     q = _rows(q)
     qn, qh, _ = q.stride()
-    ld, _ = table.stride()
-    M = table.shape[1]
     G = Hq // H
     groups, tiles = N * H * (-(-G // 8)), -(-M * bs // 32)
     if groups * (tiles + 1) >= 1 << 31:
@@ -90,9 +90,9 @@ def attention_decode(q, codes, scales, table, lens, scale: float, dev: int):
         sms = _SMS[dev] = torch.cuda.get_device_properties(dev).multi_processor_count
     # a warp takes tiles of 32 tokens; three blocks of four warps fill a multiprocessor
     workers = 4 * min(3 * sms, -(-(groups * tiles) // 4))
-    ws = torch.empty(workers * (2 * min(G, 8) * (D + 2) + 4), dtype=torch.float32, device=q.device)
-    out = torch.empty((N, Hq, D), dtype=q.dtype, device=q.device)
+    ws = torch.empty(workers * (2 * min(G, 8) * (D + 2) + 4), dtype=torch.float32, device=dev)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     launch("kv8_attention", dev, _ATTEND.pack(
         q.data_ptr(), out.data_ptr(), codes.data_ptr(), scales.data_ptr(), table.data_ptr(), lens.data_ptr(), ws.data_ptr(),
-        _stream(dev), qn, qh, ld, blocks, N, H, Hq, D, bs, M, DTYPE[q.dtype], codes.dtype != torch.int8, workers, scale))
+        _stream(dev), qn, qh, table.stride(0), blocks, N, H, Hq, D, bs, M, DTYPE[q.dtype], codes.dtype != torch.int8, workers, scale))
     return out

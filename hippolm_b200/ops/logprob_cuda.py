@@ -19,7 +19,7 @@ def _rows(z: torch.Tensor) -> torch.Tensor:
 def forward(logits, ids, top_k: int, keep: bool, dev: int):
     """``keep``: also the statistics (maximum, log of the sum behind it) that the backward pass reads."""
     T, V = logits.shape
-    z, ids, d = _rows(logits), ids.contiguous(), logits.device
+    z, ids, d = _rows(logits), ids.contiguous(), dev
     lp = torch.empty(T, dtype=torch.float32, device=d)
     ent = torch.empty_like(lp)
     stat = torch.empty((T, 2), dtype=torch.float32, device=d) if keep else None

@@ -67,8 +67,7 @@ def kv8_plan(table, lens, new_lens, free_list, free_count, block_size: int, num_
             b = int(table[n, p // block_size])
             slots[start + i] = b * block_size + p % block_size if b >= 0 else -1
     i32 = dict(dtype=torch.int32)
-    return (slots, torch.tensor(out, **i32), torch.tensor([count - used], **i32), torch.tensor(served, dtype=torch.bool),
-            torch.tensor(cu, **i32))
+    return slots, torch.tensor(out, **i32), torch.tensor([count - used], **i32), torch.tensor(served, dtype=torch.bool)
 
 
 def _write_run(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, off: int) -> None:

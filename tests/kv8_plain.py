@@ -108,7 +108,7 @@ def check_attend(got, q, codes, scales, table, lens, scale):
 
 
 def plan(table, lens, new, free, count, bs, tokens, release=None):
-    """The plan by lists: -> (slots, lens, count, served, cu, table, free) as python lists."""
+    """The plan by lists: -> (slots, lens, count, served, table, free) as python lists."""
     table, free = [list(map(int, r)) for r in table.tolist()], list(map(int, free.tolist()))
     M = len(table[0])
     lens = [min(max(int(x), 0), M * bs) for x in lens.tolist()]
@@ -143,7 +143,7 @@ def plan(table, lens, new, free, count, bs, tokens, release=None):
             b = table[n][p // bs]
             slots[end - new[n] + i] = b * bs + p % bs if b >= 0 else -1
         lens[n] += new[n]
-    return slots, lens, [len(stack)], served, cu, table, mem
+    return slots, lens, [len(stack)], served, table, mem
 
 
 def scores(logits, ids, top):

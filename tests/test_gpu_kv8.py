@@ -60,7 +60,7 @@ def test_write_matches_64_bits(kind, D, bs, form):
         dt = dtypes[(runs + bs // 16) % 3]
         k, v = ((torch.randn(slots.numel(), 3, D, generator=g) * 20 ** float(i)).to(dt) for i in range(2))
         k, v, slots = to(DEV, k, v, slots)
-        check_write(k, v, slots, codes, scales, kind, write=lambda *a: kv8_cuda.write(*a, 0, form=form))
+        check_write(k, v, slots, codes, scales, kind, write=lambda *a: kv8_cuda.write(*a, 0, a[0].shape, a[3].shape, form=form))
 
 
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
@@ -74,7 +74,7 @@ def test_write_poison_zeros_far_slots_and_strides(kind, form):
     qkv = qkv.to(DEV)
     k, v = qkv[..., :64], qkv[..., 64:128]                                    # strided heads
     slots = torch.tensor([5, 16, 17, 4 * 16, 2 * 16, 1 << 40, 3 * 16], device=DEV)
-    write = lambda *a: kv8_cuda.write(*a, 0, form=form)                         # noqa: E731
+    write = lambda *a: kv8_cuda.write(*a, 0, a[0].shape, a[3].shape, form=form)                         # noqa: E731
     check_write(k, v, slots, codes, scales, kind, write=write)
     check_write(k[5:6], v[5:6], torch.tensor([18], device=DEV), codes, scales, kind, write=write)
     check_write(k[5:6], v[5:6], torch.tensor([16], device=DEV), codes, scales, kind, write=write)
