@@ -268,114 +268,98 @@ __device__ __forceinline__ bool continues(const WriteArgs& a, long long prev, lo
   return slot_ok(a, prev) && s == prev + 1 && (s & ((1 << a.sh) - 1)) != 0;
 }
 
-// One warp for a (run of tokens in a block, head, half): the form for few tokens (decoding), where every token is a run of its own.
-// Warps whose token is not the first of a run leave at once.
-template <typename T, int D, int E4M3>
-__global__ void __launch_bounds__(256) kv8_write_rows_kernel(WriteArgs a) {
-  constexpr int LPR = D / 8, RPW = 32 / LPR;         // lanes a row, rows of a warp's load
-  const int lane = threadIdx.x & 31;
-  const long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int half = blockIdx.y;
-  const long long t = u / a.H;
-  const int h = (int)(u - t * a.H);
-  if (t >= a.T) return;
-  const long long s = a.slots[t];
-  if (!slot_ok(a, s) || (t > 0 && continues(a, a.slots[t - 1], s))) return;
-  const int bs = 1 << a.sh, off = (int)(s & (bs - 1));
-  const T* x = (const T*)(half ? a.v : a.k) + t * (half ? a.v_t : a.k_t) + h * (half ? a.v_h : a.k_h);
-  const long long ld = half ? a.v_t : a.k_t;
-  const int r0 = lane / LPR, col = (lane % LPR) * 8;
-  const long long bh = (s >> a.sh) * a.H + h;
-  float* scale = a.scales + half * a.half_scales + bh;
-  uint8_t* codes = a.codes + half * a.half_codes + (bh << a.sh) * D;
-  // length of the run
-  int L = 1;
-  for (int base = 1; base < bs - off; base += 32) {
-    const long long i = base + lane;
-    const bool go = off + i < bs && t + i < a.T && a.slots[t + i] == s + i;
-    const unsigned m = __ballot_sync(0xffffffffu, go);
-    if (m != 0xffffffffu) { L = base + __ffs(~m) - 1; break; }
-    L = base + 32;
-  }
-  const float old = off ? *scale : 0.f;
-  constexpr int U = 4;
-  Row8<T> keep[U];                                   // the first U * RPW rows stay in registers between the two passes
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int r = r0 + i * RPW;
-    if (r < L) keep[i].load(x + r * ld + col); else keep[i].zero();
-  }
-#pragma unroll
-  for (int i = 0; i < U; ++i) m = keep[i].amax(m);
-  for (int r = r0 + U * RPW; r < L; r += RPW) {
-    Row8<T> row;
-    row.load(x + r * ld + col);
-    m = row.amax(m);
-  }
-  m = __reduce_max_sync(0xffffffffu, Row8<T>::bits(m));
-  const RunScale rs = run_scale<E4M3>(m, old, off > 0);
-  if (rs.down < 0) shift_codes<E4M3>(codes, off * D, rs.down, lane, 32);
-  const float inv = pow2f(-rs.e);
-#pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int r = r0 + i * RPW;
-    if (r < L) *(uint2*)(codes + (off + r) * D + col) = encode_row<E4M3>(keep[i], inv, rs.bad);
-  }
-  for (int r = r0 + U * RPW; r < L; r += RPW) {
-    Row8<T> row;
-    row.load(x + r * ld + col);
-    *(uint2*)(codes + (off + r) * D + col) = encode_row<E4M3>(row, inv, rs.bad);
-  }
-  if (lane == 0) *scale = rs.bad ? __uint_as_float(0x7fffffffu) : pow2f(rs.e);
-}
+// One CTA for the runs that start in a window of W tokens, and for kPairs (head, half) pairs. It finds the runs (consecutive tokens in
+// consecutive slots of one block) by ballots. Runs of up to kShort tokens (decoding: one) go to groups of lanes that hold a row, 128 /
+// (D / 8) of them at work; longer runs (prompts) are read once into registers by the whole CTA, the next pair's rows in flight while
+// this one's are reduced and stored. HBM-bound for prompts (bytes = 2 T H D (element + 1)), latency for a token a request.
+// The window is small for few tokens, which spreads them over the card, and a block's tokens for many.
+constexpr int kPairs = 4, kShort = 4;
 
-// One CTA for the runs that start in a window of bs tokens, of a group of (head, half) pairs: the form for prompts. The run is found
-// once; then the pairs follow each other, the next one's rows (at most bs) in flight while this one's are reduced over the CTA and
-// stored from registers. HBM-bound, bytes = T * H * D * (element + 1) a half.
-constexpr int kPairs = 8;
+template <typename T, int D, int E4M3, int BS> struct WriteShape {
+  static constexpr int kBytes = BS * D * (int)sizeof(T);                 // a run at most
+  static constexpr int kBlocks = kBytes <= 4096 ? 8 : kBytes <= 8192 ? 6 : kBytes <= 16384 ? 5 : 3;    // what the registers allow
+};
+
 template <typename T, int D, int E4M3, int BS>
-__global__ void __launch_bounds__(128) kv8_write_blocks_kernel(WriteArgs a) {
+__global__ void __launch_bounds__(128, WriteShape<T, D, E4M3, BS>::kBlocks) kv8_write_kernel(WriteArgs a, int W) {
   constexpr int LPR = D / 8, RPP = 128 / LPR, P = (BS + RPP - 1) / RPP;   // lanes a row, rows a pass, passes
   __shared__ unsigned s_cont[4];                     // bit i: token w0 + i continues the run of the token before it
-  __shared__ unsigned s_ok[4];
+  __shared__ int s_run[BS], s_n[2];                  // first token | length << 8: short runs from the front, long ones from the back
   __shared__ uint32_t s_max[2][4];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int first = blockIdx.y * kPairs, last = min(first + kPairs, 2 * a.H);
-  const long long w0 = (long long)blockIdx.x * BS;
+  const long long w0 = (long long)blockIdx.x * W;
   bool ok = false, cont = false;
-  if (tid < 2 * BS && w0 + tid < a.T) {
+  if (tid < W + BS && w0 + tid < a.T) {
     const long long s = a.slots[w0 + tid], prev = w0 + tid > 0 ? a.slots[w0 + tid - 1] : -1;
     ok = slot_ok(a, s);
     cont = ok && continues(a, prev, s);
   }
-  const unsigned bc = __ballot_sync(0xffffffffu, cont), bo = __ballot_sync(0xffffffffu, ok);
-  if (lane == 0) { s_cont[w] = bc; s_ok[w] = bo; }
+  const unsigned bc = __ballot_sync(0xffffffffu, cont);
+  if (lane == 0) s_cont[w] = bc;
+  if (tid < 2) s_n[tid] = 0;
   __syncthreads();
-  const unsigned long long c0 = s_cont[0] | ((unsigned long long)s_cont[1] << 32), c1 = s_cont[2] | ((unsigned long long)s_cont[3] << 32);
-  unsigned long long heads = (s_ok[0] | ((unsigned long long)s_ok[1] << 32)) & ~c0;
-  if (BS < 64) heads &= (1ull << (BS & 63)) - 1;
-  const int r0 = tid / LPR, col = (tid % LPR) * 8;
-  for (; heads; heads &= heads - 1) {
-    const int i0 = __ffsll(heads) - 1;
-    // consecutive "continues" bits behind i0
-    const unsigned long long rest = i0 == 63 ? c1 : (c0 >> (i0 + 1)) | (c1 << (63 - i0));
+  if (tid < W && ok && !cont) {                      // the first token of a run: consecutive bits behind it
+    const unsigned long long c0 = s_cont[0] | ((unsigned long long)s_cont[1] << 32), c1 = s_cont[2] | ((unsigned long long)s_cont[3] << 32);
+    const unsigned long long rest = tid == 63 ? c1 : (c0 >> (tid + 1)) | (c1 << (63 - tid));
     const int L = min(~rest ? __ffsll(~rest) : 64, BS);
-    const long long t = w0 + i0, s = a.slots[t];
+    if (L <= kShort) s_run[atomicAdd(&s_n[0], 1)] = tid | L << 8;        // (runs are independent: their order does not matter)
+    else s_run[BS - 1 - atomicAdd(&s_n[1], 1)] = tid | L << 8;
+  }
+  __syncthreads();
+  const int shorts = s_n[0], longs = s_n[1];
+  const int r0 = tid / LPR, col = (tid % LPR) * 8;
+
+  auto source = [&](int pair, long long t) {
+    const int h = pair >> 1;
+    return pair & 1 ? (const T*)a.v + t * a.v_t + h * a.v_h + col : (const T*)a.k + t * a.k_t + h * a.k_h + col;
+  };
+  for (int u = r0; u < shorts * (last - first); u += RPP) {
+    const int run = s_run[u / (last - first)], pair = first + u % (last - first), L = run >> 8;
+    const long long t = w0 + (run & 255), s = a.slots[t];
+    const int off = (int)(s & (BS - 1));
+    const long long bh = (s >> a.sh) * a.H + (pair >> 1), ld = pair & 1 ? a.v_t : a.k_t;
+    float* scale = a.scales + (pair & 1 ? a.half_scales : 0) + bh;
+    uint8_t* codes = a.codes + (pair & 1 ? a.half_codes : 0) + bh * BS * D;
+    const T* x = source(pair, t);
+    Row8<T> row[kShort];
+#pragma unroll
+    for (int i = 0; i < kShort; ++i)
+      if (i < L) row[i].load(x + i * ld); else row[i].zero();
+    const float old = off ? *scale : 0.f;
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kShort; ++i) m = row[i].amax(m);
+    m = Row8<T>::bits(m);
+    const unsigned group = (LPR == 16 ? 0xffffu : 0xffu) << (lane & ~(LPR - 1) & 31);
+#pragma unroll
+    for (int d = 1; d < LPR; d <<= 1) m = max(m, __shfl_xor_sync(group, m, d));
+    const RunScale rs = run_scale<E4M3>(m, old, off > 0);
+    if (rs.down < 0) shift_codes<E4M3>(codes, off * D, rs.down, tid % LPR, LPR);
+    const float inv = pow2f(-rs.e);
+#pragma unroll
+    for (int i = 0; i < kShort; ++i)
+      if (i < L) *(uint2*)(codes + (off + i) * D + col) = encode_row<E4M3>(row[i], inv, rs.bad);
+    __syncwarp(group);                               // every lane has read the old scale
+    if (tid % LPR == 0) *scale = rs.bad ? __uint_as_float(0x7fffffffu) : pow2f(rs.e);
+  }
+
+  for (int q = 0; q < longs; ++q) {
+    const int run = s_run[BS - 1 - q], L = run >> 8;
+    const long long t = w0 + (run & 255), s = a.slots[t];
     const int off = (int)(s & (BS - 1));
     const long long block = (s >> a.sh) * a.H;
     Row8<T> next[P];
     float next_old = 0.f;
     auto load = [&](int pair) {
-      const int h = pair >> 1, half = pair & 1;
-      const T* x = (const T*)(half ? a.v : a.k) + t * (half ? a.v_t : a.k_t) + h * (half ? a.v_h : a.k_h) + col;
-      const long long ld = half ? a.v_t : a.k_t;
+      const T* x = source(pair, t);
+      const long long ld = pair & 1 ? a.v_t : a.k_t;
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         const int r = r0 + p * RPP;
         if (r < L) next[p].load(x + r * ld); else next[p].zero();
       }
-      if (off) next_old = a.scales[half * a.half_scales + block + h];
+      if (off) next_old = a.scales[(pair & 1 ? a.half_scales : 0) + block + (pair >> 1)];
     };
     load(first);
     for (int pair = first; pair < last; ++pair) {
@@ -384,8 +368,8 @@ __global__ void __launch_bounds__(128) kv8_write_blocks_kernel(WriteArgs a) {
       for (int p = 0; p < P; ++p) row[p] = next[p];
       const float old = next_old;
       if (pair + 1 < last) load(pair + 1);
-      const int h = pair >> 1, half = pair & 1;
-      uint8_t* codes = a.codes + half * a.half_codes + (block + h) * BS * D;
+      const long long bh = block + (pair >> 1);
+      uint8_t* codes = a.codes + (pair & 1 ? a.half_codes : 0) + bh * BS * D;
       uint32_t m = 0;
 #pragma unroll
       for (int p = 0; p < P; ++p) m = row[p].amax(m);
@@ -402,32 +386,29 @@ __global__ void __launch_bounds__(128) kv8_write_blocks_kernel(WriteArgs a) {
         const int r = r0 + p * RPP;
         if (r < L) *(uint2*)(codes + (off + r) * D + col) = encode_row<E4M3>(row[p], inv, rs.bad);
       }
-      if (tid == 0) a.scales[half * a.half_scales + block + h] = rs.bad ? __uint_as_float(0x7fffffffu) : pow2f(rs.e);
+      if (tid == 0) a.scales[(pair & 1 ? a.half_scales : 0) + bh] = rs.bad ? __uint_as_float(0x7fffffffu) : pow2f(rs.e);
     }
     __syncthreads();                                 // s_max is free for the next run
   }
 }
 
-// The rows form wins while a token is a run of its own or there are few of them; a prompt's warps mostly leave at once there.
-constexpr long long kRowsMaxTokens = 2048;
-
-template <typename T, int D, int E4M3> int launch_write(const WriteArgs& a, int form, cudaStream_t st) {
-  const bool rows = form == 1 || (form == 0 && a.T <= kRowsMaxTokens);
-  if (rows) {
-    const long long g = (a.T * a.H + 7) / 8;
-    if (g > 0x7fffffffll) return -2;
-    kv8_write_rows_kernel<T, D, E4M3><<<dim3((unsigned)g, 2), 256, 0, st>>>(a);
-    return (int)cudaGetLastError();
+template <typename T, int D, int E4M3> int launch_write(const WriteArgs& a, int window, cudaStream_t st) {
+  const int bs = 1 << a.sh, groups = (2 * a.H + kPairs - 1) / kPairs;
+  int W = window;
+  if (W == 0) {                                      // some two thousand blocks, or a window of a whole block's tokens
+    W = 4;
+    while (W < bs && (a.T + W - 1) / W * groups > 2048) W *= 2;
   }
-  const dim3 grid((unsigned)((a.T + (1 << a.sh) - 1) >> a.sh), (unsigned)((2 * a.H + kPairs - 1) / kPairs));
-  if (a.sh == 4) kv8_write_blocks_kernel<T, D, E4M3, 16><<<grid, 128, 0, st>>>(a);
-  else if (a.sh == 5) kv8_write_blocks_kernel<T, D, E4M3, 32><<<grid, 128, 0, st>>>(a);
-  else kv8_write_blocks_kernel<T, D, E4M3, 64><<<grid, 128, 0, st>>>(a);
+  if (W < 1 || W > bs) return -1;
+  const dim3 grid((unsigned)((a.T + W - 1) / W), (unsigned)groups);
+  if (a.sh == 4) kv8_write_kernel<T, D, E4M3, 16><<<grid, 128, 0, st>>>(a, W);
+  else if (a.sh == 5) kv8_write_kernel<T, D, E4M3, 32><<<grid, 128, 0, st>>>(a, W);
+  else kv8_write_kernel<T, D, E4M3, 64><<<grid, 128, 0, st>>>(a, W);
   return (int)cudaGetLastError();
 }
-template <typename T> int dispatch_write(const WriteArgs& a, int D, int e4m3, int form, cudaStream_t st) {
-  if (D == 128) return e4m3 ? launch_write<T, 128, 1>(a, form, st) : launch_write<T, 128, 0>(a, form, st);
-  if (D == 64) return e4m3 ? launch_write<T, 64, 1>(a, form, st) : launch_write<T, 64, 0>(a, form, st);
+template <typename T> int dispatch_write(const WriteArgs& a, int D, int e4m3, int window, cudaStream_t st) {
+  if (D == 128) return e4m3 ? launch_write<T, 128, 1>(a, window, st) : launch_write<T, 128, 0>(a, window, st);
+  if (D == 64) return e4m3 ? launch_write<T, 64, 1>(a, window, st) : launch_write<T, 64, 0>(a, window, st);
   return -1;
 }
 }  // namespace hippo
@@ -459,12 +440,12 @@ extern "C" int hippo_kv8_plan(const KvPlanCall* c) {
   return (int)cudaGetLastError();
 }
 
-// k / v: [T][H][D] with strides (elements); dtype 0 bf16, 1 fp16, 2 fp32; codes / scales of `blocks` blocks; form 0 = by size,
-// 1 = a warp a run, 2 = a CTA a window of block_size tokens.
+// k / v: [T][H][D] with strides (elements); dtype 0 bf16, 1 fp16, 2 fp32; codes / scales of `blocks` blocks; window: tokens a
+// CTA looks through (1 .. block_size), 0 = by size.
 struct KvWriteCall {
   const void *k, *v; const long long* slots; void* codes; float* scales; void* stream;
   long long k_t, k_h, v_t, v_h, T, blocks;
-  int H, D, block_size, dtype, e4m3, form;
+  int H, D, block_size, dtype, e4m3, window;
 };
 extern "C" int hippo_kv8_write(const KvWriteCall* c) {
   if (c->T <= 0) return 0;
@@ -473,8 +454,8 @@ extern "C" int hippo_kv8_write(const KvWriteCall* c) {
   WriteArgs a{c->k, c->v, c->k_t, c->k_h, c->v_t, c->v_h, c->slots, c->T, c->blocks << sh, (uint8_t*)c->codes, c->scales, c->H, sh,
               ((c->blocks * c->H) << sh) * c->D, c->blocks * c->H};
   cudaStream_t st = (cudaStream_t)c->stream;
-  if (c->dtype == 0) return dispatch_write<__nv_bfloat16>(a, c->D, c->e4m3, c->form, st);
-  if (c->dtype == 1) return dispatch_write<__half>(a, c->D, c->e4m3, c->form, st);
-  if (c->dtype == 2) return dispatch_write<float>(a, c->D, c->e4m3, c->form, st);
+  if (c->dtype == 0) return dispatch_write<__nv_bfloat16>(a, c->D, c->e4m3, c->window, st);
+  if (c->dtype == 1) return dispatch_write<__half>(a, c->D, c->e4m3, c->window, st);
+  if (c->dtype == 2) return dispatch_write<float>(a, c->D, c->e4m3, c->window, st);
   return -1;
 }

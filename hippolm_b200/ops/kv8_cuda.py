@@ -59,8 +59,8 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x
 
 
-def write(k, v, slots, codes, scales, dev: int, ks, cs, form: int = 0):
-    """``form``: 0 by size, 1 a warp for each run of tokens, 2 a block for each window of tokens (tests)."""
+def write(k, v, slots, codes, scales, dev: int, ks, cs, window: int = 0):
+    """``window``: tokens that a block looks through, 0 by size (tests give it)."""
     T, H, D = ks
     if D != 128 and D != 64:
         raise ValueError(f"head_dim {D}: the CUDA cache supports 64 and 128")
@@ -69,7 +69,7 @@ def write(k, v, slots, codes, scales, dev: int, ks, cs, form: int = 0):
     _, blocks, _, bs, _ = cs
     launch("kv8_write", dev, _WRITE.pack(
         k.data_ptr(), v.data_ptr(), slots.data_ptr(), codes.data_ptr(), scales.data_ptr(), _stream(dev), kt, kh, vt, vh, T, blocks,
-        H, D, bs, DTYPE[k.dtype], codes.dtype != torch.int8, form))
+        H, D, bs, DTYPE[k.dtype], codes.dtype != torch.int8, window))
 
 
 def attention_decode(q, codes, scales, table, lens, scale: float, dev: int, qs, cs, M: int):

@@ -49,8 +49,8 @@ def test_plan_of_a_strided_table():
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("bs", [16, 32, 64])
-@pytest.mark.parametrize("form", [1, 2])
-def test_write_matches_64_bits(kind, D, bs, form):
+@pytest.mark.parametrize("window", [0, 5, 16])
+def test_write_matches_64_bits(kind, D, bs, window):
     from hippolm_b200.ops import kv8_cuda
     dtypes = [torch.bfloat16, torch.float16, torch.float32]
     for runs in range(len(WRITE_RUNS)):
@@ -60,12 +60,12 @@ def test_write_matches_64_bits(kind, D, bs, form):
         dt = dtypes[(runs + bs // 16) % 3]
         k, v = ((torch.randn(slots.numel(), 3, D, generator=g) * 20 ** float(i)).to(dt) for i in range(2))
         k, v, slots = to(DEV, k, v, slots)
-        check_write(k, v, slots, codes, scales, kind, write=lambda *a: kv8_cuda.write(*a, 0, a[0].shape, a[3].shape, form=form))
+        check_write(k, v, slots, codes, scales, kind, write=lambda *a: kv8_cuda.write(*a, 0, a[0].shape, a[3].shape, window=window))
 
 
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
-@pytest.mark.parametrize("form", [1, 2])
-def test_write_poison_zeros_far_slots_and_strides(kind, form):
+@pytest.mark.parametrize("window", [0, 2, 16])
+def test_write_poison_zeros_far_slots_and_strides(kind, window):
     from hippolm_b200.ops import kv8_cuda
     codes, scales, g = cache_case(0, kind, 2, 64, 16, 4)
     codes, scales = codes.to(DEV), scales.to(DEV)
@@ -74,7 +74,7 @@ def test_write_poison_zeros_far_slots_and_strides(kind, form):
     qkv = qkv.to(DEV)
     k, v = qkv[..., :64], qkv[..., 64:128]                                    # strided heads
     slots = torch.tensor([5, 16, 17, 4 * 16, 2 * 16, 1 << 40, 3 * 16], device=DEV)
-    write = lambda *a: kv8_cuda.write(*a, 0, a[0].shape, a[3].shape, form=form)                         # noqa: E731
+    write = lambda *a: kv8_cuda.write(*a, 0, a[0].shape, a[3].shape, window=window)                         # noqa: E731
     check_write(k, v, slots, codes, scales, kind, write=write)
     check_write(k[5:6], v[5:6], torch.tensor([18], device=DEV), codes, scales, kind, write=write)
     check_write(k[5:6], v[5:6], torch.tensor([16], device=DEV), codes, scales, kind, write=write)
@@ -82,10 +82,38 @@ def test_write_poison_zeros_far_slots_and_strides(kind, form):
     check_write(odd, odd, torch.tensor([32, 33], device=DEV), codes, scales, kind, write=write)
 
 
+@pytest.mark.parametrize("kind,bs", [("e4m3", 64), ("int8", 16)])
+def test_write_of_many_runs_equals_a_few(kind, bs):
+    """One call with thousands of short and long runs against calls with a few of them each (other windows)."""
+    g = torch.Generator().manual_seed(bs)
+    runs, block = [], 0
+    while sum(r[2] for r in runs) < 6000:
+        off = int(torch.randint(0, bs, (1,), generator=g)) if torch.rand(1, generator=g) < 0.7 else 0
+        ln = 1 if torch.rand(1, generator=g) < 0.5 else int(torch.randint(1, bs - off + 1, (1,), generator=g))
+        runs.append((block, off, ln))
+        block += 1
+    codes, scales = kv8_empty(block, 3, 64, bs, kind, DEV)
+    codes.view(torch.int8).copy_(torch.randint(-100, 100, codes.shape, generator=g).to(torch.int8))
+    scales.mul_(0.01).copy_(torch.exp2(torch.randint(-9, 2, scales.shape, generator=g).float()))
+    slots = runs_to_slots(runs, bs)
+    k, v = (torch.randn(slots.numel(), 3, 64, generator=g).bfloat16().to(DEV) for _ in range(2))
+    other_c, other_s = codes.clone(), scales.clone()
+    ops.kv8_write(k, v, slots.to(DEV), codes, scales)
+    at = 0
+    for i in range(0, len(runs), 9):
+        n = sum(r[2] for r in runs[i:i + 9])
+        ops.kv8_write(k[at:at + n], v[at:at + n], slots[at:at + n].to(DEV), other_c, other_s)
+        at += n
+    assert torch.equal(codes.view(torch.int8), other_c.view(torch.int8)) and torch.equal(scales, other_s)
+    few = slots[:300]
+    c0, s0 = kv8_empty(block, 3, 64, bs, kind, DEV)
+    check_write(k[:300], v[:300], few.to(DEV), c0, s0, kind)
+
+
 def test_write_leaves_the_rest_of_the_cache():
     codes, scales = kv8_empty(60, 2, 64, 64, "int8", DEV)
     codes.fill_(77); scales.fill_(0.5)
-    T = 3000                                                                  # above the size rule: the window form
+    T = 3000                                                                  # windows of whole blocks
     slots = torch.arange(T, device=DEV) + 64
     k = torch.randn(T, 2, 64, device=DEV)
     c0, s0 = codes.clone(), scales.clone()
