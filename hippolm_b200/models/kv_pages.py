@@ -1,0 +1,55 @@
+"""Pages of the 8-bit key / value caches of a batch that is being decoded (``ops/kv8.py``).
+
+One block table serves all full-attention layers: block b of a request is block b of every layer's cache. The reference keeps no
+cache (``src/models/model.py:180-219`` re-runs the forward for every token)."""
+from __future__ import annotations
+
+from typing import List, Optional, Sequence
+
+import torch
+
+from .. import ops
+
+
+class KV8Pages:
+    """Block table, lengths and free blocks of ``len(limits)`` sequences of at most ``limits[n]`` tokens each. The pool has exactly
+    the blocks that they can need, so every plan is served; a sequence in ``release`` gives its blocks back and stores nothing."""
+
+    def __init__(self, limits: Sequence[int], block_size: int = 64, device=None):
+        need = [-(-max(x, 0) // block_size) for x in limits]
+        i32 = dict(dtype=torch.int32, device=device)
+        self.block_size, self.blocks = block_size, max(1, sum(need))
+        self.table = torch.full((len(need), max([1] + need)), -1, **i32)
+        self.lens = torch.zeros(len(need), **i32)
+        self.free = torch.arange(self.blocks - 1, -1, -1, **i32)
+        self.free_count = torch.full((1,), self.blocks, **i32)
+        self.release: Optional[torch.Tensor] = None       # bool [sequences], read by the next plan
+        self.slots: Optional[torch.Tensor] = None         # of the tokens of the pass that was planned last
+        self.passes = 0
+
+    def plan(self, cu_seqlens: torch.Tensor, num_tokens: int) -> None:
+        """Slots for the tokens of the next pass, ``cu_seqlens`` [sequences + 1] packed: the whole prompts first, then one token a
+        sequence and pass. Sequences in ``release`` have their rows in the stream like the others."""
+        new = (cu_seqlens[1:] - cu_seqlens[:-1]).to(torch.int32)
+        p = ops.kv8_plan(self.table, self.lens, new, self.free, self.free_count, self.block_size, num_tokens, release=self.release)
+        self.slots, self.lens, self.free_count = p.slots, p.lens, p.free_count
+        self.passes += 1
+
+    def attend(self, q, k, v, codes, scales, scale: float) -> Optional[torch.Tensor]:
+        """Stores the pass's keys and values and, from the second pass on, returns the attention over each sequence's tokens (the
+        prompts themselves attend to their unquantised keys: None)."""
+        ops.kv8_write(k, v.to(k.dtype), self.slots, codes, scales)
+        if self.passes == 1:
+            return None
+        if q.shape[0] != self.table.shape[0]:
+            raise ValueError("the cache takes whole prompts first, then one token per sequence and step")
+        return ops.attention_decode_kv8(q, codes, scales, self.table, self.lens, scale)
+
+
+def layer_cache(pages: KV8Pages, heads: int, head_dim: int, dtype: str, device=None) -> dict:
+    codes, scales = ops.kv8_empty(pages.blocks, heads, head_dim, pages.block_size, dtype, device)
+    return {"pages": pages, "codes": codes, "scales": scales}
+
+
+def pages_of(caches: Optional[List[dict]]) -> Optional[KV8Pages]:
+    return next((c["pages"] for c in caches if "pages" in c), None) if caches is not None else None

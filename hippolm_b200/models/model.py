@@ -32,6 +32,7 @@ from ..parallel.collectives import gather_seq, reduce_scatter_seq, all_reduce_su
 from ..parallel.linear import column_linear_sp, row_linear_sp, nvfp4_column_linear_sp, nvfp4_row_linear_sp
 from ..parallel.mesh import get_mesh
 from ..ref.ops import positions_from_cu
+from .kv_pages import KV8Pages, layer_cache, pages_of
 from .nvfp4_linear import NVFP4Linear
 
 
@@ -278,14 +279,19 @@ class FullAttention(nn.Module):
         """``cache`` (inference with incremental decoding): ``{"k", "v"}`` buffers ``[sequences, capacity, Hl, dh]`` holding
         the rotated keys and the values of the ``cache["lens"][n]`` tokens seen so far of every sequence. The packed
         prompts fill them and run the regular varlen causal kernel; a step with one token per sequence appends each
-        key / value and attends over that sequence's rows."""
+        key / value and attends over that sequence's rows. A cache with ``"pages"`` (``KV8Pages``) keeps them in 8 bits
+        instead, in the blocks of ``"codes"`` / ``"scales"`` that the pass's plan gives."""
         cfg = self.cfg
         dh, Hl = cfg.head_dim, self.Hl
         qkv = column_linear_sp(h, self.qkv_proj_weight)
         T = qkv.shape[0]
         q, k, v = (t.reshape(T, Hl, dh) for t in qkv.split(Hl * dh, dim=1))
         q, k = ops.rope(q, k, positions, cfg.rope_theta)
-        if cache is not None:
+        if cache is not None and "pages" in cache:
+            o = cache["pages"].attend(q, k, v, cache["codes"], cache["scales"], dh ** -0.5)
+            if o is not None:
+                return row_linear_sp(o.reshape(T, Hl * dh), self.o_proj_weight)
+        elif cache is not None:
             lens = cache["lens"]                                              # host list: tokens cached per sequence
             N = len(lens)
             if T == N and any(lens):
@@ -720,6 +726,9 @@ class HippoModel(nn.Module):
         positions = positions_from_cu(cu_seqlens, T, input_ids.device)
         if isinstance(position_offset, torch.Tensor) or position_offset:
             positions = positions + position_offset
+        pages = pages_of(caches)
+        if pages is not None:
+            pages.plan(cu_seqlens, T)
         x = self.embed_tokens(input_ids)
         blocks = [x]
         finals: List[Optional[torch.Tensor]] = []
@@ -772,18 +781,24 @@ class HippoModel(nn.Module):
             logits = logits.masked_fill(torch.zeros_like(drop).scatter(0, si, drop), float("-inf"))
         return torch.multinomial(logits.softmax(-1), 1)[0]
 
-    def new_decode_caches(self, capacity: int, n_seq: int = 1) -> List[dict]:
+    def new_decode_caches(self, capacity: int, n_seq: int = 1, kv_cache: Optional[str] = None,
+                          limits: Optional[List[int]] = None) -> List[dict]:
         """Empty per-layer caches for ``n_seq`` sequences of at most ``capacity`` tokens each (keys / values of the
         full-attention layers, convolution tails of the KDA layers; the KDA states travel outside, in the list that
-        ``hidden`` returns)."""
+        ``hidden`` returns). ``kv_cache``: None keeps keys and values as they are, "int8" / "e4m3" in 8 bits with a scale for
+        every block of 64 tokens and head, in a pool of blocks for ``limits[n]`` tokens of sequence n (default: ``capacity``)."""
         cfg = self.cfg
         dev, dt = self.norm.weight.device, self.norm.weight.dtype
         caches: List[dict] = []
+        pages = KV8Pages(limits if limits is not None else [capacity] * n_seq, device=dev) if kv_cache is not None else None
         for layer in self.layers:
             if layer.kind == "kda":
                 caches.append({})
             else:
                 Hl = layer.attn.Hl
+                if pages is not None:
+                    caches.append(layer_cache(pages, Hl, cfg.head_dim, kv_cache, dev))
+                    continue
                 caches.append({"k": torch.empty(n_seq, capacity, Hl, cfg.head_dim, device=dev, dtype=dt),
                                "v": torch.empty(n_seq, capacity, Hl, cfg.head_dim, device=dev, dtype=dt),
                                "lens": [0] * n_seq})
@@ -791,7 +806,8 @@ class HippoModel(nn.Module):
 
     @torch.no_grad()
     def generate_batch(self, prompts: List[torch.Tensor], max_new_tokens, temperature=0.0, top_k=0,
-                       eos_token_id: Optional[int] = None, top_p=1.0) -> List[torch.Tensor]:
+                       eos_token_id: Optional[int] = None, top_p=1.0, kv_cache: Optional[str] = None,
+                       logprobs: Optional[int] = None):
         """Incremental decoding of several sequences at once. The prompts run as one packed varlen stream through the
         chunked kernels and leave, per layer, the KDA state of every sequence, its short-convolution tail and the keys /
         values of the full-attention layers; every further step feeds one token per sequence (token-recurrent KDA on the
@@ -801,6 +817,11 @@ class HippoModel(nn.Module):
         A sequence that is done (its limit, or ``eos_token_id``) keeps its slot until the others finish; its further
         tokens are discarded.
 
+        ``kv_cache`` "int8" / "e4m3" keeps the keys and values of the full-attention layers in 8 bits (see
+        ``new_decode_caches``); a sequence that is done gives its blocks back and costs no attention any more.
+        ``logprobs`` (0 .. 32): also returns, for every sequence, ``ops.TokenLogprobs`` of its new tokens under the model's
+        distribution (whatever the sampling settings) with that many alternatives: ``(sequences, scores)``.
+
         Under tensor parallelism (every rank of the group calls this with the same arguments) the token count of each
         pass must split evenly into sequence-parallel shards: dummy one-token sequences fill the batch up to a multiple
         of tp and one of them is lengthened so that the packed prompts do too; the sampled tokens are taken from the
@@ -808,16 +829,31 @@ class HippoModel(nn.Module):
         m = self.mesh
         w = m.tp
         n_real = len(prompts)
+        if logprobs is not None and not 0 <= logprobs <= min(ops.MAX_TOP, self.cfg.vocab_size):
+            raise ValueError(f"logprobs {logprobs}: 0 .. {min(ops.MAX_TOP, self.cfg.vocab_size)}")
         if n_real == 0:
-            return []
+            return [] if logprobs is None else ([], [])
         per = lambda v: list(v) if isinstance(v, (list, tuple)) else [v] * n_real   # noqa: E731
         limits, temps, topks, topps = per(max_new_tokens), per(temperature), per(top_k), per(top_p)
         seqs = [p.reshape(-1).clone() for p in prompts]
         assert all(s.numel() > 0 for s in seqs), "every prompt needs at least one token"
         dev = seqs[0].device
         done = [lim <= 0 for lim in limits]
+        scores: List[ops.TokenLogprobs] = []                # one for every step, of all sequences
+
+        def result():
+            if logprobs is None:
+                return seqs[:n_real]
+            if not scores:                                  # nothing to generate
+                e, none = torch.zeros(0, device=dev), None
+                top = (torch.zeros(0, logprobs, device=dev), torch.zeros(0, logprobs, dtype=torch.int64, device=dev)) if logprobs else (none, none)
+                return seqs[:n_real], [ops.TokenLogprobs(e, e, *top) for _ in range(n_real)]
+            cols = [torch.stack(x) if x[0] is not None else None for x in zip(*scores)]
+            return seqs[:n_real], [ops.TokenLogprobs(*[x[:seqs[n].numel() - lens[n], n] if x is not None else None for x in cols])
+                                   for n in range(n_real)]
+
         if all(done):
-            return seqs
+            return result()
         steps = max(limits)
         if w > 1:
             n_dummy = (-n_real) % w
@@ -832,16 +868,23 @@ class HippoModel(nn.Module):
             topps = topps + [1.0] * n_dummy
         N = len(seqs)
         lens = [s.numel() for s in seqs]
-        caches = self.new_decode_caches(max(lens) + steps, N)
+        caches = self.new_decode_caches(max(lens) + steps, N, kv_cache, [ln + lim for ln, lim in zip(lens, limits)])
+        pages = pages_of(caches)
+        if pages is not None and any(done):
+            pages.release = torch.tensor(done, device=dev)
         cu = torch.tensor([0] + list(torch.tensor(lens).cumsum(0).tolist()), device=dev, dtype=torch.int32)
         h, states = self.hidden(torch.cat(seqs), cu_seqlens=cu, caches=caches)
-        logits = self.lm_head.logits(h, rows=(cu[1:] - 1).long()).float()                  # [N, V]
+        raw = self.lm_head.logits(h, rows=(cu[1:] - 1).long())                             # [N, V]
         cu1 = torch.arange(0, N + 1, device=dev, dtype=torch.int32)
         for step in range(steps):
+            logits = raw.float()
             nxt = torch.stack([self._sample(logits[n], temps[n], topks[n], topps[n]) for n in range(N)])
             if w > 1:
                 dist.broadcast(nxt, src=m.tp_ranks()[0], group=m.tp_group)
+            if logprobs is not None:
+                scores.append(ops.token_logprobs(raw, nxt, top_k=logprobs))
             picked = nxt.tolist()
+            before = list(done)
             for n in range(N):
                 if done[n]:
                     continue
@@ -850,15 +893,40 @@ class HippoModel(nn.Module):
                     done[n] = True
             if all(done):
                 break
+            if pages is not None and done != before:
+                pages.release = torch.tensor(done, device=dev)
             pos = torch.tensor([l + step for l in lens], device=dev)
             h, states = self.hidden(nxt, cu_seqlens=cu1, kda_states=states, caches=caches, position_offset=pos)
-            logits = self.lm_head.logits(h).float()
-        return seqs[:n_real]
+            raw = self.lm_head.logits(h)
+        return result()
+
+    @torch.no_grad()
+    def token_logprobs(self, input_ids: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, top_k: int = 0,
+                       chunk_rows: int = 4096) -> "ops.TokenLogprobs":
+        """How the model scores a text: for every token of the (packed) stream its log probability given the tokens before it in
+        its document (0 for a document's first token), and the entropy and the ``top_k`` alternatives of the distribution that it
+        was drawn from (of a first token: of the distribution behind the document's last one, which no token follows).
+        Logits exist for ``chunk_rows`` tokens at a time."""
+        ids = input_ids.reshape(-1)
+        T = ids.numel()
+        if cu_seqlens is None:
+            row = input_ids.shape[1] if input_ids.dim() == 2 else T
+            cu_seqlens = torch.arange(0, T + 1, max(row, 1), device=ids.device, dtype=torch.int32)
+        h, _ = self.hidden(ids, cu_seqlens=cu_seqlens)
+        cu = cu_seqlens.to(ids.device).long()
+        full = cu[1:] > cu[:-1]
+        prev = torch.arange(-1, T - 1, device=ids.device)                    # the row whose distribution scores token t
+        prev[cu[:-1][full]] = cu[1:][full] - 1
+        targets = ids.clone()
+        targets[cu[:-1][full]] = -100
+        parts = [ops.token_logprobs(self.lm_head.logits(h, rows=prev[s:s + chunk_rows]), targets[s:s + chunk_rows], top_k=top_k)
+                 for s in range(0, T, chunk_rows)]
+        return ops.TokenLogprobs(*[torch.cat(x) if x[0] is not None else None for x in zip(*parts)])
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int, temperature: float = 0.0,
                  top_k: int = 0, eos_token_id: Optional[int] = None, use_cache: bool = True,
-                 top_p: float = 1.0) -> torch.Tensor:
+                 top_p: float = 1.0, kv_cache: Optional[str] = None) -> torch.Tensor:
         """Greedy / top-k sampling.
 
         ``use_cache`` (default): incremental decoding (``generate_batch`` with one sequence): the prompt runs once, every
@@ -868,7 +936,7 @@ class HippoModel(nn.Module):
         ids = input_ids.reshape(-1).clone()
         w = self.mesh.tp
         if use_cache and max_new_tokens > 0 and ids.numel() > 0:
-            return self.generate_batch([ids], max_new_tokens, temperature, top_k, eos_token_id, top_p)[0]
+            return self.generate_batch([ids], max_new_tokens, temperature, top_k, eos_token_id, top_p, kv_cache=kv_cache)[0]
         for _ in range(max_new_tokens):
             T = ids.numel()
             Tp = _pad_to(T, w)

@@ -12,4 +12,4 @@ from .functional import (  # noqa: F401
     lce_chunk_stats, lce_chunk_grad, gemm_tn_accumulate, cuda_ext_loaded,
 )
 from .kv8 import KV8Plan, attention_decode_kv8, kv8_empty, kv8_plan, kv8_write  # noqa: F401
-from .logprob import TokenLogprobs, token_logprobs  # noqa: F401
+from .logprob import MAX_TOP, TokenLogprobs, token_logprobs  # noqa: F401

@@ -40,6 +40,7 @@ def build_parser() -> argparse.ArgumentParser:
     for k in _SIZES:
         p.add_argument("--" + k.replace("_", "-"), dest=k, type=int, default=None)
     p.add_argument("--max_batch", type=int, default=8, help="requests the server decodes together")
+    p.add_argument("--kv_cache", default=None, choices=["int8", "e4m3"], help="8-bit keys and values in the server")
     # server life cycle
     p.add_argument("--host", default="127.0.0.1"); p.add_argument("--port", type=int, default=18080)
     p.add_argument("--no-server", dest="no_server", action="store_true", help="use http://host:port, start nothing")
@@ -61,6 +62,8 @@ def build_parser() -> argparse.ArgumentParser:
     # offline perplexity (no server)
     p.add_argument("--perplexity", action="store_true"); p.add_argument("--data_files", default=None)
     p.add_argument("--seq_len", type=int, default=1024); p.add_argument("--max_tokens", type=int, default=None)
+    p.add_argument("--token_scores", default=None, help="with --perplexity: .jsonl file for the scores of every token")
+    p.add_argument("--top_logprobs", type=int, default=0, help="alternatives of every token in --token_scores (up to 32)")
     return p
 
 
@@ -69,7 +72,8 @@ def server_command(a) -> List[str]:
     cmd = [sys.executable, os.path.join(ROOT, "scripts", "eval_server.py"), "--config", a.config, "--host", a.host,
            "--port", str(a.port), "--model-id", a.model_id, "--max_batch", str(a.max_batch),
            "--max_new_tokens", str(max(a.max_new, 1))]
-    for flag, val in (("--checkpoint", a.checkpoint), ("--tokenizer", a.tokenizer), ("--dtype", a.dtype), ("--device", a.device)):
+    for flag, val in (("--checkpoint", a.checkpoint), ("--tokenizer", a.tokenizer), ("--dtype", a.dtype), ("--device", a.device),
+                      ("--kv_cache", a.kv_cache)):
         if val:
             cmd += [flag, str(val)]
     for k in _SIZES:
@@ -236,7 +240,7 @@ def run_perplexity(a) -> Dict:
     from ..config import HippoConfig
     from ..data.tokenizer import load_tokenizer
     from .eval_server import build_model_and_load
-    from .perplexity import evaluate_perplexity, iter_documents
+    from .perplexity import evaluate_perplexity, iter_documents, score_documents
     if not a.data_files:
         raise SystemExit("--perplexity needs --data_files")
     args = parse_args(["--config", a.config])
@@ -247,8 +251,13 @@ def run_perplexity(a) -> Dict:
     dtype = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16,
              None: torch.bfloat16 if dev.type == "cuda" else torch.float32}[a.dtype]
     model = build_model_and_load(a.checkpoint, HippoConfig.from_namespace(args), dev, dtype)
-    res = evaluate_perplexity(model, load_tokenizer(a.tokenizer or args.tokenizer_path),
-                              iter_documents(a.data_files.split(","), args.text_field), seq_len=a.seq_len,
+    tok = load_tokenizer(a.tokenizer or args.tokenizer_path)
+    if a.token_scores:
+        with open(a.token_scores, "w") as f:
+            for row in score_documents(model, tok, iter_documents(a.data_files.split(","), args.text_field), seq_len=a.seq_len,
+                                       top_logprobs=a.top_logprobs, max_tokens=a.max_tokens):
+                f.write(json.dumps(row) + "\n")
+    res = evaluate_perplexity(model, tok, iter_documents(a.data_files.split(","), args.text_field), seq_len=a.seq_len,
                               max_tokens=a.max_tokens)
     os.makedirs(a.work_dir, exist_ok=True)
     with open(os.path.join(a.work_dir, "perplexity.json"), "w") as f:

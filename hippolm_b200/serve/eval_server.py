@@ -1,7 +1,8 @@
 """OpenAI-compatible evaluation server on the standard library (``scripts/eval_server.py:94-575``).
 
 Endpoints: ``GET /health``, ``GET /v1/models``, ``GET /metrics`` (Prometheus text format: requests, tokens, decoding
-passes, latency), ``POST /v1/completions``, ``POST /v1/chat/completions``.
+passes, latency), ``POST /v1/completions``, ``POST /v1/chat/completions`` (with log probabilities where the request asks for them:
+``logprobs`` N for completions, ``logprobs`` true and ``top_logprobs`` N for chats, N up to 32).
 Greedy decoding (temperature 0) or temperature / top-k sampling; chat requests are rendered with the tokenizer's chat
 template (ChatML for the byte tokenizer). Requests that arrive while a batch is being decoded wait in a queue; the decoding
 thread takes up to ``max_batch`` of them at a time and runs them through ``HippoModel.generate_batch`` together (one packed
@@ -22,6 +23,7 @@ import torch
 
 from ..config import HippoConfig
 from ..models.model import HippoModel
+from ..ops import MAX_TOP
 from ..train.checkpoint import is_sharded_state_dict
 
 
@@ -49,18 +51,24 @@ def build_model_and_load(ckpt_path: Optional[str], cfg: HippoConfig, device: tor
 
 
 class _Pending:
-    __slots__ = ("ids", "max_tokens", "temperature", "top_k", "top_p", "done", "new", "error")
+    __slots__ = ("ids", "max_tokens", "temperature", "top_k", "top_p", "logprobs", "done", "new", "scores", "error")
 
-    def __init__(self, ids, max_tokens, temperature, top_k, top_p=1.0):
+    def __init__(self, ids, max_tokens, temperature, top_k, top_p=1.0, logprobs=None):
         self.ids, self.max_tokens, self.temperature, self.top_k, self.top_p = ids, max_tokens, temperature, top_k, top_p
+        self.logprobs = logprobs                                      # None, or the number of alternatives of every new token
         self.done = threading.Event()
-        self.new, self.error = None, None
+        self.new, self.scores, self.error = None, None, None
+
+
+class BadRequest(ValueError):
+    """A request that the service refuses (HTTP 400)."""
 
 
 class EvalService:
     def __init__(self, model: HippoModel, tokenizer, model_name: str = "hippolm-b200", max_new_tokens: int = 256,
-                 max_batch: int = 8):
+                 max_batch: int = 8, kv_cache: Optional[str] = None):
         self.model, self.tok, self.name, self.max_new = model, tokenizer, model_name, max_new_tokens
+        self.kv_cache = kv_cache             # None, "int8" or "e4m3": how the keys and values of a request are kept
         self.max_batch = max(1, int(max_batch))
         self.batches_run = 0                 # decoding passes so far, and the largest number of requests one of them served
         self.largest_batch = 0
@@ -99,9 +107,15 @@ class EvalService:
                 prompts = [torch.tensor(p.ids, dtype=torch.long, device=dev) for p in batch]
                 with self.lock:
                     if self._batched:
+                        asked = [p.logprobs for p in batch if p.logprobs is not None]
                         outs = self.model.generate_batch(prompts, [p.max_tokens for p in batch],
                                                          [p.temperature for p in batch], [p.top_k for p in batch], eos,
-                                                         [p.top_p for p in batch])
+                                                         [p.top_p for p in batch], kv_cache=self.kv_cache,
+                                                         logprobs=max(asked) if asked else None)
+                        if asked:
+                            outs, scores = outs
+                            for p, sc in zip(batch, scores):
+                                p.scores = sc
                     else:
                         outs = [self.model.generate(x, p.max_tokens, temperature=p.temperature, top_k=p.top_k,
                                                     eos_token_id=eos, top_p=p.top_p) for x, p in zip(prompts, batch)]
@@ -115,11 +129,12 @@ class EvalService:
             for p in batch:
                 p.done.set()
 
-    def _generate(self, prompt_ids, max_tokens: int, temperature: float, top_k: int, top_p: float = 1.0):
+    def _generate(self, prompt_ids, max_tokens: int, temperature: float, top_k: int, top_p: float = 1.0,
+                  logprobs: Optional[int] = None):
         if not prompt_ids:                                            # nothing to condition on: start from the EOS token
             eos0 = getattr(self.tok, "eos_token_id", None)
             prompt_ids = [eos0 if eos0 is not None else 0]
-        req = _Pending(list(prompt_ids), max(0, min(max_tokens, self.max_new)), temperature, top_k, top_p)
+        req = _Pending(list(prompt_ids), max(0, min(max_tokens, self.max_new)), temperature, top_k, top_p, logprobs)
         self._queue.put(req)
         req.done.wait()
         if req.error is not None:
@@ -127,7 +142,48 @@ class EvalService:
         new = req.new
         eos = getattr(self.tok, "eos_token_id", None)
         finish = "stop" if (new and eos is not None and new[-1] == eos) else "length"
-        return new, finish
+        return (new, finish) if logprobs is None else (new, finish, req.scores)
+
+    def _asked_logprobs(self, body: dict, chat: bool) -> Optional[int]:
+        """Alternatives that the request wants for every new token; None where it wants no log probabilities."""
+        n = body.get("logprobs")
+        if chat:
+            if not n:
+                if body.get("top_logprobs"):
+                    raise BadRequest("top_logprobs needs logprobs: true")
+                return None
+            n = body.get("top_logprobs") or 0
+        if n is None or n is False:
+            return None
+        most = min(MAX_TOP, self.model.cfg.vocab_size)
+        if isinstance(n, bool) or not isinstance(n, int) or not 0 <= n <= most:
+            raise BadRequest(f"log probabilities of {n!r} alternatives: 0 .. {most}")
+        return n
+
+    def _logprobs_body(self, new, scores, n_top: int, chat: bool, text: str) -> dict:
+        """The ``logprobs`` object of a choice, for the tokens that begin within its text."""
+        eos = getattr(self.tok, "eos_token_id", None)
+        say = lambda t: self.tok.decode([t], skip_special_tokens=False)                   # noqa: E731
+        lp = scores.logprob.tolist()
+        top_lp = scores.top_logprobs.tolist() if scores.top_logprobs is not None else [[]] * len(new)
+        top_id = scores.top_ids.tolist() if scores.top_ids is not None else [[]] * len(new)
+        rows = []
+        for i, t in enumerate(new):
+            offset = len(self.tok.decode(new[:i], skip_special_tokens=True))
+            if t == eos or (i > 0 and offset >= len(text)):
+                break
+            rows.append((say(t), lp[i], [(say(j), x) for j, x in zip(top_id[i][:n_top], top_lp[i][:n_top])], offset))
+        if chat:
+            item = lambda s, x: {"token": s, "logprob": x, "bytes": list(s.encode())}     # noqa: E731
+            return {"content": [dict(item(s, x), top_logprobs=[item(*a) for a in alts]) for s, x, alts, _ in rows]}
+        tops = []
+        for _, _, alts, _ in rows:
+            d: dict = {}
+            for s, x in alts:                                          # tokens that print alike: the likeliest one counts
+                d.setdefault(s, x)
+            tops.append(d)
+        return {"tokens": [r[0] for r in rows], "token_logprobs": [r[1] for r in rows], "top_logprobs": tops if n_top else None,
+                "text_offset": [r[3] for r in rows]}
 
     def metrics_text(self) -> str:
         """Counters of this service in the Prometheus text exposition format."""
@@ -165,8 +221,10 @@ class EvalService:
             if isinstance(prompt, list):
                 prompt = prompt[0] if prompt else ""
         ids = self.tok.encode(prompt, add_special_tokens=False)
-        new, finish = self._generate(ids, int(body.get("max_tokens", 64)), float(body.get("temperature", 0.0)),
-                                     int(body.get("top_k", 0)), float(body.get("top_p", 1.0)))
+        asked = self._asked_logprobs(body, chat)
+        got = self._generate(ids, int(body.get("max_tokens", 64)), float(body.get("temperature", 0.0)),
+                             int(body.get("top_k", 0)), float(body.get("top_p", 1.0)), **({} if asked is None else {"logprobs": asked}))
+        new, finish = got[:2]
         text = self.tok.decode(new, skip_special_tokens=True)
         stop = body.get("stop")
         if stop:                                                      # the text ends before the first stop string
@@ -180,6 +238,8 @@ class EvalService:
                                                             "message": {"role": "assistant", "content": text}}])
         else:
             base.update(object="text_completion", choices=[{"index": 0, "finish_reason": finish, "text": text}])
+        if asked is not None:
+            base["choices"][0]["logprobs"] = self._logprobs_body(new, got[2], asked, chat, text)
         return base
 
 
@@ -224,6 +284,8 @@ def make_handler(svc: EvalService):
                     self._send(200, svc.complete(body, chat=False))
                 else:
                     self._send(404, {"error": "not found"})
+            except BadRequest as ex:
+                self._send(400, {"error": f"bad request: {ex}"})
             except Exception as ex:
                 self._send(500, {"error": repr(ex)})
     return Handler

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import json
 import math
-from typing import Dict, Iterable, Iterator, List, Optional
+from typing import Dict, Iterable, Iterator, List, Optional, Tuple
 
 import torch
 
@@ -93,3 +93,54 @@ def evaluate_perplexity(model, tokenizer, documents: Iterable[str], seq_len: int
     model.train(was_training)
     nll = total_nll / max(1, total_tok)
     return {"nll": nll, "perplexity": math.exp(min(nll, 700.0)), "tokens": total_tok, "documents": n_docs}
+
+
+@torch.no_grad()
+def score_documents(model, tokenizer, documents: Iterable[str], seq_len: int = 1024, batch_tokens: int = 8192,
+                    top_logprobs: int = 0, max_tokens: Optional[int] = None) -> Iterator[Dict[str, object]]:
+    """Scores of every token, a row for each piece of at most ``seq_len`` tokens of a document (each piece on its own context, as
+    in ``evaluate_perplexity``): ``{"document", "tokens", "logprobs", "entropy"}`` and, with ``top_logprobs``, ``"top_tokens"`` /
+    ``"top_logprobs"``. The first token of a piece has no score (null). Pieces run packed, some ``batch_tokens`` at a time."""
+    dev = next(model.parameters()).device
+    eos = getattr(tokenizer, "eos_token_id", None)
+    w = model.mesh.tp
+    was_training = model.training
+    model.eval()
+    pending: List[Tuple[int, List[int]]] = []
+    seen = 0
+
+    def flush() -> Iterator[Dict[str, object]]:
+        nonlocal pending
+        take, pending = pending, []
+        if not take:
+            return
+        flat = [t for _, p in take for t in p]
+        ends = [0]
+        for _, p in take:
+            ends.append(ends[-1] + len(p))
+        pad = -len(flat) % w                               # a dummy document fills the stream up to even shards
+        cu = ends + ([ends[-1] + pad] if pad else [])
+        got = model.token_logprobs(torch.tensor(flat + [0] * pad, dtype=torch.long, device=dev),
+                                   cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=dev), top_k=top_logprobs)
+        cols = [x.tolist() if x is not None else None for x in got]
+        for (doc, p), s, e in zip(take, ends, ends[1:]):
+            row: Dict[str, object] = {"document": doc, "tokens": p, "logprobs": [None] + cols[0][s + 1:e], "entropy": [None] + cols[1][s + 1:e]}
+            if top_logprobs:
+                row["top_logprobs"], row["top_tokens"] = [None] + cols[2][s + 1:e], [None] + cols[3][s + 1:e]
+            yield row
+
+    for d, text in enumerate(documents):
+        toks = tokenizer.encode(text, add_special_tokens=False)
+        if eos is not None:
+            toks = toks + [eos]
+        for s in range(0, len(toks), seq_len):
+            piece = toks[s:s + seq_len]
+            if len(piece) >= 2:
+                pending.append((d, piece))
+                seen += len(piece) - 1
+        if sum(len(p) for _, p in pending) >= batch_tokens:
+            yield from flush()
+        if max_tokens is not None and seen >= max_tokens:
+            break
+    yield from flush()
+    model.train(was_training)

@@ -1,0 +1,242 @@
+"""8-bit caches and log probabilities through the model, the server, the evaluation script and tensor-parallel ranks (CPU)."""
+import json
+import math
+import threading
+import urllib.error
+import urllib.request
+
+import pytest
+import torch
+
+import kv8_plain as plain
+from hippolm_b200 import ops
+from hippolm_b200.config import HippoConfig
+from hippolm_b200.data.tokenizer import ByteTokenizer
+from hippolm_b200.models import kv_pages
+from hippolm_b200.models.model import HippoModel
+from hippolm_b200.ref import kv8 as ref
+from hippolm_b200.serve.eval_server import EvalService, serve
+
+BASE = dict(vocab_size=96, hidden_size=32, num_heads=2, head_dim=16, num_layers=4, num_blocks=2, intermediate_size=64, full_attn_interval=2)
+
+
+def model(**kw):
+    torch.manual_seed(0)
+    return HippoModel(HippoConfig(**dict(BASE, **kw)), seed=4).eval()
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("kw", [dict(), dict(use_short_conv=True)])
+def test_cached_keys_and_values_are_the_layers_own(kind, kw, monkeypatch):
+    """Every attention call of a batched decode sees, for every sequence that still runs, all keys and values of its tokens in order,
+    rounded to codes; sequences that are done see none, and their blocks are free again."""
+    m = model(**kw)
+    prompts = [torch.randint(0, 96, (n,)) for n in (1, 70, 12, 64, 3)]
+    limits = [6, 3, 8, 2, 0]
+    hist, calls = {}, []
+    write, attend, plan = ops.kv8_write, ops.attention_decode_kv8, ops.kv8_plan
+    per_pass = {}
+
+    def on_plan(table, lens, new, *a, **k):
+        p = plan(table, lens, new, *a, **k)
+        per_pass.update(new=new.tolist(), served=p.served.tolist(), table=table)
+        return p
+
+    def on_write(k, v, slots, codes, scales):
+        write(k, v, slots, codes, scales)
+        rows, at = hist.setdefault(codes.data_ptr(), [[] for _ in prompts]), 0
+        for n, c in enumerate(per_pass["new"]):
+            if per_pass["served"][n]:
+                rows[n] += [(k[at + i], v[at + i]) for i in range(c)]
+            at += c
+
+    def on_attend(q, codes, scales, table, lens, scale):
+        for n, rows in enumerate(hist[codes.data_ptr()]):
+            ln = int(lens[n])
+            assert ln == (len(rows) if per_pass["served"][n] else 0), n
+            if ln == 0:
+                continue
+            for got, want in zip(ref.gather(codes, scales, table[n, :-(-ln // 64)], ln), zip(*rows)):
+                want = torch.stack(want)
+                size = torch.stack([x.abs().amax((0, 2)) for x in want.split(64)]).repeat_interleave(64, 0)[:ln]     # of a block and head
+                # int8: half a step of at most 2 / 127 of the block's largest, twice (codes may be rounded anew as it fills);
+                # e4m3: half of 2^-3 of the value, twice, or of the subnormals' step
+                tol = size[..., None] * (2 / 127) if kind == "int8" else want.abs() * 2 * 2.0 ** -4 + size[..., None] * 2.0 ** -15
+                assert bool(((got - want).abs() <= tol).all())
+        calls.append(lens.tolist())
+        return attend(q, codes, scales, table, lens, scale)
+
+    monkeypatch.setattr(kv_pages.ops, "kv8_plan", on_plan)
+    monkeypatch.setattr(kv_pages.ops, "kv8_write", on_write)
+    monkeypatch.setattr(kv_pages.ops, "attention_decode_kv8", on_attend)
+    out = m.generate_batch(prompts, limits, kv_cache=kind)
+    assert [o.numel() for o in out] == [p.numel() + lim for p, lim in zip(prompts, limits)]
+    assert len(calls) == 2 * 7 and calls[0] == [2, 71, 13, 65, 0] and calls[-1] == [0, 0, 19, 0, 0]
+
+
+def test_pages_hold_what_the_limits_need():
+    pages = kv_pages.KV8Pages([130, 0, 64, 1], block_size=64)
+    assert pages.blocks == 3 + 0 + 1 + 1
+    cu = torch.tensor([0, 100, 103, 167, 168], dtype=torch.int32)
+    pages.release = torch.tensor([False, True, False, False])
+    pages.plan(cu, 168)
+    assert pages.lens.tolist() == [100, 0, 64, 1] and pages.slots[100:103].tolist() == [-1] * 3 and int(pages.free_count) == 1
+    pages.release = torch.tensor([False, True, True, True])
+    for i in range(30):
+        pages.plan(torch.arange(5, dtype=torch.int32), 4)
+    assert pages.lens.tolist() == [130, 0, 0, 0] and int(pages.free_count) == 2 and int(pages.slots[0]) >= 0
+    used = pages.table[0, :3].tolist()
+    assert sorted(used + pages.free[:2].tolist()) == list(range(5))
+
+
+@pytest.mark.parametrize("kind", [None, "int8", "e4m3"])
+def test_scores_of_generated_tokens(kind):
+    m = model()
+    prompts = [torch.randint(0, 96, (n,)) for n in (5, 9)]
+    seqs, scores = m.generate_batch(prompts, [4, 6], logprobs=3, kv_cache=kind)
+    again = m.generate_batch(prompts, [4, 6], kv_cache=kind)
+    for p, s, sc, a in zip(prompts, seqs, scores, again):
+        n = s.numel() - p.numel()
+        assert s.tolist() == a.tolist() and sc.logprob.shape == (n,) and sc.top_ids.shape == (n, 3)
+        assert sc.top_ids[:, 0].tolist() == s[p.numel():].tolist()            # greedy: the likeliest token
+        assert torch.equal(sc.top_logprobs[:, 0], sc.logprob)
+        if kind is None:                                                       # fp32 both ways: the full forward's distribution
+            lp = torch.log_softmax(m(s)["logits"].float(), -1)[p.numel() - 1:-1]
+            assert torch.allclose(sc.logprob, lp.gather(1, s[p.numel():, None])[:, 0], atol=2e-4)
+            assert torch.allclose(sc.entropy, -(lp.exp() * lp).sum(-1), atol=2e-3)
+    none, empty = m.generate_batch(prompts, 0, logprobs=2)
+    assert [x.numel() for x in none] == [5, 9] and empty[0].top_ids.shape == (0, 2)
+    assert m.generate_batch([], 3, logprobs=1) == ([], [])
+    for bad in (-1, 33):
+        with pytest.raises(ValueError):
+            m.generate_batch(prompts, 2, logprobs=bad)
+    with pytest.raises(ValueError):
+        m.generate_batch(prompts, 2, kv_cache="int4")
+
+
+def test_model_scores_of_packed_text():
+    m = model()
+    lens = [7, 1, 12]
+    ids = torch.randint(0, 96, (20,))
+    cu = torch.tensor([0, 7, 8, 20], dtype=torch.int32)
+    got = m.token_logprobs(ids, cu_seqlens=cu, top_k=2, chunk_rows=6)
+    at = 0
+    for ln in lens:
+        lp = torch.log_softmax(m(ids[at:at + ln])["logits"].float(), -1)
+        assert float(got.logprob[at]) == 0.0
+        assert torch.allclose(got.logprob[at + 1:at + ln], lp[:-1].gather(1, ids[at + 1:at + ln, None])[:, 0], atol=2e-4)
+        assert torch.allclose(got.top_logprobs[at + 1:at + ln], lp[:-1].topk(2, -1).values, atol=2e-4)
+        at += ln
+    rows = m.token_logprobs(ids.view(2, 10))
+    assert rows.top_ids is None and float(rows.logprob[10]) == 0.0 and rows.logprob.shape == (20,)
+
+
+def small_service(**kw):
+    cfg = HippoConfig(vocab_size=258, hidden_size=32, num_heads=2, head_dim=16, num_layers=2, num_blocks=1, intermediate_size=64,
+                      full_attn_interval=2)
+    return EvalService(HippoModel(cfg, seed=1).eval(), ByteTokenizer(), max_new_tokens=6, **kw)
+
+
+@pytest.mark.parametrize("kv_cache", [None, "int8"])
+def test_server_answers_with_log_probabilities(kv_cache):
+    svc = small_service(kv_cache=kv_cache)
+    srv = serve(svc, port=0)
+    url = f"http://127.0.0.1:{srv.server_address[1]}/v1/"
+
+    def post(path, body):
+        req = urllib.request.Request(url + path, json.dumps(body).encode(), {"Content-Type": "application/json"})
+        with urllib.request.urlopen(req, timeout=60) as r:
+            return json.loads(r.read())["choices"][0]
+
+    c = post("completions", {"prompt": "hello", "max_tokens": 5, "logprobs": 4})
+    lp = c["logprobs"]
+    assert len(lp["tokens"]) == len(lp["token_logprobs"]) == len(lp["top_logprobs"]) == len(lp["text_offset"]) >= 1
+    assert all(x <= 0 and max(t.values()) == pytest.approx(x) for x, t in zip(lp["token_logprobs"], lp["top_logprobs"]))
+    assert "".join(lp["tokens"]) == c["text"] or any(ord(ch) > 127 for ch in c["text"])
+    plain_c = post("completions", {"prompt": "hello", "max_tokens": 5})
+    assert plain_c["text"] == c["text"] and "logprobs" not in plain_c
+    zero = post("completions", {"prompt": "hello", "max_tokens": 5, "logprobs": 0})["logprobs"]
+    assert zero["token_logprobs"] == lp["token_logprobs"] and zero["top_logprobs"] is None
+    chat = post("chat/completions", {"messages": [{"role": "user", "content": "hi"}], "max_tokens": 3, "logprobs": True, "top_logprobs": 2})
+    item = chat["logprobs"]["content"][0]
+    assert len(item["top_logprobs"]) == 2 and item["logprob"] == pytest.approx(item["top_logprobs"][0]["logprob"]) and item["bytes"]
+    for path, body in (("completions", {"prompt": "a", "logprobs": 33}), ("completions", {"prompt": "a", "logprobs": "x"}),
+                       ("completions", {"prompt": "a", "logprobs": True}),
+                       ("chat/completions", {"messages": [], "top_logprobs": 2}), ("chat/completions", {"messages": [], "logprobs": True, "top_logprobs": -1})):
+        with pytest.raises(urllib.error.HTTPError) as e:
+            post(path, body)
+        assert e.value.code == 400
+    srv.shutdown()
+    svc.close()
+
+
+def test_requests_with_and_without_log_probabilities_share_a_pass():
+    svc = small_service(max_batch=8)
+    bodies = [{"prompt": "ab", "max_tokens": 4}, {"prompt": "abc", "max_tokens": 3, "logprobs": 2}, {"prompt": "x", "max_tokens": 5, "logprobs": 5}]
+    alone = [svc.complete(b, chat=False)["choices"][0] for b in bodies]
+    got = [None] * 3
+    with svc.lock:
+        ts = [threading.Thread(target=lambda i=i: got.__setitem__(i, svc.complete(bodies[i], chat=False)["choices"][0])) for i in range(3)]
+        for t in ts:
+            t.start()
+    for t in ts:
+        t.join(timeout=60)
+    for a, g in zip(alone, got):
+        assert a["text"] == g["text"] and ("logprobs" in a) == ("logprobs" in g)
+        if "logprobs" in a:
+            assert a["logprobs"]["token_logprobs"] == pytest.approx(g["logprobs"]["token_logprobs"], abs=2e-4)
+            assert [len(t) for t in a["logprobs"]["top_logprobs"]] == [len(t) for t in g["logprobs"]["top_logprobs"]]
+    svc.close()
+
+
+def test_token_scores_of_documents(tmp_path):
+    from hippolm_b200.serve.perplexity import evaluate_perplexity, score_documents
+    cfg = HippoConfig(vocab_size=258, hidden_size=32, num_heads=2, head_dim=16, num_layers=2, num_blocks=1, intermediate_size=64,
+                      full_attn_interval=2)
+    m, tok = HippoModel(cfg, seed=1), ByteTokenizer()
+    docs = ["some words to score", "b", "a longer document that is cut in pieces " * 5]
+    rows = list(score_documents(m, tok, docs, seq_len=64, batch_tokens=50, top_logprobs=2))
+    lp = [x for r in rows for x in r["logprobs"] if x is not None]
+    want = evaluate_perplexity(m, tok, docs, seq_len=64)
+    assert len(lp) == want["tokens"] and -sum(lp) / len(lp) == pytest.approx(want["nll"], abs=1e-4)
+    assert m.training and [r["document"] for r in rows] == sorted(r["document"] for r in rows)
+    for r in rows:
+        assert r["logprobs"][0] is None and len(r["tokens"]) == len(r["entropy"]) == len(r["top_tokens"])
+        assert all(len(t) == 2 for t in r["top_tokens"][1:]) and all(0 <= e <= math.log(258) + 1e-4 for e in r["entropy"][1:])
+
+
+def _tp_worker(rank, world, port, out_path):
+    import os
+    os.environ.update({"RANK": str(rank), "WORLD_SIZE": str(world), "LOCAL_RANK": str(rank), "MASTER_ADDR": "127.0.0.1",
+                       "MASTER_PORT": str(port), "HIPPO_TP_SIM": "1"})
+    torch.set_num_threads(1)
+    from hippolm_b200.parallel.mesh import init_distributed_from_env, init_mesh
+    init_distributed_from_env(backend="gloo")
+    init_mesh(tp=world)
+    m = model()
+    g = torch.Generator().manual_seed(7)
+    prompts = [torch.randint(0, 96, (n,), generator=g) for n in (5, 2, 8)]
+    seqs, scores = m.generate_batch(prompts, [4, 6, 3], kv_cache="int8", logprobs=2)
+    packed = torch.cat(prompts + [torch.zeros(1, dtype=torch.long)])
+    text = m.token_logprobs(packed, cu_seqlens=torch.tensor([0, 5, 7, 15, 16], dtype=torch.int32))
+    torch.save({"seqs": [s.tolist() for s in seqs], "lp": [s.logprob.tolist() for s in scores], "text": text.logprob.tolist()}, out_path + f".{rank}")
+    import torch.distributed as dist
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_tensor_parallel_ranks_decode_from_8_bit_caches(tmp_path):
+    import torch.multiprocessing as mp
+    from test_context_parallel import _free_port
+    out = str(tmp_path / "tp")
+    mp.spawn(_tp_worker, args=(2, _free_port(), out), nprocs=2, join=True)
+    a, b = torch.load(out + ".0"), torch.load(out + ".1")
+    assert a == b
+    m = model()
+    g = torch.Generator().manual_seed(7)
+    prompts = [torch.randint(0, 96, (n,), generator=g) for n in (5, 2, 8)]
+    seqs, scores = m.generate_batch(prompts, [4, 6, 3], kv_cache="int8", logprobs=2)
+    assert [s.tolist() for s in seqs] == a["seqs"]                            # heads do not share a block: the same codes on one rank
+    for s, lp in zip(scores, a["lp"]):
+        assert torch.allclose(s.logprob, torch.tensor(lp), atol=1e-3)
+    assert len(a["text"]) == 16 and a["text"][0] == a["text"][5] == 0.0
