@@ -17,7 +17,7 @@ namespace hippo {
 // then dealt out one by one to all threads, which find their request by bisection of the sums in shared memory (a request may
 // own one block or hundreds). Released requests push first. The work is a few dependent loads and barriers (latency-bound); more
 // CTAs would need a grid-wide order between pushes and pops.
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024, kBatch = 4;        // entries a thread has in flight
 
 __device__ __forceinline__ long long block_inclusive_scan(long long v, long long* warp_sum, long long& total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -53,11 +53,10 @@ __device__ __forceinline__ long long slot_of(const int* row, int pos, int sh) {
 
 // first index whose sum is above p (the sums ascend, the last one is above p)
 __device__ __forceinline__ int owner_of(const int* sum, int p) {
-  int lo = 0, hi = kPlanThreads - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (sum[mid] > p) hi = mid; else lo = mid + 1;
-  }
+  int lo = 0;
+#pragma unroll
+  for (int step = kPlanThreads / 2; step; step >>= 1)
+    if (sum[lo + step - 1] <= p) lo += step;
   return lo;
 }
 
@@ -85,9 +84,18 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(
       __syncthreads();
       // what does not fit the list any more (more blocks than it holds: a table that is not ours) is dropped
       const int push = (int)min(total, cap - count);
-      for (int p = tid; p < push; p += kPlanThreads) {
-        const int r = owner_of(s_sum, p);
-        free_list[count + p] = table[(long long)(base + r) * table_ld + p - (r ? s_sum[r - 1] : 0)];
+      for (int p0 = tid; p0 < push; p0 += kBatch * kPlanThreads) {
+        int got[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int p = p0 + i * kPlanThreads;
+          if (p >= push) break;
+          const int r = owner_of(s_sum, p);
+          got[i] = table[(long long)(base + r) * table_ld + p - (r ? s_sum[r - 1] : 0)];
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+          if (p0 + i * kPlanThreads < push) free_list[count + p0 + i * kPlanThreads] = got[i];
       }
       count += push;
       __syncthreads();                               // pushes are visible to the pops of every thread; s_sum is free
@@ -121,17 +129,36 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(
       if (cu) cu[n + 1] = (int)min(end, (long long)0x7fffffff);
     }
     __syncthreads();
-    for (int p = tid; p < (int)total; p += kPlanThreads) {
-      const int r = owner_of(s_sum, p);
-      table[(long long)(base + r) * table_ld + s_have[r] + p - (r ? s_sum[r - 1] : 0)] = free_list[count - 1 - used - p];
+    const int pops = (int)total;
+    for (int p0 = tid; p0 < pops; p0 += kBatch * kPlanThreads) {
+      int got[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (p0 + i * kPlanThreads < pops) got[i] = free_list[count - 1 - used - p0 - i * kPlanThreads];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int p = p0 + i * kPlanThreads;
+        if (p >= pops) break;
+        const int r = owner_of(s_sum, p);
+        table[(long long)(base + r) * table_ld + s_have[r] + p - (r ? s_sum[r - 1] : 0)] = got[i];
+      }
     }
-    used += total;
+    used += pops;
     if (write_slots) {
       __syncthreads();                               // the popped blocks are in the table
       const int last = (int)min(tokens, num_tokens);
-      for (int t = (int)min(chunk_begin, num_tokens) + tid; t < last; t += kPlanThreads) {
-        const int r = owner_of(s_end, t), first = r ? s_end[r - 1] : (int)chunk_begin;
-        slots[t] = s_pos[r] < 0 ? -1ll : slot_of(table + (long long)(base + r) * table_ld, s_pos[r] + t - first, sh);
+      for (int t0 = (int)min(chunk_begin, num_tokens) + tid; t0 < last; t0 += kBatch * kPlanThreads) {
+        long long got[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int t = t0 + i * kPlanThreads;
+          if (t >= last) break;
+          const int r = owner_of(s_end, t), first = r ? s_end[r - 1] : (int)chunk_begin;
+          got[i] = s_pos[r] < 0 ? -1ll : slot_of(table + (long long)(base + r) * table_ld, s_pos[r] + t - first, sh);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+          if (t0 + i * kPlanThreads < last) slots[t0 + i * kPlanThreads] = got[i];
       }
     }
     __syncthreads();
