@@ -176,7 +176,8 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
   const int each = nw ? total / nw : 0, odd = total - each * nw;         // the first `odd` workers have one place more
   const int begin = worker < nw ? each * worker + min(worker, odd) : 0;
   const int end = worker < nw ? begin + each + (worker < odd) : 0;
-  int4 found = make_int4(-1, 0, 0, 0);               // unit that begins here and ends in a later worker
+  // unit that begins here and ends in a later worker: sequence, first query head * 16 + query rows, slot, last worker
+  int4 found = make_int4(-1, 0, 0, 0);
   uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023) + w * S::kWarpBytes;
 
   if (begin < end) {
@@ -429,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
         }
         if (whole && !done) {                        // begins here, goes on: this worker's unit to join
           const int last = end - left - tile + tiles - 1, wide = (each + 1) * odd;     // place of its last tile
-          found = make_int4(n, h * a.QG + g0 / (4 * SETS), sl, last < wide ? last / (each + 1) : odd + (last - wide) / each);
+          found = make_int4(n, (h * a.G + g0) << 4 | min(4 * SETS, a.G - g0), sl, last < wide ? last / (each + 1) : odd + (last - wide) / each);
         }
         fresh = true;
         first = false;
@@ -443,66 +444,88 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
   if (lane == 0) a.desc[worker] = found;
 }
 
-// Joins the parts of the units that begin in the workers of a block of the first kernel, a query row at a time: the maximum over all parts first, then their
-// sums with weights 2^(m_i - m), every warp over its share of the parts (independent loads) and warp 0 over the warps, in order.
-constexpr int kJoinWarps = 8;
-template <int D, int SETS> __global__ void __launch_bounds__(kJoinWarps * 32) kv8_join_kernel(KvAttnArgs a) {
+// Joins the parts of the units that begin in the four workers of a block of the first kernel: the maximum over a row's parts first,
+// then their sums with weights 2^(m_i - m), in order. A warp takes a row of few parts by itself; the rows of a unit of many (a long
+// sequence) are shared by the warps, one of which adds their sums in order.
+constexpr int kJoinWarps = 8, kFewParts = 4;
+struct JoinUnit {
+  int n, head0, w0, slot0, parts, rows;              // sequence, first query head, first worker and its slot, query rows
+};
+template <int D> __global__ void __launch_bounds__(kJoinWarps * 32, 3) kv8_join_kernel(KvAttnArgs a, int per_unit) {
   constexpr int C = D / 32;                          // columns a lane
   __shared__ float s_o[kJoinWarps][D], s_m[kJoinWarps], s_l[kJoinWarps];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int4 all[kWarps];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  auto unit = [&](int k) {
+    const int w0 = blockIdx.x * kWarps + k;
+    const int4 d = a.desc[w0];
+    return d.x < 0 ? JoinUnit{} : JoinUnit{d.x, d.y >> 4, w0, d.z, min(d.w, a.NW - 1) - w0 + 1, d.y & 15};
+  };
+  auto slot = [&](const JoinUnit& u, int row, int i) { return (long long)(i == 0 ? u.slot0 : 2 * (u.w0 + i)) * a.rows + row; };
+  auto add = [&](const JoinUnit& u, int row, int i, float m, float& l, float (&o)[C]) {
+    const long long sl = slot(u, row, i);
+    const float2 ml = *(const float2*)(a.part_ml + sl * 2);
+    const float r = ex2(ml.x - m);
+    l += ml.y * r;
+    if (C == 4) {
+      const float4 x = *(const float4*)(a.part + sl * D + lane * 4);
+      o[0] += x.x * r; o[1] += x.y * r; o[C - 2] += x.z * r; o[C - 1] += x.w * r;
+    } else {
+      const float2 x = *(const float2*)(a.part + sl * D + lane * 2);
+      o[0] += x.x * r; o[1] += x.y * r;
+    }
+  };
+  auto put = [&](const JoinUnit& u, int row, float l, const float (&o)[C]) {
+    const float r = l == 0.f ? 0.f : 1.f / l;
+    const long long oi = ((long long)u.n * a.H * a.G + u.head0 + row) * D + lane * C;
 #pragma unroll
-  for (int k = 0; k < kWarps; ++k) all[k] = a.desc[blockIdx.x * kWarps + k];
-#pragma unroll 1
-  for (int k = 0; k < kWarps; ++k) {
-  const int4 d = k == 0 ? all[0] : k == 1 ? all[1] : k == 2 ? all[2] : all[3];
-  if (d.x < 0) continue;
-  const int w0 = blockIdx.x * kWarps + k, parts = min(d.w, a.NW - 1) - w0 + 1, h = d.y / a.QG, g0 = (d.y - h * a.QG) * 4 * SETS;
-  for (int row = blockIdx.y; row < 4 * SETS && g0 + row < a.G; row += gridDim.y) {
-    auto slot = [&](int i) { return (long long)(i == 0 ? d.z : 2 * (w0 + i)) * a.rows + row; };
-    float m = -INFINITY;
-    for (int i = threadIdx.x; i < parts; i += kJoinWarps * 32) m = fmaxf(m, a.part_ml[slot(i) * 2]);
+    for (int j = 0; j < C; j += 2) store_out(a, oi + j, o[j] * r, o[j + 1] * r);
+  };
+  for (int t = w; t < kWarps * per_unit; t += kJoinWarps) {
+    const JoinUnit u = unit(t % kWarps);
+    const int row = t / kWarps;
+    if (row >= u.rows || u.parts > kFewParts) continue;
+    float m = lane < u.parts ? a.part_ml[slot(u, row, lane) * 2] : -INFINITY, l = 0.f, o[C] = {};
 #pragma unroll
     for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    if (m == -INFINITY) m = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < u.parts; ++i) add(u, row, i, m, l, o);
+    put(u, row, l, o);
+  }
+#pragma unroll 1
+  for (int k = 0; k < kWarps; ++k) {
+    const JoinUnit u = unit(k);
+    if (u.parts <= kFewParts) continue;
+    // the rows side by side, `team` warps each
+    const int team = u.rows > 4 ? 1 : u.rows > 2 ? 2 : u.rows > 1 ? 4 : 8, row = w / team, first = w - row * team;
+    const bool on = row < u.rows;
+    float m = -INFINITY, l = 0.f, o[C] = {};
+    if (on)
+      for (int i = first * 32 + lane; i < u.parts; i += team * 32) m = fmaxf(m, a.part_ml[slot(u, row, i) * 2]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     if (lane == 0) s_m[w] = m;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kJoinWarps; ++i) m = fmaxf(m, s_m[i]);
+    for (int i = 0; i < team; ++i) m = fmaxf(m, s_m[row * team + i]);
     if (m == -INFINITY) m = 0.f;
-    float l = 0.f, o[C] = {};
+    if (on) {
 #pragma unroll 8
-    for (int i = w; i < parts; i += kJoinWarps) {
-      const long long sl = slot(i);
-      const float2 ml = *(const float2*)(a.part_ml + sl * 2);
-      const float r = ex2(ml.x - m);
-      l += ml.y * r;
-      if (C == 4) {
-        const float4 x = *(const float4*)(a.part + sl * D + lane * 4);
-        o[0] += x.x * r; o[1] += x.y * r; o[C - 2] += x.z * r; o[C - 1] += x.w * r;
-      } else {
-        const float2 x = *(const float2*)(a.part + sl * D + lane * 2);
-        o[0] += x.x * r; o[1] += x.y * r;
-      }
+      for (int i = first; i < u.parts; i += team) add(u, row, i, m, l, o);
     }
 #pragma unroll
     for (int j = 0; j < C; ++j) s_o[w][lane * C + j] = o[j];
     if (lane == 0) s_l[w] = l;
     __syncthreads();
-    if (w == 0) {
+    if (on && first == 0) {
+      for (int i = 1; i < team; ++i) {
+        l += s_l[w + i];
 #pragma unroll
-      for (int i = 1; i < kJoinWarps; ++i) {
-        l += s_l[i];
-#pragma unroll
-        for (int j = 0; j < C; ++j) o[j] += s_o[i][lane * C + j];
+        for (int j = 0; j < C; ++j) o[j] += s_o[w + i][lane * C + j];
       }
-      const float r = l == 0.f ? 0.f : 1.f / l;
-      const long long oi = ((long long)d.x * a.H * a.G + h * a.G + g0 + row) * D + lane * C;
-#pragma unroll
-      for (int j = 0; j < C; j += 2) store_out(a, oi + j, o[j] * r, o[j + 1] * r);
+      put(u, row, l, o);
     }
     __syncthreads();
-  }
   }
 }
 
@@ -519,7 +542,7 @@ template <int D, int E4M3, int SETS> int launch_sets(const KvAttnArgs& a, const 
   kv8_attention_kernel<D, E4M3, SETS><<<grid, kThreads, S::kSmem, st>>>(map, a);
   // the joining kernel is launched while the first one runs and waits for its end on the device
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid, (unsigned)a.rows);
+  cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -527,7 +550,7 @@ template <int D, int E4M3, int SETS> int launch_sets(const KvAttnArgs& a, const 
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, kv8_join_kernel<D, SETS>, a);
+  return (int)cudaLaunchKernelEx(&cfg, kv8_join_kernel<D>, a, 4 * SETS);
 }
 template <int D, int E4M3> int launch_kv8_attention(const KvAttnArgs& a, const CUtensorMap& map, int grid, cudaStream_t st) {
   return a.G <= 4 ? launch_sets<D, E4M3, 1>(a, map, grid, st) : launch_sets<D, E4M3, 2>(a, map, grid, st);
