@@ -2,7 +2,7 @@
 // and one (s_K, s_V) per (block, kv head).
 //
 // Bound by HBM: a token and kv head costs 2 D bytes of codes, read once for the query heads that share the kv head (up to 8 of them
-// together). Work is cut in tiles of 32 tokens; the tiles of all (sequence, kv head, group of query heads) form one list that is
+// together). Work is cut in tiles of 32 tokens (64 for head_dim 64: 8 KB); the tiles of all (sequence, kv head, group of query heads) form one list that is
 // divided evenly over all warps of one resident wave, whatever the lengths (the start of a unit counts as one more tile: its query
 // rows and its result cost about as much). A warp streams its tiles through its own TMA ring (no
 // block-wide barrier in the loop) and carries the running maximum and sum; a unit that spans several warps leaves partial (m, l, o)
@@ -21,7 +21,7 @@
 #include "kv8_common.cuh"
 
 namespace hippo {
-constexpr int kTile = 32, kWarps = 4, kThreads = kWarps * 32;
+constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct KvAttnArgs {
@@ -37,8 +37,9 @@ struct KvAttnArgs {
 };
 
 template <int D> struct KvShape {
+  static constexpr int kTile = 4096 / D, kGroups = kTile / 16;       // tokens, groups of 16 of them (a block holds one or more)
   static constexpr int kStageBytes = 2 * kTile * D;
-  static constexpr int kStages = D == 128 ? 2 : 4;
+  static constexpr int kStages = 2;
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kSmem = kWarps * kWarpBytes + 1024;
 };
@@ -111,7 +112,7 @@ __device__ __forceinline__ int cached_len(const KvAttnArgs& a, int n) {
 }
 
 // Where a warp stands in the list of tiles: sequence, kv head, group of query heads, tile.
-struct Cursor {
+template <int kTile> struct Cursor {
   int n, h, grp, tile, len, tiles, left;             // left: places of the warp's range that are still ahead, this tile's included
   __device__ void advance(const KvAttnArgs& a) {
     if (--left <= 0 || ++tile < tiles) return;
@@ -129,11 +130,12 @@ struct Cursor {
 template <int D, int E4M3, int SETS>
 __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid_constant__ CUtensorMap codes_map, KvAttnArgs a) {
   using S = KvShape<D>;
+  constexpr int kTile = S::kTile, NG = S::kGroups;
   constexpr int KS = D / 16, MT = D / 16, DL = D / 8;        // k steps of K q, row tiles of V^T P, output columns a lane
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kWarps][S::kStages];
-  __shared__ float4 s_scale[kWarps][S::kStages];     // K, V scale of the tile's first 16 tokens, K, V of the others
-  __shared__ int s_there[kWarps][S::kStages];        // which 16-token groups of the tile lie in a block of the pool
+  __shared__ float2 s_scale[kWarps][S::kStages][NG]; // K and V scale of every 16 tokens of the tile
+  __shared__ unsigned s_there[kWarps][S::kStages];   // bit 2g: tokens and a block of the pool in group g of the tile
   __shared__ int s_pre[kThreads + 1];
   __shared__ int s_warp[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
   if (lane == 31) s_warp[w] = inc;
   if (tid == 0) {
     for (int i = 0; i < kWarps; ++i)
-      for (int j = 0; j < S::kStages; ++j) mbar_init(&full[i][j], 5);      // TMA bytes + four lanes' scale copies
+      for (int j = 0; j < S::kStages; ++j) mbar_init(&full[i][j], 1 + 2 * NG);      // TMA bytes, the lanes' scale copies
     fence_barrier_init();
   }
   __syncthreads();
@@ -181,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
   uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023) + w * S::kWarpBytes;
 
   if (begin < end) {
-    Cursor put;                                      // next tile to fetch
+    Cursor<kTile> put;                               // next tile to fetch
     {
       int lo = 0, hi = kThreads - 1;
       while (lo < hi) { const int mid = (lo + hi) >> 1; if (s_pre[mid + 1] > begin) hi = mid; else lo = mid + 1; }
@@ -202,47 +204,39 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
       put.h = unit / a.QG;
       put.grp = unit - put.h * a.QG;
     }
-    Cursor get = put;
+    Cursor<kTile> get = put;
     // fetching: lanes hold 32 entries of the table row
     int held_n = -1, held_base = 0, held = -1;
     const int box = min(kTile, 1 << a.sh);           // rows of one TMA box
     const int half_rows = (int)a.half_rows;
     auto fetch = [&](int stage) {
       const int tok = put.tile * kTile, blk = tok >> a.sh;
-      const int base = blk & ~31;                    // a tile never spans two batches of 32 entries (at most 2 blocks, even start)
+      const int base = blk & ~31;                    // a tile never spans two batches of 32 entries (its blocks start at a multiple)
       if (held_n != put.n || held_base != base) {
         held_n = put.n; held_base = base;
         const int j = base + lane;
         held = j < a.M && ((long long)j << a.sh) < put.len ? a.table[(long long)put.n * a.table_ld + j] : -1;
         if (held >= a.blocks) held = -1;
       }
-      const int b0 = __shfl_sync(0xffffffffu, held, blk & 31);
-      const int b1 = a.sh == 4 ? __shfl_sync(0xffffffffu, held, (blk + 1) & 31) : b0;
-      int there = b0 >= 0 ? 3 : 0;
-      if (a.sh == 4) there = (b0 >= 0 ? 1 : 0) | (tok + 16 < put.len && b1 >= 0 ? 2 : 0);
+      // lanes 2g and 2g + 1: 16 tokens from 16g on, their key and their value side
+      const int grp = lane >> 1, first = tok + grp * 16;
+      const int b = __shfl_sync(0xffffffffu, held, (first >> a.sh) & 31);
+      const bool there = lane < 2 * NG && first < put.len && b >= 0, box_here = there && (grp * 16 & (box - 1)) == 0;
+      const unsigned m = __ballot_sync(0xffffffffu, there), boxes = __ballot_sync(0xffffffffu, box_here);
       uint64_t* bar = &full[w][stage];
-      if (lane < 4) {
-        const int bh = (lane < 2 ? b0 : b1) * a.H + put.h;           // below 2^31 with the rows of all blocks
-        if (there & (lane < 2 ? 1 : 2)) {
-          const float* src = a.scales + (lane & 1 ? a.half_scales : 0) + bh;
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32((float*)&s_scale[w][stage] + lane)), "l"(src) : "memory");
-        }
+      if (lane < 2 * NG) {
         if (lane == 0) {
-          uint8_t* dst = ring + stage * S::kStageBytes;
-          s_there[w][stage] = there;
-          const int boxes = a.sh == 4 ? __popc(there) : there & 1;
-          mbar_expect_tx(bar, (uint32_t)(boxes * 2 * box * D));
-          if (there & 1) {
-            const int y = (bh << a.sh) + (tok & ((1 << a.sh) - 1));
-            tma_load_2d(dst, &codes_map, bar, 0, y);
-            tma_load_2d(dst + kTile * D, &codes_map, bar, 0, y + half_rows);
-          }
-          if (a.sh == 4 && (there & 2)) {
-            const int y = (b1 * a.H + put.h) << 4;
-            tma_load_2d(dst + 16 * D, &codes_map, bar, 0, y);
-            tma_load_2d(dst + kTile * D + 16 * D, &codes_map, bar, 0, y + half_rows);
-          }
+          s_there[w][stage] = m;
+          mbar_expect_tx(bar, (uint32_t)(__popc(boxes) * box * D));
         }
+        const int bh = b * a.H + put.h;              // below 2^31 with the rows of all blocks
+        if (there) {
+          const float* src = a.scales + (lane & 1 ? a.half_scales : 0) + bh;
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32((float*)&s_scale[w][stage][0] + lane)), "l"(src) : "memory");
+        }
+        if (box_here)
+          tma_load_2d(ring + stage * S::kStageBytes + (lane & 1) * kTile * D + grp * 16 * D, &codes_map, bar, 0,
+                      (bh << a.sh) + (first & ((1 << a.sh) - 1)) + (lane & 1 ? half_rows : 0));
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
       }
       put.advance(a);
@@ -297,21 +291,23 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
       if (!mbar_wait(&full[w][stage], phase, kWaitTmaFull, worker)) { alive = false; break; }
       const uint8_t* kt = ring + stage * S::kStageBytes;
       const uint8_t* vt = kt + kTile * D;
-      const int valid = min(kTile, get.len - get.tile * kTile), there = s_there[w][stage];
-      const bool ragged = valid < kTile || there != 3;
-      const float4 sc = s_scale[w][stage];
-      const float lv0 = log2f(sc.y), lv1 = log2f(sc.w);
-      uint32_t pb[SETS][4];                          // P^T as the second operand: two k steps of 16 tokens
+      const int valid = min(kTile, get.len - get.tile * kTile);
+      const unsigned there = s_there[w][stage];
+      const bool ragged = valid < kTile || there != (1u << 2 * NG) - 1;
+      float2 sc[NG];
+#pragma unroll
+      for (int j = 0; j < NG; ++j) sc[j] = s_scale[w][stage][j];
+      uint32_t pb[SETS][2 * NG];                     // P^T as the second operand: a k step for each 16 tokens
       {
-        float s[SETS][2][4];
+        float s[SETS][NG][4];
 #pragma unroll
         for (int t = 0; t < SETS; ++t)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) s[t][j][0] = s[t][j][1] = s[t][j][2] = s[t][j][3] = 0.f;
+          for (int j = 0; j < NG; ++j) s[t][j][0] = s[t][j][1] = s[t][j][2] = s[t][j][3] = 0.f;
 #pragma unroll
         for (int q4 = 0; q4 < D / 64; ++q4)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
+          for (int j = 0; j < NG; ++j) {
             const uint4 x = *(const uint4*)(kt + j * 16 * D + (k_at ^ (q4 * 16)));           // row 16j + g
             const uint4 y = *(const uint4*)(kt + j * 16 * D + 8 * D + (k_at ^ (q4 * 16)));   // row 16j + g + 8
             const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
@@ -326,18 +322,22 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
           }
 #pragma unroll
         for (int t = 0; t < SETS; ++t) {
-          // tokens 16j + g and 16j + g + 8 of query head c
-          float y[4], z[4];
-          const float f0 = f[t] * sc.x, f1 = f[t] * sc.z;
-          y[0] = (s[t][0][0] + s[t][0][1]) * f0; y[1] = (s[t][0][2] + s[t][0][3]) * f0;
-          y[2] = (s[t][1][0] + s[t][1][1]) * f1; y[3] = (s[t][1][2] + s[t][1][3]) * f1;
-          z[0] = y[0] + lv0; z[1] = y[1] + lv0; z[2] = y[2] + lv1; z[3] = y[3] + lv1;
+          // tokens 16j + g and 16j + g + 8 of query head c, and with the value scale's logarithm
+          float y[2 * NG], z[2 * NG];
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            const float fk = f[t] * sc[j].x, lv = log2f(sc[j].y);
+            y[2 * j] = (s[t][j][0] + s[t][j][1]) * fk; y[2 * j + 1] = (s[t][j][2] + s[t][j][3]) * fk;
+            z[2 * j] = y[2 * j] + lv; z[2 * j + 1] = y[2 * j + 1] + lv;
+          }
           if (ragged) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (i * 8 + g >= valid || !(there >> (i >> 1) & 1)) y[i] = z[i] = -INFINITY;
+            for (int i = 0; i < 2 * NG; ++i)
+              if (i * 8 + g >= valid || !(there >> (i & ~1) & 1)) y[i] = z[i] = -INFINITY;
           }
-          float mx = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), mz = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+          float mx = y[0], mz = z[0];
+#pragma unroll
+          for (int i = 1; i < 2 * NG; ++i) { mx = fmaxf(mx, y[i]); mz = fmaxf(mz, z[i]); }
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) {
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
             for (int i = 0; i < MT; ++i) { o[t][i][0] *= alpha; o[t][i][1] *= alpha; o[t][i][2] *= alpha; o[t][i][3] *= alpha; }
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 2 * NG; ++i) {
             l[t] += ex2(y[i] - mu);
             const float p = ex2(z[i] - mzu);
             pb[t][i] = transpose8x8(pack2(p, p - __half2float(__float2half_rn(p))));
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
         }
       }
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
+      for (int kk = 0; kk < NG; ++kk) {
         constexpr int W = D / 32;                    // 32-bit words a lane reads of a row
         uint32_t v[4][W];
 #pragma unroll
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid
         if (ragged) {                                // bytes behind the last token may be NaN codes
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t keep = kk * 16 + 2 * c + (i & 1) + (i >> 1) * 8 < valid && (there >> kk & 1) ? 0xffffffffu : 0u;
+            const uint32_t keep = kk * 16 + 2 * c + (i & 1) + (i >> 1) * 8 < valid && (there >> 2 * kk & 1) ? 0xffffffffu : 0u;
 #pragma unroll
             for (int j = 0; j < W; ++j) v[i][j] &= keep;
           }
@@ -577,12 +577,12 @@ extern "C" int hippo_kv8_attention(const KvAttendCall* c) {
   const long long half_rows = (c->blocks * c->H) << sh;
   if (2 * half_rows > 0x7fffffffll) return -2;       // TMA coordinates are 32-bit
   const long long groups = (long long)c->N * c->H * ((c->Hq / c->H + 7) / 8);
-  if (groups * ((((long long)c->M << sh) + kTile - 1) / kTile + 1) > 0x7fffffffll) return -3;
+  if (groups * ((((long long)c->M << sh) + 4096 / D - 1) / (4096 / D) + 1) > 0x7fffffffll) return -3;
   if (((uintptr_t)c->q & 15) || c->q_n * (c->dtype == 2 ? 4 : 2) % 16 || c->q_h * (c->dtype == 2 ? 4 : 2) % 16) return -4;
   auto fn = get_encode_fn();
   if (!fn) return -100;
   CUtensorMap map;
-  const int box = c->block_size < kTile ? c->block_size : kTile;
+  const int tile = 4096 / D, box = c->block_size < tile ? c->block_size : tile;
   const cuuint64_t dim[2] = {(cuuint64_t)D, (cuuint64_t)(2 * half_rows)}, pitch[1] = {(cuuint64_t)D};
   const cuuint32_t bx[2] = {(cuuint32_t)D, (cuuint32_t)box}, one[2] = {1, 1};
   const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(c->codes), dim, pitch, bx, one,

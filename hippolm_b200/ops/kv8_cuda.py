@@ -82,13 +82,13 @@ def attention_decode(q, codes, scales, table, lens, scale: float, dev: int, qs, 
     q = _rows(q)
     qn, qh, _ = q.stride()
     G = Hq // H
-    groups, tiles = N * H * (-(-G // 8)), -(-M * bs // 32)
+    groups, tiles = N * H * (-(-G // 8)), -(-M * bs * D // 4096)
     if groups * (tiles + 1) >= 1 << 31:
-        raise ValueError(f"{N} requests of up to {M * bs} tokens and {H} heads: 2^31 tiles of 32 tokens or more")
+        raise ValueError(f"{N} requests of up to {M * bs} tokens and {H} heads: 2^31 tiles of 4096 / {D} tokens or more")
     sms = _SMS.get(dev)
     if sms is None:
         sms = _SMS[dev] = torch.cuda.get_device_properties(dev).multi_processor_count
-    # a warp takes tiles of 32 tokens; three blocks of four warps fill a multiprocessor
+    # a warp takes tiles of 4096 / D tokens; three blocks of four warps fill a multiprocessor
     workers = 4 * min(3 * sms, -(-(groups * tiles) // 4))
     ws = torch.empty(workers * (2 * min(G, 8) * (D + 2) + 4), dtype=torch.float32, device=dev)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
