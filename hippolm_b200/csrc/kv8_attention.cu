@@ -36,10 +36,11 @@ struct KvAttnArgs {
   float* part; float* part_ml; int4* desc; int NW, rows;   // parts of `rows` query rows each, two a worker
 };
 
-template <int D> struct KvShape {
+template <int D, int SETS> struct KvShape {
   static constexpr int kTile = 4096 / D, kGroups = kTile / 16;       // tokens, groups of 16 of them (a block holds one or more)
   static constexpr int kStageBytes = 2 * kTile * D;
-  static constexpr int kStages = 2;
+  // two groups of heads of 128 need more registers than a third block leaves: two blocks with a deeper ring
+  static constexpr int kBlocks = D * SETS > 128 ? 2 : 3, kStages = kBlocks == 2 ? 3 : 2;
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kSmem = kWarps * kWarpBytes + 1024;
 };
@@ -128,8 +129,8 @@ template <int kTile> struct Cursor {
 
 // SETS: groups of 4 query heads that one pass over the codes serves
 template <int D, int E4M3, int SETS>
-__global__ void __launch_bounds__(kThreads, 3) kv8_attention_kernel(const __grid_constant__ CUtensorMap codes_map, KvAttnArgs a) {
-  using S = KvShape<D>;
+__global__ void __launch_bounds__(kThreads, KvShape<D, SETS>::kBlocks) kv8_attention_kernel(const __grid_constant__ CUtensorMap codes_map, KvAttnArgs a) {
+  using S = KvShape<D, SETS>;
   constexpr int kTile = S::kTile, NG = S::kGroups;
   constexpr int KS = D / 16, MT = D / 16, DL = D / 8;        // k steps of K q, row tiles of V^T P, output columns a lane
   extern __shared__ uint8_t smem_raw[];
@@ -530,7 +531,7 @@ template <int D> __global__ void __launch_bounds__(kJoinWarps * 32, 3) kv8_join_
 }
 
 template <int D, int E4M3, int SETS> int launch_sets(const KvAttnArgs& a, const CUtensorMap& map, int grid, cudaStream_t st) {
-  using S = KvShape<D>;
+  using S = KvShape<D, SETS>;
   static bool set[16] = {};
   int dev = 0;
   cudaGetDevice(&dev);
