@@ -39,8 +39,9 @@ struct KvAttnArgs {
 template <int D, int SETS> struct KvShape {
   static constexpr int kTile = 4096 / D, kGroups = kTile / 16;       // tokens, groups of 16 of them (a block holds one or more)
   static constexpr int kStageBytes = 2 * kTile * D;
-  // two groups of heads of 128 need more registers than a third block leaves: two blocks with a deeper ring
-  static constexpr int kBlocks = D * SETS > 128 ? 2 : 3, kStages = kBlocks == 2 ? 3 : 2;
+  // More registers than a third block leaves keep the compiler from spilling (two groups of heads of 128) and let it run further
+  // ahead (one): two blocks with a deeper ring. 16 x 4096 x 32 heads of 128: 93 us against 96 of three blocks.
+  static constexpr int kBlocks = D * SETS > 64 ? 2 : 3, kStages = kBlocks == 2 ? 3 : 2;
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kSmem = kWarps * kWarpBytes + 1024;
 };
