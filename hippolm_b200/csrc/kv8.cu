@@ -195,8 +195,8 @@ __global__ void __launch_bounds__(256) kv8_slots_kernel(
 }
 
 // ------------------------------------------------------------------------------------------------ write
-// 8 consecutive values as they are loaded, and as fp32. amax() joins their sizes to a running maximum of absolute bits (integer order
-// keeps infinities and NaN on top; two 16-bit fields for the 16-bit types); bits() makes fp32 bits of it.
+// 8 consecutive values as they are loaded, and as fp32. amax() joins their sizes to a running maximum of absolute values (as bits,
+// infinities and NaN on top; a pair for the 16-bit types); bits() makes fp32 bits of it.
 template <typename T> struct Row8;
 template <> struct Row8<float> {
   float4 a, b;
@@ -212,31 +212,39 @@ template <> struct Row8<float> {
   }
   static __device__ uint32_t bits(uint32_t m) { return m; }
 };
-struct Row8h {
+template <> struct Row8<__nv_bfloat16> {
   uint4 a;
-  __device__ void zero() { a = make_uint4(0, 0, 0, 0); }
-  __device__ uint32_t amax(uint32_t m) const {
-    m = __vmaxu2(m, a.x & 0x7fff7fffu);
-    m = __vmaxu2(m, a.y & 0x7fff7fffu);
-    m = __vmaxu2(m, a.z & 0x7fff7fffu);
-    return __vmaxu2(m, a.w & 0x7fff7fffu);
-  }
-};
-template <> struct Row8<__nv_bfloat16> : Row8h {
   __device__ void load(const __nv_bfloat16* p) { a = __ldg((const uint4*)p); }
+  __device__ void zero() { a = make_uint4(0, 0, 0, 0); }
   __device__ void get(float* f) const {
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
   }
+  __device__ uint32_t amax(uint32_t m) const {
+    const __nv_bfloat162* h = (const __nv_bfloat162*)&a;
+    __nv_bfloat162 r = *(const __nv_bfloat162*)&m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r = __hmax2_nan(r, __habs2(h[i]));
+    return *(const uint32_t*)&r;
+  }
   static __device__ uint32_t bits(uint32_t m) { return max(m & 0xffffu, m >> 16) << 16; }
 };
-template <> struct Row8<__half> : Row8h {
+template <> struct Row8<__half> {
+  uint4 a;
   __device__ void load(const __half* p) { a = __ldg((const uint4*)p); }
+  __device__ void zero() { a = make_uint4(0, 0, 0, 0); }
   __device__ void get(float* f) const {
     const __half2* h = (const __half2*)&a;
 #pragma unroll
     for (int i = 0; i < 4; ++i) { const float2 v = __half22float2(h[i]); f[2 * i] = v.x; f[2 * i + 1] = v.y; }
+  }
+  __device__ uint32_t amax(uint32_t m) const {
+    const __half2* h = (const __half2*)&a;
+    __half2 r = *(const __half2*)&m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r = __hmax2_nan(r, __habs2(h[i]));
+    return *(const uint32_t*)&r;
   }
   static __device__ uint32_t bits(uint32_t m) {
     return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16))));
@@ -271,10 +279,11 @@ template <int E4M3> __device__ __forceinline__ void shift_codes(uint8_t* codes, 
 }
 
 template <int E4M3, typename R> __device__ __forceinline__ uint2 encode_row(const R& r, float inv, bool bad) {
+  if (bad) return make_uint2(0, 0);
   float f[8];
   r.get(f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = bad ? 0.f : f[i] * inv;
+  for (int i = 0; i < 8; ++i) f[i] *= inv;
   return encode8<E4M3>(f);
 }
 
