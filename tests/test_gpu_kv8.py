@@ -472,3 +472,95 @@ def test_captured_gradient():
         gr.replay()
         torch.cuda.synchronize()
         assert torch.equal(d, grad())
+
+
+def _in_a_thread(fn):
+    import threading
+    got = []
+
+    def run():
+        try:
+            got.append(fn())
+        except BaseException as e:                                            # noqa: BLE001
+            got.append(e)
+    t = threading.Thread(target=run)
+    t.start()
+    t.join(timeout=120)
+    assert got, "the thread did not come back"
+    if isinstance(got[0], BaseException):
+        raise got[0]
+    return got[0]
+
+
+def test_first_call_of_a_thread_may_be_captured():
+    """A thread whose first calls stand inside a capture (nothing of the thread has touched the device before)."""
+    c = attend_case(11, "int8", 4, 2, 64, 16, [90, 5], torch.bfloat16)
+    z, ids = torch.randn(3, 900, device=DEV), torch.arange(3, device=DEV)
+    st = step_state(5)
+    want, lp = ops.attention_decode_kv8(*c), ops.token_logprobs(z, ids, top_k=2)
+    ref = step({k: x.clone() for k, x in st.items()})
+    torch.cuda.synchronize()
+
+    def run():
+        s, gr = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=s):
+            a, b = ops.attention_decode_kv8(*c), ops.token_logprobs(z, ids, top_k=2)
+            d = step(st)
+        gr.replay()
+        torch.cuda.synchronize()
+        return a, b, d
+    a, b, d = _in_a_thread(run)
+    assert torch.equal(a, want) and torch.equal(b.logprob, lp.logprob) and torch.equal(b.top_ids, lp.top_ids)
+    for x, y in zip(d, ref):
+        assert torch.equal(x, y)
+
+
+def test_two_threads_on_two_streams():
+    import threading
+    cases = [attend_case(20 + i, "e4m3", 4, 2, 128, 64, [700 + i, 3, 0, 250], torch.bfloat16) for i in range(2)]
+    want = [ops.attention_decode_kv8(*c) for c in cases]
+    zs = [torch.randn(5, 40000, device=DEV) for _ in range(2)]
+    ids = torch.zeros(5, dtype=torch.int64, device=DEV)
+    scores = [ops.token_logprobs(z, ids, top_k=4) for z in zs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(60):
+                a, b = ops.attention_decode_kv8(*cases[i]), ops.token_logprobs(zs[i], ids, top_k=4)
+                if not (torch.equal(a, want[i]) and torch.equal(b.logprob, scores[i].logprob) and torch.equal(b.top_ids, scores[i].top_ids)):
+                    bad.append(i)
+    ts = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join(timeout=120)
+    assert not bad
+
+
+def test_more_requests_than_workers_and_a_wide_table():
+    lens = [(i * 7) % 23 for i in range(5000)]
+    q, codes, scales, table, ln = attend_case(30, "int8", 2, 1, 64, 16, [1], torch.float32)
+    codes, scales, _ = cache_case(31, "int8", 1, 64, 16, 40)
+    codes, scales = codes.to(DEV), scales.to(DEV)
+    g = torch.Generator().manual_seed(1)
+    table = torch.randint(0, 40, (5000, 300), generator=g).to(torch.int32).to(DEV)      # shared blocks, width far beyond the lengths
+    ln = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    q = torch.randn(5000, 2, 64, generator=g).to(DEV)
+    got = ops.attention_decode_kv8(q, codes, scales, table, ln)
+    pick = [0, 1, 2, 3, 1776, 2500, 4998, 4999]
+    plain.check_attend(got[pick], q[pick], codes, scales, table[pick], ln[pick], 64 ** -0.5)
+    assert not got[ln == 0].any()
+    one = torch.cat([ops.attention_decode_kv8(q[i:i + 50], codes, scales, table[i:i + 50], ln[i:i + 50]) for i in range(0, 5000, 50)])
+    assert float((one - got).abs().max()) < 1e-5 * float(got.abs().max())
+
+
+def test_a_block_of_zeros_beside_large_values():
+    """Scales from 2^-100 (zeros) to 2^90 in one sequence, in one warp and joined over many."""
+    for lens in ([40], [6000]):
+        q, codes, scales, table, ln = attend_case(40, "e4m3", 1, 1, 64, 16, lens, torch.float32)
+        codes[1, int(table[0, 1])] = 0
+        scales[1, int(table[0, 1])] = 2.0 ** -100
+        scales[1, int(table[0, 0])] = 2.0 ** 90
+        plain.check_attend(ops.attention_decode_kv8(q, codes, scales, table, ln), q, codes, scales, table, ln, 64 ** -0.5)
