@@ -12,7 +12,7 @@ from ._ext import check, lib
 
 DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _stream = torch._C._cuda_getCurrentRawStream            # the handle of a device's current stream
-_current = torch.cuda.current_device
+_current = torch._C._cuda_getDevice                     # (the tensors of a call have initialised CUDA)
 ONE_BLOCK_TOKENS = 16384
 _FNS: dict = {}
 _SMS: dict = {}

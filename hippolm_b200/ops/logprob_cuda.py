@@ -23,8 +23,7 @@ def forward(logits, ids, top_k: int, keep: bool, dev: int):
     lp = torch.empty(T, dtype=torch.float32, device=d)
     ent = torch.empty_like(lp)
     stat = torch.empty((T, 2), dtype=torch.float32, device=d) if keep else None
-    top = torch.empty((T, top_k), dtype=torch.float32, device=d) if top_k else None
-    top_ids = torch.empty((T, top_k), dtype=torch.int64, device=d) if top_k else None
+    top, top_ids = (lp.new_empty((T, top_k)), ids.new_empty((T, top_k))) if top_k else (None, None)
     launch("token_logprobs", dev, _FWD.pack(
         z.data_ptr(), ids.data_ptr(), lp.data_ptr(), ent.data_ptr(), stat.data_ptr() if keep else 0, top.data_ptr() if top_k else 0,
         top_ids.data_ptr() if top_k else 0, _stream(dev), z.stride(0), T, V, top_k, DTYPE[z.dtype]))
