@@ -224,8 +224,8 @@ template <typename T> struct LpRow {
   }
 };
 
-// One segment: statistics of the lane, keys of the granules' maxima. GR: logits a granule (0: no alternatives are asked for).
-template <typename T, int GR> __device__ __forceinline__ void lp_segment(const LpRow<T>& r, int g, Vec8<T> (&x)[LpRow<T>::NV], LpStat& st, int* gran) {
+// One segment: statistics of the lane, the granules' maxima. GR: logits a granule (0: no alternatives are asked for).
+template <typename T, int GR> __device__ __forceinline__ void lp_segment(const LpRow<T>& r, int g, Vec8<T> (&x)[LpRow<T>::NV], LpStat& st, float* gran) {
   constexpr int NV = LpRow<T>::NV, kSeg = LpRow<T>::kSeg;
   const int lane = threadIdx.x & 31;
   float m[NV], mx;
@@ -240,16 +240,15 @@ template <typename T, int GR> __device__ __forceinline__ void lp_segment(const L
       float k;
       asm("max.NaN.f32 %0, %1, %2;" : "=f"(k) : "f"(m[i]), "f"(m[i + 1]));
       asm("redux.sync.max.NaN.f32 %0, %0, 0xffffffff;" : "+f"(k));
-      const int at = g * (kSeg / 512) + i / 2;
-      if (lane == 0 && at * 512 < r.span) gran[at] = order_key(k);
+      if (lane == 0) gran[g * (kSeg / 512) + i / 2] = k;               // (behind the row's last granule: -inf)
     }
   } else if constexpr (GR > 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      int k = order_key(m[i]);
+      float k = m[i];
       if (GR == 64)
 #pragma unroll
-        for (int d = 1; d < 8; d <<= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, d));
+        for (int d = 1; d < 8; d <<= 1) asm("max.NaN.f32 %0, %0, %1;" : "+f"(k) : "f"(__shfl_xor_sync(0xffffffffu, k, d)));
       const int at = g * (kSeg / GR) + (i * 256 + lane * 8) / GR;
       if (lane % (GR / 8) == 0 && at * GR < r.span) gran[at] = k;
     }
@@ -286,9 +285,9 @@ struct LpSelect {
   unsigned floor;
 };
 
-// The alternatives of a row from the keys of its granules, by the whole block.
+// The alternatives of a row from the maxima of its granules, by the whole block.
 template <typename T, int GR>
-__device__ __forceinline__ void lp_select(const LpArgs& a, long long row, const LpRow<T>& r, const int* gran, LpSelect& s, const float2& s_ml) {
+__device__ __forceinline__ void lp_select(const LpArgs& a, long long row, const LpRow<T>& r, const float* gran, LpSelect& s, const float2& s_ml) {
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, w = tid >> 5, warps = threads >> 5;
   const int grans = (r.span + GR - 1) / GR, want = min(a.top, grans);
   // keys as unsigned integers without the low bits that this type's values never differ in
@@ -298,7 +297,7 @@ __device__ __forceinline__ void lp_select(const LpArgs& a, long long row, const 
       constexpr int K = decltype(count)::value;
       unsigned key[K], t = 0;                        // of granules lane, lane + 32, ...; 0 is below every key
 #pragma unroll
-      for (int i = 0; i < K; ++i) key[i] = i * 32 + lane < grans ? ((unsigned)gran[i * 32 + lane] ^ 0x80000000u) >> kShift : 0u;
+      for (int i = 0; i < K; ++i) key[i] = i * 32 + lane < grans ? ((unsigned)order_key(gran[i * 32 + lane]) ^ 0x80000000u) >> kShift : 0u;
       // t: the largest number that `want` keys reach, or a smaller one that exactly `want` keys reach; it begins like all keys do
       unsigned most = key[0], least = 0xffffffffu;
 #pragma unroll
@@ -451,13 +450,13 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(LpArgs a)
   cg::cluster_group cl = cg::this_cluster();
   const int part = (int)cl.block_rank(), parts = (int)cl.num_blocks();
   const long long row = blockIdx.x / parts;
-  __shared__ int s_gran[GR ? kMaxGranules : 1];      // order keys of the granules' maxima (of all parts, in part 0)
+  __shared__ float s_gran[GR ? kMaxGranules : 1];    // the granules' maxima (of all parts, in part 0)
   __shared__ LpStat s_stat[kLpWarps], s_part[8];
   __shared__ LpSelect s_sel[1];
   __shared__ float2 s_ml;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, warps = blockDim.x >> 5;
   const LpRow<T> r(a, row);
-  int* gran0 = GR ? cl.map_shared_rank(s_gran, 0) : nullptr;
+  float* gran0 = GR ? cl.map_shared_rank(s_gran, 0) : nullptr;
   if (parts > 1) cl.sync();                          // part 0 runs: its shared memory may be written
   bool scored = false;
   float zy = 0.f;
