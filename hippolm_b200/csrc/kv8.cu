@@ -387,14 +387,14 @@ __global__ void __launch_bounds__(128, WriteShape<T, D, E4M3, BS>::kBlocks) kv8_
     const long long block = (s >> a.sh) * a.H;
     Row8<T> next[P];
     float next_old = 0.f;
+    const T* xk = source(0, t) + r0 * a.k_t;         // this thread's first row, of head 0
+    const T* xv = source(1, t) + r0 * a.v_t;
     auto load = [&](int pair) {
-      const T* x = source(pair, t);
-      const long long ld = pair & 1 ? a.v_t : a.k_t;
+      const T* x = pair & 1 ? xv + (pair >> 1) * a.v_h : xk + (pair >> 1) * a.k_h;
+      const long long step = RPP * (pair & 1 ? a.v_t : a.k_t);
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-        const int r = r0 + p * RPP;
-        if (r < L) next[p].load(x + r * ld); else next[p].zero();
-      }
+      for (int p = 0; p < P; ++p, x += step)
+        if (r0 + p * RPP < L) next[p].load(x); else next[p].zero();
       if (off) next_old = a.scales[(pair & 1 ? a.half_scales : 0) + block + (pair >> 1)];
     };
     load(first);
@@ -417,11 +417,10 @@ __global__ void __launch_bounds__(128, WriteShape<T, D, E4M3, BS>::kBlocks) kv8_
       const RunScale rs = run_scale<E4M3>(m, old, off > 0);
       if (rs.down < 0) shift_codes<E4M3>(codes, off * D, rs.down, tid, 128);
       const float inv = pow2f(-rs.e);
+      uint8_t* dst = codes + (off + r0) * D + col;
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-        const int r = r0 + p * RPP;
-        if (r < L) *(uint2*)(codes + (off + r) * D + col) = encode_row<E4M3>(row[p], inv, rs.bad);
-      }
+      for (int p = 0; p < P; ++p)
+        if (r0 + p * RPP < L) *(uint2*)(dst + p * RPP * D) = encode_row<E4M3>(row[p], inv, rs.bad);
       if (tid == 0) a.scales[(pair & 1 ? a.half_scales : 0) + bh] = rs.bad ? __uint_as_float(0x7fffffffu) : pow2f(rs.e);
     }
     __syncthreads();                                 // s_max is free for the next run
