@@ -304,26 +304,26 @@ __device__ __forceinline__ bool continues(const WriteArgs& a, long long prev, lo
   return slot_ok(a, prev) && s == prev + 1 && (s & ((1 << a.sh) - 1)) != 0;
 }
 
-// One CTA for the runs that start in a window of W tokens, and for kPairs (head, half) pairs. It finds the runs (consecutive tokens in
+// One CTA for the runs that start in a window of W tokens, and for a few (head, half) pairs. It finds the runs (consecutive tokens in
 // consecutive slots of one block) by ballots. Runs of up to kShort tokens (decoding: one) go to groups of lanes that hold a row, 128 /
 // (D / 8) of them at work; longer runs (prompts) are read once into registers by the whole CTA, the next pair's rows in flight while
 // this one's are reduced and stored. HBM-bound for prompts (bytes = 2 T H D (element + 1)), latency for a token a request.
 // The window is small for few tokens, which spreads them over the card, and a block's tokens for many.
-constexpr int kPairs = 4, kShort = 4;
+constexpr int kShort = 4;
 
 template <typename T, int D, int E4M3, int BS> struct WriteShape {
   static constexpr int kBytes = BS * D * (int)sizeof(T);                 // a run at most
-  static constexpr int kBlocks = kBytes <= 4096 ? 8 : kBytes <= 8192 ? 6 : kBytes <= 16384 ? 5 : 3;    // what the registers allow
+  static constexpr int kBlocks = kBytes <= 4096 ? 8 : kBytes <= 8192 ? 7 : kBytes <= 16384 ? 5 : 3;    // what the registers allow
 };
 
 template <typename T, int D, int E4M3, int BS>
-__global__ void __launch_bounds__(128, WriteShape<T, D, E4M3, BS>::kBlocks) kv8_write_kernel(WriteArgs a, int W) {
+__global__ void __launch_bounds__(128, WriteShape<T, D, E4M3, BS>::kBlocks) kv8_write_kernel(WriteArgs a, int W, int pairs) {
   constexpr int LPR = D / 8, RPP = 128 / LPR, P = (BS + RPP - 1) / RPP;   // lanes a row, rows a pass, passes
   __shared__ unsigned s_cont[4];                     // bit i: token w0 + i continues the run of the token before it
   __shared__ int s_run[BS], s_n[2];                  // first token | length << 8: short runs from the front, long ones from the back
   __shared__ uint32_t s_max[2][4];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const int first = blockIdx.y * kPairs, last = min(first + kPairs, 2 * a.H);
+  const int first = blockIdx.y * pairs, last = min(first + pairs, 2 * a.H);
   const long long w0 = (long long)blockIdx.x * W;
   bool ok = false, cont = false;
   if (tid < W + BS && w0 + tid < a.T) {
@@ -428,7 +428,9 @@ __global__ void __launch_bounds__(128, WriteShape<T, D, E4M3, BS>::kBlocks) kv8_
 }
 
 template <typename T, int D, int E4M3> int launch_write(const WriteArgs& a, int window, cudaStream_t st) {
-  const int bs = 1 << a.sh, groups = (2 * a.H + kPairs - 1) / kPairs;
+  // 2 pairs a block spread few tokens over more of them (32 single tokens 2.9 us against 3.6, 1000 in prompts 8.8 against 11.5),
+  // 4 share the search for the runs (25k tokens 57 against 63)
+  const int bs = 1 << a.sh, pairs = a.T * a.H <= 32768 ? 2 : 4, groups = (2 * a.H + pairs - 1) / pairs;
   int W = window;
   if (W == 0) {                                      // some two thousand blocks, or a window of a whole block's tokens
     W = 4;
@@ -436,9 +438,9 @@ template <typename T, int D, int E4M3> int launch_write(const WriteArgs& a, int 
   }
   if (W < 1 || W > bs) return -1;
   const dim3 grid((unsigned)((a.T + W - 1) / W), (unsigned)groups);
-  if (a.sh == 4) kv8_write_kernel<T, D, E4M3, 16><<<grid, 128, 0, st>>>(a, W);
-  else if (a.sh == 5) kv8_write_kernel<T, D, E4M3, 32><<<grid, 128, 0, st>>>(a, W);
-  else kv8_write_kernel<T, D, E4M3, 64><<<grid, 128, 0, st>>>(a, W);
+  if (a.sh == 4) kv8_write_kernel<T, D, E4M3, 16><<<grid, 128, 0, st>>>(a, W, pairs);
+  else if (a.sh == 5) kv8_write_kernel<T, D, E4M3, 32><<<grid, 128, 0, st>>>(a, W, pairs);
+  else kv8_write_kernel<T, D, E4M3, 64><<<grid, 128, 0, st>>>(a, W, pairs);
   return (int)cudaGetLastError();
 }
 template <typename T> int dispatch_write(const WriteArgs& a, int D, int e4m3, int window, cudaStream_t st) {
