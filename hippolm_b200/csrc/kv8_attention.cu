@@ -3,9 +3,8 @@
 //
 // Bound by HBM: a token and kv head costs 2 D bytes of codes, read once for the query heads that share the kv head (up to 8 of them
 // together). Work is cut in tiles of 32 tokens (64 for head_dim 64: 8 KB); the tiles of all (sequence, kv head, group of query heads) form one list that is
-// divided evenly over all warps of one resident wave, whatever the lengths (the start of a unit counts as one more tile: its query
-// rows and its result cost about as much). A warp streams its tiles through its own TMA ring (no
-// block-wide barrier in the loop) and carries the running maximum and sum; a unit that spans several warps leaves partial (m, l, o)
+// divided evenly over one resident wave of one-warp blocks, whatever the lengths (the start of a unit counts as one more tile: its
+// query rows and its result cost about as much). A warp streams its tiles through a TMA ring and carries the running maximum and sum; a unit that spans several warps leaves partial (m, l, o)
 // rows that a second, small kernel joins in a fixed order, so results do not depend on timing.
 //
 // Arithmetic: codes are exact in fp16, so mma.m16n8k16 (fp16 operands, fp32 accumulators) is exact for them. They are the 16-row
@@ -21,7 +20,7 @@
 #include "kv8_common.cuh"
 
 namespace hippo {
-constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kUnits = 4;                            // workers whose units a block of the joining kernel looks after
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct KvAttnArgs {
@@ -39,11 +38,10 @@ struct KvAttnArgs {
 template <int D, int SETS> struct KvShape {
   static constexpr int kTile = 4096 / D, kGroups = kTile / 16;       // tokens, groups of 16 of them (a block holds one or more)
   static constexpr int kStageBytes = 2 * kTile * D;
-  // More registers than a third block leaves keep the compiler from spilling (two groups of heads of 128) and let it run further
-  // ahead (one): two blocks with a deeper ring. 16 x 4096 x 32 heads of 128: 93 us against 96 of three blocks.
-  static constexpr int kBlocks = D * SETS > 64 ? 2 : 3, kStages = kBlocks == 2 ? 3 : 2;
-  static constexpr int kWarpBytes = kStages * kStageBytes;
-  static constexpr int kSmem = kWarps * kWarpBytes + 1024;
+  // More registers than twelve blocks leave keep the compiler from spilling (two groups of heads of 128) and let it run further
+  // ahead (one): eight blocks with a deeper ring. 16 x 4096 x 32 heads of 128: 93 us against 96.
+  static constexpr int kBlocks = D * SETS > 64 ? 8 : 12, kStages = kBlocks == 8 ? 3 : 2;
+  static constexpr int kSmem = kStages * kStageBytes + 1024;
 };
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
@@ -130,29 +128,27 @@ template <int kTile> struct Cursor {
 
 // SETS: groups of 4 query heads that one pass over the codes serves
 template <int D, int E4M3, int SETS>
-__global__ void __launch_bounds__(kThreads, KvShape<D, SETS>::kBlocks) kv8_attention_kernel(const __grid_constant__ CUtensorMap codes_map, KvAttnArgs a) {
+__global__ void __launch_bounds__(32, KvShape<D, SETS>::kBlocks) kv8_attention_kernel(const __grid_constant__ CUtensorMap codes_map, KvAttnArgs a) {
   using S = KvShape<D, SETS>;
   constexpr int kTile = S::kTile, NG = S::kGroups;
   constexpr int KS = D / 16, MT = D / 16, DL = D / 8;        // k steps of K q, row tiles of V^T P, output columns a lane
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kWarps][S::kStages];
-  __shared__ float2 s_scale[kWarps][S::kStages][NG]; // K and V scale of every 16 tokens of the tile
-  __shared__ unsigned s_there[kWarps][S::kStages];   // bit 2g: tokens and a block of the pool in group g of the tile
-  __shared__ int s_pre[kThreads + 1];
-  __shared__ int s_warp[kWarps];
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  __shared__ uint64_t full[S::kStages];
+  __shared__ float2 s_scale[S::kStages][NG];         // K and V scale of every 16 tokens of the tile
+  __shared__ unsigned s_there[S::kStages];           // bit 2g: tokens and a block of the pool in group g of the tile
+  const int lane = threadIdx.x;
   const int units = a.H * a.QG;
   asm volatile("griddepcontrol.launch_dependents;");
 
   // rows of empty sequences
   for (int n = blockIdx.x; n < a.N; n += gridDim.x)
     if (a.lens[n] <= 0)
-      for (int i = tid; i < a.H * a.G * (D / 2); i += kThreads) store_out(a, (long long)n * a.H * a.G * D + i * 2, 0.f, 0.f);
+      for (int i = lane; i < a.H * a.G * (D / 2); i += 32) store_out(a, (long long)n * a.H * a.G * D + i * 2, 0.f, 0.f);
 
-  // places before every thread's share of the sequences: a unit has one more than tiles
-  const int share = (a.N + kThreads - 1) / kThreads;
+  // places before every lane's share of the sequences: a unit has one more than tiles
+  const int share = (a.N + 31) / 32;
   int mine = 0;                                      // (the host has seen to it that all places are below 2^31)
-  for (int n = tid * share; n < min(a.N, (tid + 1) * share); ++n) {
+  for (int n = lane * share; n < min(a.N, (lane + 1) * share); ++n) {
     const int len = cached_len(a, n);
     if (len > 0) mine += ((len + kTile - 1) / kTile + 1) * units;
   }
@@ -162,34 +158,27 @@ __global__ void __launch_bounds__(kThreads, KvShape<D, SETS>::kBlocks) kv8_atten
     const int y = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += y;
   }
-  if (lane == 31) s_warp[w] = inc;
-  if (tid == 0) {
-    for (int i = 0; i < kWarps; ++i)
-      for (int j = 0; j < S::kStages; ++j) mbar_init(&full[i][j], 1 + 2 * NG);      // TMA bytes, the lanes' scale copies
+  if (lane == 0) {
+    for (int j = 0; j < S::kStages; ++j) mbar_init(&full[j], 1 + 2 * NG);      // TMA bytes, the lanes' scale copies
     fence_barrier_init();
   }
-  __syncthreads();
-  for (int i = 0; i < w; ++i) inc += s_warp[i];
-  s_pre[tid + 1] = inc;
-  if (tid == 0) s_pre[0] = 0;
-  __syncthreads();
-  const int total = s_pre[kThreads];
+  __syncwarp();
+  const int total = __shfl_sync(0xffffffffu, inc, 31);
 
   // no more workers than half the places: each has two at least, so one tile or more of every unit between its ends
-  const int worker = blockIdx.x * kWarps + w, nw = min(a.NW, total >> 1);
+  const int worker = blockIdx.x, nw = min(a.NW, total >> 1);
   const int each = nw ? total / nw : 0, odd = total - each * nw;         // the first `odd` workers have one place more
   const int begin = worker < nw ? each * worker + min(worker, odd) : 0;
   const int end = worker < nw ? begin + each + (worker < odd) : 0;
   // unit that begins here and ends in a later worker: sequence, first query head * 16 + query rows, slot, last worker
   int4 found = make_int4(-1, 0, 0, 0);
-  uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023) + w * S::kWarpBytes;
+  uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
 
   if (begin < end) {
     Cursor<kTile> put;                               // next tile to fetch
     {
-      int lo = 0, hi = kThreads - 1;
-      while (lo < hi) { const int mid = (lo + hi) >> 1; if (s_pre[mid + 1] > begin) hi = mid; else lo = mid + 1; }
-      int at = s_pre[lo];
+      const int lo = __ffs(__ballot_sync(0xffffffffu, inc > begin)) - 1;
+      int at = __shfl_sync(0xffffffffu, inc - mine, lo);
       int n = lo * share;
       for (;;) {                                     // the sequence of the share that holds `begin`
         put.len = cached_len(a, n);
@@ -225,16 +214,16 @@ __global__ void __launch_bounds__(kThreads, KvShape<D, SETS>::kBlocks) kv8_atten
       const int b = __shfl_sync(0xffffffffu, held, (first >> a.sh) & 31);
       const bool there = lane < 2 * NG && first < put.len && b >= 0, box_here = there && (grp * 16 & (box - 1)) == 0;
       const unsigned m = __ballot_sync(0xffffffffu, there), boxes = __ballot_sync(0xffffffffu, box_here);
-      uint64_t* bar = &full[w][stage];
+      uint64_t* bar = &full[stage];
       if (lane < 2 * NG) {
         if (lane == 0) {
-          s_there[w][stage] = m;
+          s_there[stage] = m;
           mbar_expect_tx(bar, (uint32_t)(__popc(boxes) * box * D));
         }
         const int bh = b * a.H + put.h;              // below 2^31 with the rows of all blocks
         if (there) {
           const float* src = a.scales + (lane & 1 ? a.half_scales : 0) + bh;
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32((float*)&s_scale[w][stage][0] + lane)), "l"(src) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32((float*)&s_scale[stage][0] + lane)), "l"(src) : "memory");
         }
         if (box_here)
           tma_load_2d(ring + stage * S::kStageBytes + (lane & 1) * kTile * D + grp * 16 * D, &codes_map, bar, 0,
@@ -290,15 +279,15 @@ __global__ void __launch_bounds__(kThreads, KvShape<D, SETS>::kBlocks) kv8_atten
           m[t] = mv[t] = -INFINITY; l[t] = 0.f;
         }
       }
-      if (!mbar_wait(&full[w][stage], phase, kWaitTmaFull, worker)) { alive = false; break; }
+      if (!mbar_wait(&full[stage], phase, kWaitTmaFull, worker)) { alive = false; break; }
       const uint8_t* kt = ring + stage * S::kStageBytes;
       const uint8_t* vt = kt + kTile * D;
       const int valid = min(kTile, get.len - get.tile * kTile);
-      const unsigned there = s_there[w][stage];
+      const unsigned there = s_there[stage];
       const bool ragged = valid < kTile || there != (1u << 2 * NG) - 1;
       float2 sc[NG];
 #pragma unroll
-      for (int j = 0; j < NG; ++j) sc[j] = s_scale[w][stage][j];
+      for (int j = 0; j < NG; ++j) sc[j] = s_scale[stage][j];
       uint32_t pb[SETS][2 * NG];                     // P^T as the second operand: a k step for each 16 tokens
       {
         float s[SETS][NG][4];
@@ -439,14 +428,14 @@ __global__ void __launch_bounds__(kThreads, KvShape<D, SETS>::kBlocks) kv8_atten
       }
     }
     if (!alive) {                                    // a wait ran out: let the copies in flight land before the block ends
-      for (int i = 0; i < S::kStages; ++i) mbar_wait(&full[w][i], phase, kWaitTmaFull, -1);
+      for (int i = 0; i < S::kStages; ++i) mbar_wait(&full[i], phase, kWaitTmaFull, -1);
       found.x = -1;
     }
   }
   if (lane == 0) a.desc[worker] = found;
 }
 
-// Joins the parts of the units that begin in the four workers of a block of the first kernel: the maximum over a row's parts first,
+// Joins the parts of the units that begin in four workers of the first kernel: the maximum over a row's parts first,
 // then their sums with weights 2^(m_i - m), in order. A warp takes a row of few parts by itself; the rows of a unit of many (a long
 // sequence) are shared by the warps, one of which adds their sums in order.
 constexpr int kJoinWarps = 8, kFewParts = 4;
@@ -459,7 +448,7 @@ template <int D> __global__ void __launch_bounds__(kJoinWarps * 32, 3) kv8_join_
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   auto unit = [&](int k) {
-    const int w0 = blockIdx.x * kWarps + k;
+    const int w0 = blockIdx.x * kUnits + k;
     const int4 d = a.desc[w0];
     return d.x < 0 ? JoinUnit{} : JoinUnit{d.x, d.y >> 4, w0, d.z, min(d.w, a.NW - 1) - w0 + 1, d.y & 15};
   };
@@ -483,9 +472,9 @@ template <int D> __global__ void __launch_bounds__(kJoinWarps * 32, 3) kv8_join_
 #pragma unroll
     for (int j = 0; j < C; j += 2) store_out(a, oi + j, o[j] * r, o[j + 1] * r);
   };
-  for (int t = w; t < kWarps * per_unit; t += kJoinWarps) {
-    const JoinUnit u = unit(t % kWarps);
-    const int row = t / kWarps;
+  for (int t = w; t < kUnits * per_unit; t += kJoinWarps) {
+    const JoinUnit u = unit(t % kUnits);
+    const int row = t / kUnits;
     if (row >= u.rows || u.parts > kFewParts) continue;
     float m = lane < u.parts ? a.part_ml[slot(u, row, lane) * 2] : -INFINITY, l = 0.f, o[C] = {};
 #pragma unroll
@@ -496,7 +485,7 @@ template <int D> __global__ void __launch_bounds__(kJoinWarps * 32, 3) kv8_join_
     put(u, row, l, o);
   }
 #pragma unroll 1
-  for (int k = 0; k < kWarps; ++k) {
+  for (int k = 0; k < kUnits; ++k) {
     const JoinUnit u = unit(k);
     if (u.parts <= kFewParts) continue;
     // the rows side by side, `team` warps each
@@ -531,7 +520,7 @@ template <int D> __global__ void __launch_bounds__(kJoinWarps * 32, 3) kv8_join_
   }
 }
 
-template <int D, int E4M3, int SETS> int launch_sets(const KvAttnArgs& a, const CUtensorMap& map, int grid, cudaStream_t st) {
+template <int D, int E4M3, int SETS> int launch_sets(const KvAttnArgs& a, const CUtensorMap& map, cudaStream_t st) {
   using S = KvShape<D, SETS>;
   static bool set[16] = {};
   int dev = 0;
@@ -541,10 +530,10 @@ template <int D, int E4M3, int SETS> int launch_sets(const KvAttnArgs& a, const 
     if (e != cudaSuccess) return (int)e;
     if (dev >= 0 && dev < 16) set[dev] = true;
   }
-  kv8_attention_kernel<D, E4M3, SETS><<<grid, kThreads, S::kSmem, st>>>(map, a);
+  kv8_attention_kernel<D, E4M3, SETS><<<a.NW, 32, S::kSmem, st>>>(map, a);
   // the joining kernel is launched while the first one runs and waits for its end on the device
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
+  cfg.gridDim = dim3((unsigned)(a.NW / kUnits));
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -554,8 +543,8 @@ template <int D, int E4M3, int SETS> int launch_sets(const KvAttnArgs& a, const 
   cfg.numAttrs = 1;
   return (int)cudaLaunchKernelEx(&cfg, kv8_join_kernel<D>, a, 4 * SETS);
 }
-template <int D, int E4M3> int launch_kv8_attention(const KvAttnArgs& a, const CUtensorMap& map, int grid, cudaStream_t st) {
-  return a.G <= 4 ? launch_sets<D, E4M3, 1>(a, map, grid, st) : launch_sets<D, E4M3, 2>(a, map, grid, st);
+template <int D, int E4M3> int launch_kv8_attention(const KvAttnArgs& a, const CUtensorMap& map, cudaStream_t st) {
+  return a.G <= 4 ? launch_sets<D, E4M3, 1>(a, map, st) : launch_sets<D, E4M3, 2>(a, map, st);
 }
 }  // namespace hippo
 
@@ -572,7 +561,7 @@ struct KvAttendCall {
 };
 extern "C" int hippo_kv8_attention(const KvAttendCall* c) {
   const int sh = c->block_size == 16 ? 4 : c->block_size == 32 ? 5 : c->block_size == 64 ? 6 : -1;
-  if (sh < 0 || c->N < 1 || c->M < 1 || c->H < 1 || c->Hq % c->H || c->blocks < 1 || c->workers < kWarps || c->workers % kWarps ||
+  if (sh < 0 || c->N < 1 || c->M < 1 || c->H < 1 || c->Hq % c->H || c->blocks < 1 || c->workers < kUnits || c->workers % kUnits ||
       c->dtype < 0 || c->dtype > 2 || (c->D != 64 && c->D != 128))
     return -1;
   const int D = c->D;
@@ -597,7 +586,6 @@ extern "C" int hippo_kv8_attention(const KvAttendCall* c) {
                G <= 4 ? 1 : (G + 7) / 8, sh, (int)c->blocks, c->dtype, half_rows, c->scale, c->ws, c->ws + parts * D,
                (int4*)(c->ws + parts * (D + 2)), c->workers, rows};
   cudaStream_t st = (cudaStream_t)c->stream;
-  const int grid = c->workers / kWarps;
-  if (D == 128) return c->e4m3 ? launch_kv8_attention<128, 1>(a, map, grid, st) : launch_kv8_attention<128, 0>(a, map, grid, st);
-  return c->e4m3 ? launch_kv8_attention<64, 1>(a, map, grid, st) : launch_kv8_attention<64, 0>(a, map, grid, st);
+  if (D == 128) return c->e4m3 ? launch_kv8_attention<128, 1>(a, map, st) : launch_kv8_attention<128, 0>(a, map, st);
+  return c->e4m3 ? launch_kv8_attention<64, 1>(a, map, st) : launch_kv8_attention<64, 0>(a, map, st);
 }

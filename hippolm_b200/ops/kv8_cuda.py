@@ -88,7 +88,7 @@ def attention_decode(q, codes, scales, table, lens, scale: float, dev: int, qs, 
     sms = _SMS.get(dev)
     if sms is None:
         sms = _SMS[dev] = torch.cuda.get_device_properties(dev).multi_processor_count
-    # a warp takes tiles of 4096 / D tokens; three blocks of four warps (two where registers are short) fill a multiprocessor
+    # a warp takes tiles of 4096 / D tokens; twelve of them (eight where they need more registers) fill a multiprocessor
     workers = 4 * min((2 if D == 128 or G > 4 else 3) * sms, -(-(groups * tiles) // 4))
     ws = torch.empty(workers * (2 * min(G, 8) * (D + 2) + 4), dtype=torch.float32, device=dev)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
