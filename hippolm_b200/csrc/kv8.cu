@@ -4,6 +4,7 @@
 // code * scale. With a power of two the scaled value is rounded exactly once (x * 2^-e is exact), and a block whose scale has to
 // grow by 2^k only shifts its older codes: exact in e4m3 above the subnormals, one more rounding in int8.
 // The reference has no cache (src/models/model.py:180-219 re-runs the forward for every token).
+#include <type_traits>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include "sm100.cuh"
@@ -15,8 +16,8 @@ namespace hippo {
 // One CTA of 1024 threads walks the requests 1024 at a time: a thread owns a request, prefix sums over the CTA give the
 // positions in the stack of free blocks, in the packed tokens, and decide who still fits. Blocks pushed, blocks popped and slots are
 // then dealt out one by one to all threads, which find their request by bisection of the sums in shared memory (a request may
-// own one block or hundreds). Released requests push first. The work is a few dependent loads and barriers (latency-bound); more
-// CTAs would need a grid-wide order between pushes and pops.
+// own one block or hundreds). Released requests push first. The work is a few dependent loads and barriers (latency-bound: 4.2 us for
+// 16 requests of a token); more CTAs would need a grid-wide order between pushes and pops.
 constexpr int kPlanThreads = 1024, kBatch = 4;        // entries a thread has in flight
 
 __device__ __forceinline__ long long block_inclusive_scan(long long v, long long* warp_sum, long long& total) {
@@ -172,7 +173,9 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(
 }
 
 // Slot map of many tokens (prompts): 4 tokens a thread, the request of the first found in the packed ends, the table rows stay in
-// L1. Runs behind the planning kernel, whose single CTA would write 8 bytes a token at one SM's rate.
+// L1. Runs behind the planning kernel, whose single CTA would write 8 bytes a token at one SM's rate: 32 000 tokens 7.6 us with this
+// kernel, 19.2 without, 8 192 7.3 and 8.3, 2 048 7.3 and 5.5. The second launch costs the host some 5 us, so that it is taken from
+// 16 thousand tokens on, where the device is the longer of the two.
 __global__ void __launch_bounds__(256) kv8_slots_kernel(
     const int* __restrict__ table, long long table_ld, const int* __restrict__ lens_out, const unsigned char* __restrict__ served,
     const int* __restrict__ cu, int N, int sh, long long num_tokens, long long* __restrict__ slots) {
@@ -304,12 +307,16 @@ __device__ __forceinline__ bool continues(const WriteArgs& a, long long prev, lo
   return slot_ok(a, prev) && s == prev + 1 && (s & ((1 << a.sh) - 1)) != 0;
 }
 
-// One CTA for the runs that start in a window of W tokens, and for a few (head, half) pairs. It finds the runs (consecutive tokens in
-// consecutive slots of one block) by ballots. Runs of up to kShort tokens (decoding: one) go to groups of lanes that hold a row, 128 /
-// (D / 8) of them at work; longer runs (prompts) are read once into registers by the whole CTA, the next pair's rows in flight while
-// this one's are reduced and stored. HBM-bound for prompts (bytes = 2 T H D (element + 1)), latency for a token a request.
-// The window is small for few tokens, which spreads them over the card, and a block's tokens for many.
-constexpr int kShort = 4;
+// scale = 2^e with the smallest e under which a run's largest value (and the older ones of its block) fit the codes; code =
+// round(x 2^-e). One CTA for the runs that start in a window of W tokens, and for a few (head, half) pairs. It finds the runs
+// (consecutive tokens in consecutive slots of one block) by ballots. Runs of up to kShort tokens (decoding: one) go to groups of lanes
+// that hold a row, 128 / (D / 8) of them at work, kHeld rows in registers at a time (of a longer one the first are read again, from
+// L1); longer runs (prompts) are read once into registers by the whole CTA, the next pair's rows in flight while this one's are
+// reduced and stored. With kShort 12 instead of 4, 2000 x 8 tokens of 16 heads of 128 take 42 us, not 78 (196 MB: 4.7 TB/s); with 16,
+// the ends of 24 x 1040 cost 2 us more. A single token has a form of its own (2000 x 1, 32 heads: 24.0 us against 26.7 with the one for four).
+// HBM and issue slots both bound prompts (24 x 1040 tokens, 16 heads of 128, bf16 -> e4m3: 307 MB in 57.4 us = 5.3 TB/s; issue 65 %),
+// latency a token a request (32 x 1, 32 heads: 2.8 us).
+constexpr int kShort = 12, kHeld = 4;
 
 template <typename T, int D, int E4M3, int BS> struct WriteShape {
   static constexpr int kBytes = BS * D * (int)sizeof(T);                 // a run at most
@@ -358,26 +365,46 @@ __global__ void __launch_bounds__(128, WriteShape<T, D, E4M3, BS>::kBlocks) kv8_
     float* scale = a.scales + (pair & 1 ? a.half_scales : 0) + bh;
     uint8_t* codes = a.codes + (pair & 1 ? a.half_codes : 0) + bh * BS * D;
     const T* x = source(pair, t);
-    Row8<T> row[kShort];
-#pragma unroll
-    for (int i = 0; i < kShort; ++i)
-      if (i < L) row[i].load(x + i * ld); else row[i].zero();
     const float old = off ? *scale : 0.f;
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < kShort; ++i) m = row[i].amax(m);
-    m = Row8<T>::bits(m);
     const unsigned group = (LPR == 16 ? 0xffffu : 0xffu) << (lane & ~(LPR - 1) & 31);
+    auto store = [&](auto held, auto reload) {       // `held` rows in registers at a time; a run of more is read again to be encoded
+      constexpr int K = decltype(held)::value;
+      constexpr bool kReload = decltype(reload)::value;
+      Row8<T> row[K];
+      auto load = [&](int i0) {
 #pragma unroll
-    for (int d = 1; d < LPR; d <<= 1) m = max(m, __shfl_xor_sync(group, m, d));
-    const RunScale rs = run_scale<E4M3>(m, old, off > 0);
-    if (rs.down < 0) shift_codes<E4M3>(codes, off * D, rs.down, tid % LPR, LPR);
-    const float inv = pow2f(-rs.e);
+        for (int i = 0; i < K; ++i)
+          if (i0 + i < L) row[i].load(x + (i0 + i) * ld); else row[i].zero();
+      };
+      uint32_t m = 0;
+      int i0 = kReload ? (L - 1) / K * K : 0;         // from the last rows, so that the first ones stay in registers
+#pragma unroll 1
+      for (;; i0 -= K) {
+        load(i0);
 #pragma unroll
-    for (int i = 0; i < kShort; ++i)
-      if (i < L) *(uint2*)(codes + (off + i) * D + col) = encode_row<E4M3>(row[i], inv, rs.bad);
-    __syncwarp(group);                               // every lane has read the old scale
-    if (tid % LPR == 0) *scale = rs.bad ? __uint_as_float(0x7fffffffu) : pow2f(rs.e);
+        for (int i = 0; i < K; ++i) m = row[i].amax(m);
+        if (!kReload || i0 == 0) break;
+      }
+      m = Row8<T>::bits(m);
+#pragma unroll
+      for (int d = 1; d < LPR; d <<= 1) m = max(m, __shfl_xor_sync(group, m, d));
+      const RunScale rs = run_scale<E4M3>(m, old, off > 0);
+      if (rs.down < 0) shift_codes<E4M3>(codes, off * D, rs.down, tid % LPR, LPR);
+      const float inv = pow2f(-rs.e);
+#pragma unroll 1
+      for (;;) {
+#pragma unroll
+        for (int i = 0; i < K; ++i)
+          if (i0 + i < L) *(uint2*)(codes + (off + i0 + i) * D + col) = encode_row<E4M3>(row[i], inv, rs.bad);
+        if (!kReload || (i0 += K) >= L) break;
+        load(i0);
+      }
+      __syncwarp(group);                             // every lane has read the old scale
+      if (tid % LPR == 0) *scale = rs.bad ? __uint_as_float(0x7fffffffu) : pow2f(rs.e);
+    };
+    if (L == 1) store(std::integral_constant<int, 1>(), std::false_type());
+    else if (L <= kHeld) store(std::integral_constant<int, kHeld>(), std::false_type());
+    else store(std::integral_constant<int, kHeld>(), std::true_type());
   }
 
   for (int q = 0; q < longs; ++q) {
@@ -433,7 +460,7 @@ template <typename T, int D, int E4M3> int launch_write(const WriteArgs& a, int 
   const int bs = 1 << a.sh, pairs = a.T * a.H <= 32768 ? 2 : 4, groups = (2 * a.H + pairs - 1) / pairs;
   int W = window;
   if (W == 0) {                                      // some two thousand blocks, or a window of a whole block's tokens
-    W = 4;
+    W = 4;                                           // (24 x 1040 tokens 77 us with windows of 4, 58 of 32; 32 x 1 2.8 and 7.6)
     while (W < bs && (a.T + W - 1) / W * groups > 2048) W *= 2;
   }
   if (W < 1 || W > bs) return -1;
@@ -456,7 +483,7 @@ using namespace hippo;
 
 // table [N][M] int32 (row pitch table_ld), lens / new_lens [N], free_list [cap], free_count [1], release [N] or null; out: slots
 // [num_tokens], lens_out [N], count_out [1], served [N], cu [N + 1]
-// (ends of the packed tokens; null: the planning block writes the slots itself, which is the faster form up to some 16 thousand).
+// (ends of the packed tokens; null: the planning block writes the slots itself).
 struct KvPlanCall {
   int* table; const int *lens, *new_lens; int* free_list; const int* free_count; const unsigned char* release;
   long long* slots; int *lens_out, *count_out; unsigned char* served; int* cu; void* stream;

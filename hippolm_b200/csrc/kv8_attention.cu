@@ -2,16 +2,21 @@
 // and one (s_K, s_V) per (block, kv head).
 //
 // Bound by HBM: a token and kv head costs 2 D bytes of codes, read once for the query heads that share the kv head (up to 8 of them
-// together). Work is cut in tiles of 32 tokens (64 for head_dim 64: 8 KB); the tiles of all (sequence, kv head, group of query heads) form one list that is
-// divided evenly over one resident wave of one-warp blocks, whatever the lengths (the start of a unit counts as one more tile: its
-// query rows and its result cost about as much). A warp streams its tiles through a TMA ring and carries the running maximum and sum; a unit that spans several warps leaves partial (m, l, o)
-// rows that a second, small kernel joins in a fixed order, so results do not depend on timing.
+// together). Work is cut in tiles of 32 tokens (64 for head_dim 64: 8 KB); the tiles of all (sequence, kv head, group of query heads)
+// form one list that is divided evenly over one resident wave of one-warp blocks, whatever the lengths (the start of a unit counts as
+// one more tile: its query rows and its result cost about as much). A warp streams its tiles through a TMA ring and carries the
+// running maximum and sum; a unit that spans several warps leaves partial (m, l, o) rows that a second, small kernel joins in a fixed
+// order, so results do not depend on timing.
 //
 // Arithmetic: codes are exact in fp16, so mma.m16n8k16 (fp16 operands, fp32 accumulators) is exact for them. They are the 16-row
 // operand of both products (S^T = K q^T, O^T = V^T P^T); the 8 columns are 4 query heads, each as two fp16 terms of the query and of
 // the probabilities (21 bits or more), whose two sums meet in one thread. P^T comes from the scores' fragments by movmatrix. The
 // converted codes, not the tensor pipe, set the instruction count, so the narrow side of the product is the query's. Legacy mma is
 // deliberate: with 1 to 8 live columns a 128-row tcgen05 tile would multiply zeros, and the kernel waits for memory.
+//
+// Measured, both kernels (device time in a row of calls, inputs above L2): 32 sequences of 6001 to 8192 tokens, 32 heads of 128, e4m3:
+// 300 us = 6.2 TB/s; 16 x 4096 tokens, 32 heads of 128: 93 us = 5.8 TB/s (int8 90); 2 x 131072, 4 heads of 128: 50.3 us = 5.3 TB/s;
+// 16 x 4096, 64 heads on 8 of 128: 38.1 us; 1 x 500, 16 heads: 9.0 us. Short calls wait for lens -> table -> first tiles (4 us) and for the join (3 us).
 // In the reference a decoding step re-runs the whole forward (src/models/model.py:180-219).
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
@@ -544,6 +549,7 @@ template <int D, int E4M3, int SETS> int launch_sets(const KvAttnArgs& a, const 
   return (int)cudaLaunchKernelEx(&cfg, kv8_join_kernel<D>, a, 4 * SETS);
 }
 template <int D, int E4M3> int launch_kv8_attention(const KvAttnArgs& a, const CUtensorMap& map, cudaStream_t st) {
+  // five to eight heads on one kv head read the codes once together (16 x 4096 tokens, 64 heads on 8: 38 us, in passes of four 48)
   return a.G <= 4 ? launch_sets<D, E4M3, 1>(a, map, st) : launch_sets<D, E4M3, 2>(a, map, st);
 }
 }  // namespace hippo

@@ -110,6 +110,24 @@ def test_write_of_many_runs_equals_a_few(kind, bs):
     check_write(k[:300], v[:300], few.to(DEV), c0, s0, kind)
 
 
+@pytest.mark.parametrize("kind,dtype", [("e4m3", torch.bfloat16), ("int8", torch.float32), ("int8", torch.float16)])
+@pytest.mark.parametrize("D,bs", [(64, 32), (128, 32), (128, 16)])
+def test_write_of_runs_of_every_short_length(kind, dtype, D, bs):
+    """Runs of 1 to 16 tokens, alone and behind older ones, the largest value in their first, middle or last row; one is poisoned."""
+    runs = [(b, 0 if b % 2 == 0 else min(b, bs - 1 - b // 2), b // 2 + 1) for b in range(32)]
+    runs = [(b, min(off, bs - ln), ln) for b, off, ln in runs]
+    codes, scales, g = cache_case(7, kind, 3, D, bs, 32)
+    slots = runs_to_slots(runs, bs)
+    k, v = (torch.randn(slots.numel(), 3, D, generator=g) for _ in range(2))
+    at = 0
+    for b, _, ln in runs:
+        k[at + (b * 5) % ln, b % 3, b % D] = 300.0
+        if b == 21:
+            v[at + ln - 1, 1, 5] = math.inf
+        at += ln
+    check_write(*to(DEV, k.to(dtype), v.to(dtype), slots, codes, scales), kind, write=ops.kv8_write)
+
+
 def test_write_leaves_the_rest_of_the_cache():
     codes, scales = kv8_empty(60, 2, 64, 64, "int8", DEV)
     codes.fill_(77); scales.fill_(0.5)
