@@ -909,6 +909,8 @@ class HippoModel(nn.Module):
         Logits exist for ``chunk_rows`` tokens at a time."""
         ids = input_ids.reshape(-1)
         T = ids.numel()
+        if T == 0:
+            return ops.token_logprobs(torch.empty(0, self.cfg.vocab_size, device=ids.device), ids, top_k=top_k)
         if cu_seqlens is None:
             row = input_ids.shape[1] if input_ids.dim() == 2 else T
             cu_seqlens = torch.arange(0, T + 1, max(row, 1), device=ids.device, dtype=torch.int32)

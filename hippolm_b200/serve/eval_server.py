@@ -106,8 +106,8 @@ class EvalService:
                 eos = getattr(self.tok, "eos_token_id", None)
                 prompts = [torch.tensor(p.ids, dtype=torch.long, device=dev) for p in batch]
                 with self.lock:
-                    if self._batched:
-                        asked = [p.logprobs for p in batch if p.logprobs is not None]
+                    asked = [p.logprobs for p in batch if p.logprobs is not None]
+                    if self._batched or asked:
                         outs = self.model.generate_batch(prompts, [p.max_tokens for p in batch],
                                                          [p.temperature for p in batch], [p.top_k for p in batch], eos,
                                                          [p.top_p for p in batch], kv_cache=self.kv_cache,
@@ -118,7 +118,8 @@ class EvalService:
                                 p.scores = sc
                     else:
                         outs = [self.model.generate(x, p.max_tokens, temperature=p.temperature, top_k=p.top_k,
-                                                    eos_token_id=eos, top_p=p.top_p) for x, p in zip(prompts, batch)]
+                                                    eos_token_id=eos, top_p=p.top_p, kv_cache=self.kv_cache)
+                                for x, p in zip(prompts, batch)]
                 self.batches_run += 1
                 self.largest_batch = max(self.largest_batch, len(batch))
                 for p, o in zip(batch, outs):

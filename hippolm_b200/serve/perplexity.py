@@ -129,18 +129,20 @@ def score_documents(model, tokenizer, documents: Iterable[str], seq_len: int = 1
                 row["top_logprobs"], row["top_tokens"] = [None] + cols[2][s + 1:e], [None] + cols[3][s + 1:e]
             yield row
 
-    for d, text in enumerate(documents):
-        toks = tokenizer.encode(text, add_special_tokens=False)
-        if eos is not None:
-            toks = toks + [eos]
-        for s in range(0, len(toks), seq_len):
-            piece = toks[s:s + seq_len]
-            if len(piece) >= 2:
-                pending.append((d, piece))
-                seen += len(piece) - 1
-        if sum(len(p) for _, p in pending) >= batch_tokens:
-            yield from flush()
-        if max_tokens is not None and seen >= max_tokens:
-            break
-    yield from flush()
-    model.train(was_training)
+    try:
+        for d, text in enumerate(documents):
+            toks = tokenizer.encode(text, add_special_tokens=False)
+            if eos is not None:
+                toks = toks + [eos]
+            for s in range(0, len(toks), seq_len):
+                piece = toks[s:s + seq_len]
+                if len(piece) >= 2:
+                    pending.append((d, piece))
+                    seen += len(piece) - 1
+            if sum(len(p) for _, p in pending) >= batch_tokens:
+                yield from flush()
+            if max_tokens is not None and seen >= max_tokens:
+                break
+        yield from flush()
+    finally:                                               # (also of a caller that reads some of the rows only)
+        model.train(was_training)

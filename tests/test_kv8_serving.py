@@ -205,6 +205,30 @@ def test_token_scores_of_documents(tmp_path):
         assert all(len(t) == 2 for t in r["top_tokens"][1:]) and all(0 <= e <= math.log(258) + 1e-4 for e in r["entropy"][1:])
 
 
+def test_scores_of_no_text_and_of_a_few_rows():
+    from hippolm_b200.serve.perplexity import score_documents
+    m = model()
+    got = m.token_logprobs(torch.empty(0, dtype=torch.long), top_k=3)
+    assert got.logprob.shape == got.entropy.shape == (0,) and got.top_ids.shape == got.top_logprobs.shape == (0, 3)
+    cfg = HippoConfig(vocab_size=258, hidden_size=32, num_heads=2, head_dim=16, num_layers=2, num_blocks=1, intermediate_size=64,
+                      full_attn_interval=2)
+    m = HippoModel(cfg, seed=1)
+    rows = score_documents(m, ByteTokenizer(), ["one text", "another"], batch_tokens=4)
+    assert next(rows)["document"] == 0
+    rows.close()                                                               # what stops early leaves the model as it was
+    assert m.training
+
+
+def test_requests_served_one_by_one_have_the_same_answers():
+    body = {"prompt": "abc", "max_tokens": 4, "logprobs": 2}
+    want, got = small_service(kv_cache="int8"), small_service(kv_cache="int8")
+    got._batched = False
+    for b in (body, {"prompt": "abc", "max_tokens": 4}):
+        assert got.complete(b, chat=False)["choices"] == want.complete(b, chat=False)["choices"]
+    want.close()
+    got.close()
+
+
 def _tp_worker(rank, world, port, out_path):
     import os
     os.environ.update({"RANK": str(rank), "WORLD_SIZE": str(world), "LOCAL_RANK": str(rank), "MASTER_ADDR": "127.0.0.1",
