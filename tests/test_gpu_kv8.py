@@ -278,6 +278,31 @@ def test_scores_match_64_bits(T, V, top, dtype):
     assert plain_call.top_ids is None and torch.equal(plain_call.logprob, got.logprob) and torch.equal(plain_call.entropy, got.entropy)
 
 
+@pytest.mark.parametrize("T,V,top", [(5000, 4099, 20), (5000, 2047, 0), (4800, 9001, 3), (2500, 4097, 32), (600, 20011, 5), (150, 66001, 20)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_scores_of_many_rows(T, V, top, dtype):
+    """More rows than the card holds at once (blocks of one warp and of few), rows at odd addresses, equal logits among the largest."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    z = (torch.randn(T, V + 3, device=DEV, generator=g) * 3).to(dtype)[:, 1:V + 1]
+    z[::7] = z[::7].round()
+    z[5, :] = -math.inf
+    z[5, V - 1] = 1.0
+    ids = torch.randint(0, V, (T,), device=DEV, generator=g)
+    ids[5] = V - 1
+    got = ops.token_logprobs(z, ids, top_k=top)
+    b = score_bound(z[6:], dtype)
+    for s in range(0, T, 500):
+        lp = torch.log_softmax(z[s:s + 500].double(), -1)
+        assert float((got.logprob[s:s + 500] - lp.gather(1, ids[s:s + 500, None])[:, 0]).abs().max()) <= b
+        assert float((got.entropy[s:s + 500] - torch.special.entr(lp.exp()).sum(-1)).abs().max()) <= b * (1 + 2 * float(z[6:].abs().max()))
+        if top:
+            order = torch.sort(z[s:s + 500].float() + 0.0, dim=-1, descending=True, stable=True).indices[:, :top]
+            assert torch.equal(got.top_ids[s:s + 500], order)
+            want, have = lp.gather(1, order), got.top_logprobs[s:s + 500]
+            assert torch.equal(torch.isneginf(want), torch.isneginf(have))
+            assert float((have - want).nan_to_num(0.0).abs().max()) <= b
+
+
 def test_scores_of_masked_and_broken_rows():
     check_special(DEV)
 
