@@ -18,6 +18,7 @@
 // 300 us = 6.2 TB/s; 16 x 4096 tokens, 32 heads of 128: 93 us = 5.8 TB/s (int8 90); 2 x 131072, 4 heads of 128: 50.3 us = 5.3 TB/s;
 // 16 x 4096, 64 heads on 8 of 128: 38.1 us; 1 x 500, 16 heads: 9.0 us. Short calls wait for lens -> table -> first tiles (4 us) and for the join (3 us).
 // In the reference a decoding step re-runs the whole forward (src/models/model.py:180-219).
+#include <type_traits>
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include "sm100.cuh"
@@ -440,9 +441,11 @@ __global__ void __launch_bounds__(32, KvShape<D, SETS>::kBlocks) kv8_attention_k
   if (lane == 0) a.desc[worker] = found;
 }
 
-// Joins the parts of the units that begin in four workers of the first kernel: the maximum over a row's parts first,
-// then their sums with weights 2^(m_i - m), in order. A warp takes a row of few parts by itself; the rows of a unit of many (a long
-// sequence) are shared by the warps, one of which adds their sums in order.
+// Joins the parts of the units that begin in four workers of the first kernel: (m, l, o) of the parts in order, rescaled whenever a
+// batch of them brings a larger m. The kernel is a chain of dependent reads (3 to 4 us after the first one's end), so a batch's
+// maxima and rows are under way together. A warp takes a row of few parts by itself; the rows of a unit of many (a long sequence) are
+// shared by the warps, one of which joins their sums in order. Blocks of eight warps for four workers: with four warps for two
+// 2 x 131072 tokens take 52.7 us, not 50.5, with two for one 57.0.
 constexpr int kJoinWarps = 8, kFewParts = 4;
 struct JoinUnit {
   int n, head0, w0, slot0, parts, rows;              // sequence, first query head, first worker and its slot, query rows
@@ -457,69 +460,87 @@ template <int D> __global__ void __launch_bounds__(kJoinWarps * 32, 3) kv8_join_
     const int4 d = a.desc[w0];
     return d.x < 0 ? JoinUnit{} : JoinUnit{d.x, d.y >> 4, w0, d.z, min(d.w, a.NW - 1) - w0 + 1, d.y & 15};
   };
-  auto slot = [&](const JoinUnit& u, int row, int i) { return (long long)(i == 0 ? u.slot0 : 2 * (u.w0 + i)) * a.rows + row; };
-  auto add = [&](const JoinUnit& u, int row, int i, float m, float& l, float (&o)[C]) {
-    const long long sl = slot(u, row, i);
-    const float2 ml = *(const float2*)(a.part_ml + sl * 2);
-    const float r = ex2(ml.x - m);
-    l += ml.y * r;
-    if (C == 4) {
-      const float4 x = *(const float4*)(a.part + sl * D + lane * 4);
-      o[0] += x.x * r; o[1] += x.y * r; o[C - 2] += x.z * r; o[C - 1] += x.w * r;
-    } else {
-      const float2 x = *(const float2*)(a.part + sl * D + lane * 2);
-      o[0] += x.x * r; o[1] += x.y * r;
+  struct Sum { float m, l, o[C]; };
+  // parts first, first + step, ... of a row
+  auto gather = [&](const JoinUnit& u, int row, int first, int step, auto batch) {
+    constexpr int B = decltype(batch)::value;
+    Sum t{-INFINITY, 0.f, {}};
+#pragma unroll 1
+    for (int i0 = first; i0 < u.parts; i0 += B * step) {
+      float2 ml[B];
+      float x[B][C];
+#pragma unroll
+      for (int j = 0; j < B; ++j) {
+        const int i = i0 + j * step;
+        ml[j] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int k = 0; k < C; ++k) x[j][k] = 0.f;
+        if (i < u.parts) {
+          const long long sl = (long long)(i == 0 ? u.slot0 : 2 * (u.w0 + i)) * a.rows + row;
+          ml[j] = *(const float2*)(a.part_ml + sl * 2);
+          if (C == 4) *(float4*)x[j] = *(const float4*)(a.part + sl * D + lane * 4);
+          else *(float2*)x[j] = *(const float2*)(a.part + sl * D + lane * 2);
+        }
+      }
+      float m = t.m;
+#pragma unroll
+      for (int j = 0; j < B; ++j) m = fmaxf(m, ml[j].x);
+      const float mu = m == -INFINITY ? 0.f : m, back = ex2(t.m - mu);
+      t.m = m;
+      t.l *= back;
+#pragma unroll
+      for (int k = 0; k < C; ++k) t.o[k] *= back;
+#pragma unroll
+      for (int j = 0; j < B; ++j) {
+        const float r = ex2(ml[j].x - mu);
+        t.l += ml[j].y * r;
+#pragma unroll
+        for (int k = 0; k < C; ++k) t.o[k] += x[j][k] * r;
+      }
     }
+    return t;
   };
-  auto put = [&](const JoinUnit& u, int row, float l, const float (&o)[C]) {
-    const float r = l == 0.f ? 0.f : 1.f / l;
+  auto put = [&](const JoinUnit& u, int row, const Sum& t) {
+    const float r = t.l == 0.f ? 0.f : 1.f / t.l;
     const long long oi = ((long long)u.n * a.H * a.G + u.head0 + row) * D + lane * C;
 #pragma unroll
-    for (int j = 0; j < C; j += 2) store_out(a, oi + j, o[j] * r, o[j + 1] * r);
+    for (int j = 0; j < C; j += 2) store_out(a, oi + j, t.o[j] * r, t.o[j + 1] * r);
   };
   for (int t = w; t < kUnits * per_unit; t += kJoinWarps) {
     const JoinUnit u = unit(t % kUnits);
     const int row = t / kUnits;
     if (row >= u.rows || u.parts > kFewParts) continue;
-    float m = lane < u.parts ? a.part_ml[slot(u, row, lane) * 2] : -INFINITY, l = 0.f, o[C] = {};
-#pragma unroll
-    for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-    if (m == -INFINITY) m = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < u.parts; ++i) add(u, row, i, m, l, o);
-    put(u, row, l, o);
+    put(u, row, gather(u, row, 0, 1, std::integral_constant<int, kFewParts>()));
   }
 #pragma unroll 1
   for (int k = 0; k < kUnits; ++k) {
     const JoinUnit u = unit(k);
     if (u.parts <= kFewParts) continue;
     // the rows side by side, `team` warps each
-    const int team = u.rows > 4 ? 1 : u.rows > 2 ? 2 : u.rows > 1 ? 4 : 8, row = w / team, first = w - row * team;
+    const int team = u.rows > 4 ? 1 : u.rows > 2 ? 2 : u.rows > 1 ? 4 : 8, row = w / team, first = w % team;
     const bool on = row < u.rows;
-    float m = -INFINITY, l = 0.f, o[C] = {};
-    if (on)
-      for (int i = first * 32 + lane; i < u.parts; i += team * 32) m = fmaxf(m, a.part_ml[slot(u, row, i) * 2]);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    if (lane == 0) s_m[w] = m;
-    __syncthreads();
-    for (int i = 0; i < team; ++i) m = fmaxf(m, s_m[row * team + i]);
-    if (m == -INFINITY) m = 0.f;
-    if (on) {
-#pragma unroll 8
-      for (int i = first; i < u.parts; i += team) add(u, row, i, m, l, o);
+    Sum t{-INFINITY, 0.f, {}};
+    if (on) t = gather(u, row, first, team, std::integral_constant<int, 8>());
+    if (team == 1) {
+      if (on) put(u, row, t);
+      continue;
     }
 #pragma unroll
-    for (int j = 0; j < C; ++j) s_o[w][lane * C + j] = o[j];
-    if (lane == 0) s_l[w] = l;
+    for (int j = 0; j < C; ++j) s_o[w][lane * C + j] = t.o[j];
+    if (lane == 0) { s_m[w] = t.m; s_l[w] = t.l; }
     __syncthreads();
     if (on && first == 0) {
-      for (int i = 1; i < team; ++i) {
-        l += s_l[w + i];
+      float m = t.m;
+      for (int i = 1; i < team; ++i) m = fmaxf(m, s_m[w + i]);
+      const float mu = m == -INFINITY ? 0.f : m;
+      Sum all{m, 0.f, {}};
+      for (int i = 0; i < team; ++i) {
+        const float r = ex2(s_m[w + i] - mu);
+        all.l += s_l[w + i] * r;
 #pragma unroll
-        for (int j = 0; j < C; ++j) o[j] += s_o[w + i][lane * C + j];
+        for (int j = 0; j < C; ++j) all.o[j] += s_o[w + i][lane * C + j] * r;
       }
-      put(u, row, l, o);
+      put(u, row, all);
     }
     __syncthreads();
   }
