@@ -10,9 +10,10 @@
 //
 // Arithmetic: codes are exact in fp16, so mma.m16n8k16 (fp16 operands, fp32 accumulators) is exact for them. They are the 16-row
 // operand of both products (S^T = K q^T, O^T = V^T P^T); the 8 columns are 4 query heads, each as two fp16 terms of the query and of
-// the probabilities (21 bits or more), whose two sums meet in one thread. P^T comes from the scores' fragments by movmatrix. The
-// converted codes, not the tensor pipe, set the instruction count, so the narrow side of the product is the query's. Legacy mma is
-// deliberate: with 1 to 8 live columns a 128-row tcgen05 tile would multiply zeros, and the kernel waits for memory.
+// the probabilities, whose two sums meet in one thread. Two terms hold 22 bits of a probability down to 2^-17 of the largest, and steps
+// of 2^-39 of it below. P^T comes from the scores' fragments by movmatrix. The converted codes, not the tensor pipe, set the
+// instruction count, so the narrow side of the product is the query's. Legacy mma is deliberate: with 1 to 8 live columns a 128-row
+// tcgen05 tile would multiply zeros, and the kernel waits for memory.
 //
 // Measured, both kernels (device time in a row of calls, inputs above L2): 32 sequences of 6001 to 8192 tokens, 32 heads of 128, e4m3:
 // 300 us = 6.2 TB/s; 16 x 4096 tokens, 32 heads of 128: 93 us = 5.8 TB/s (int8 90); 2 x 131072, 4 heads of 128: 50.3 us = 5.3 TB/s;
@@ -28,6 +29,9 @@
 namespace hippo {
 constexpr int kUnits = 4;                            // workers whose units a block of the joining kernel looks after
 constexpr float kLog2e = 1.4426950408889634f;
+// Probabilities (times their value scale, relative to the largest: 0 .. 1) are multiplied by 2^15 before they are split: fp16's smallest
+// step, 2^-24, then is 2^-39 of the largest, so that thousands of weak tokens beside a strong one keep their share.
+constexpr float kLift = 32768.f;
 
 struct KvAttnArgs {
   const void* q; void* out;
@@ -352,7 +356,7 @@ __global__ void __launch_bounds__(32, KvShape<D, SETS>::kBlocks) kv8_attention_k
 #pragma unroll
           for (int i = 0; i < 2 * NG; ++i) {
             l[t] += ex2(y[i] - mu);
-            const float p = ex2(z[i] - mzu);
+            const float p = ex2(z[i] - mzu) * kLift;
             pb[t][i] = transpose8x8(pack2(p, p - __half2float(__float2half_rn(p))));
           }
         }
@@ -410,8 +414,8 @@ __global__ void __launch_bounds__(32, KvShape<D, SETS>::kBlocks) kv8_attention_k
           float lt = l[t];
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, d);
-          // o is held relative to the maximum of p s_V, l to that of p
-          const float back = lt == 0.f ? 0.f : ex2(mv[t] - m[t]), r = done ? (lt == 0.f ? 0.f : back / lt) : back;
+          // o is held relative to the maximum of p s_V and kLift times as large, l relative to the maximum of p
+          const float back = lt == 0.f ? 0.f : ex2(mv[t] - m[t]) * (1.f / kLift), r = done ? (lt == 0.f ? 0.f : back / lt) : back;
           const int row = t * 4 + c;                 // this lane: query head c of the set, output columns DL g ...
           if (g0 + row >= a.G) continue;
           if (done) {

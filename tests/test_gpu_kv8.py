@@ -607,3 +607,39 @@ def test_a_block_of_zeros_beside_large_values():
         scales[1, int(table[0, 1])] = 2.0 ** -100
         scales[1, int(table[0, 0])] = 2.0 ** 90
         plain.check_attend(ops.attention_decode_kv8(q, codes, scales, table, ln), q, codes, scales, table, ln, 64 ** -0.5)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("D,heads", [(64, 4), (128, 4), (64, 8), (128, 8)])
+@pytest.mark.parametrize("sink_scale", [0, 4])
+def test_attention_of_a_sink_and_a_flat_tail(kind, D, heads, sink_scale):
+    """One strong token whose value is zero before thousands of equal weak ones: the output is the tail's share, from 2^-8 to 2^-38 of
+    the strong token's weight each. Far more units than warps (one table row for all), so that a warp holds whole units; queries of
+    one channel, positive values, so that every bound is relative. ``sink_scale``: the strong token's block has a value scale of
+    2^4 times the others'."""
+    L, bs, N = 8192, 64, 4 * 12 * 148
+    g = torch.Generator().manual_seed(D + heads)
+    codes, scales = kv8_empty(L // bs, 1, D, bs, kind, DEV)
+    keys, values = torch.zeros(L, D), torch.randint(1, 15, (L, D), generator=g).float()
+    keys[0, 0], values[0] = 64.0, 0.0                                          # whole numbers below 16 and 64 are codes of both types
+    values[1:bs] = 0.0                                                         # (the strong token's block holds no other value)
+    for i, x in enumerate((keys, values)):
+        codes[i, :, 0] = x.view(-1, bs, D).to(codes.dtype).to(DEV)
+    scales.fill_(2.0 ** -6)
+    scales[1, 0] *= 2.0 ** sink_scale
+    offsets = torch.tensor([8.0, 17.0, 21.0, 25.05, 12.0, 19.5, 30.0, 38.0])[:heads]
+    q = torch.zeros(heads, D)
+    q[:, 0] = offsets / (math.log2(math.e) * D ** -0.5)                        # the strong token's score: key 64 * 2^-6 = 1
+    table = torch.arange(L // bs, dtype=torch.int32, device=DEV)[None].expand(N, -1)
+    got = ops.attention_decode_kv8(q.to(DEV).expand(N, -1, -1), codes, scales, table, torch.full((N,), L, dtype=torch.int32, device=DEV))
+    s = q.double()[:, :1] * (keys.double()[:, 0] * 2.0 ** -6) * D ** -0.5
+    p = torch.exp(s - s.amax(1, keepdim=True))
+    want = (p / p.sum(1, keepdim=True)) @ (values.double() * 2.0 ** -6)
+    A = float(offsets.max())
+    # a score: the query's two terms 2^-23, its sum and the factors of the scale eight roundings, the exponential's argument and value;
+    # then the split of the probabilities (2^-21), sums of the tokens, the division. All terms are positive: relative.
+    rel = 2 * math.log(2) * (A * 16 * 2.0 ** -24 + 2.0 ** -21) + 2.0 ** -20 + (L / 8 + 64) * 2.0 ** -24
+    # and half the last step of a probability's two terms, 2^-40 of the largest p * value scale, for every token's code
+    tol = want * rel + L * 2.0 ** -40 * 2.0 ** (sink_scale - 6) * 14
+    off = (got.double().cpu() - want).abs()
+    assert bool((off <= tol).all()), ((off / want).amax((0, 2)), (off / tol).amax((0, 2)))
