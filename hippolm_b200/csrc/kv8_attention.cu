@@ -10,10 +10,10 @@
 //
 // Arithmetic: codes are exact in fp16, so mma.m16n8k16 (fp16 operands, fp32 accumulators) is exact for them. They are the 16-row
 // operand of both products (S^T = K q^T, O^T = V^T P^T); the 8 columns are 4 query heads, each as two fp16 terms of the query and of
-// the probabilities, whose two sums meet in one thread. Two terms hold 22 bits of a probability down to 2^-17 of the largest, and steps
-// of 2^-39 of it below. P^T comes from the scores' fragments by movmatrix. The converted codes, not the tensor pipe, set the
-// instruction count, so the narrow side of the product is the query's. Legacy mma is deliberate: with 1 to 8 live columns a 128-row
-// tcgen05 tile would multiply zeros, and the kernel waits for memory.
+// the probabilities, whose two sums meet in one thread. Both are brought to fp16's range first: two terms hold 22 bits of a value
+// down to 2^-16 of the row's largest, and steps of 2^-38 of it below. P^T comes from the scores' fragments by movmatrix. The
+// converted codes, not the tensor pipe, set the instruction count, so the narrow side of the product is the query's. Legacy mma is
+// deliberate: with 1 to 8 live columns a 128-row tcgen05 tile would multiply zeros, and the kernel waits for memory.
 //
 // Measured, both kernels (device time in a row of calls, inputs above L2): 32 sequences of 6001 to 8192 tokens, 32 heads of 128, e4m3:
 // 300 us = 6.2 TB/s; 16 x 4096 tokens, 32 heads of 128: 93 us = 5.8 TB/s (int8 90); 2 x 131072, 4 heads of 128: 50.3 us = 5.3 TB/s;
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(32, KvShape<D, SETS>::kBlocks) kv8_attention_k
     const uint32_t k_at = g * D + (D == 128 ? ((2 * c) ^ g) * 16 : (c ^ ((g >> 1) & 3)) * 16);
     while (get.left > 0) {
       const int n = get.n, h = get.h, g0 = get.grp * 4 * SETS;
-      if (fresh) {                                   // a new unit: its query rows, normalised to [1, 2) and split in two fp16
+      if (fresh) {                                   // a new unit: its query rows, brought to fp16's range and split in two fp16
         fresh = false;
         whole = get.tile == 0;
 #pragma unroll
@@ -271,7 +271,8 @@ __global__ void __launch_bounds__(32, KvShape<D, SETS>::kBlocks) kv8_attention_k
           for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 126);
+          // the largest element lies in [2^14, 2^15) then, so fp16's smallest step is 2^-38 of it
+          const int e = max((int)(__float_as_uint(top) >> 23) - 127, -100) - 14;     // -114 .. 114
           const float down = pow2f(-e);
           f[t] = __shfl_sync(0xffffffffu, pow2f(e), c * 8) * a.scale * kLog2e;       // of head c: its column 2c is lane 8c's
 #pragma unroll

@@ -643,3 +643,25 @@ def test_attention_of_a_sink_and_a_flat_tail(kind, D, heads, sink_scale):
     tol = want * rel + L * 2.0 ** -40 * 2.0 ** (sink_scale - 6) * 14
     off = (got.double().cpu() - want).abs()
     assert bool((off <= tol).all()), ((off / want).amax((0, 2)), (off / tol).amax((0, 2)))
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("D,heads", [(64, 2), (128, 6)])
+@pytest.mark.parametrize("outlier", [2.0 ** 8, 2.0 ** 14, 2.0 ** 20, 2.0 ** 127])
+def test_attention_of_queries_with_an_outlier_channel(kind, D, heads, outlier):
+    """A channel of the query that is larger than the others by far, where the keys have nothing."""
+    q, codes, scales, table, lens = attend_case(41, kind, heads, 1, D, 16, [300, 33], torch.float32)
+    codes[0, ..., 3] = 0
+    if outlier == 2.0 ** 127:
+        q *= 2.0 ** 108                                                       # (the largest exponent; keys to match)
+        scales[0] *= 2.0 ** -108
+    q[..., 3] = 1.9 * outlier
+    got = ops.attention_decode_kv8(q, codes, scales, table, lens)
+    ref, bound = plain.attend(q, codes, scales, table.cpu(), lens.cpu(), D ** -0.5)
+    used = [table[n, j] for n in range(2) for j in range(-(-int(lens[n]) // 16))]
+    keys = (codes[0].float() * scales[0][..., None, None])[torch.stack(used).long()]
+    # a query's element is off by 2^-39 of the row's largest at most: so much for every key channel; both ways in the exponent
+    extra = float(keys.abs().sum(-1).max()) * 1.9 * outlier * 2.0 ** -39 * D ** -0.5
+    values = (codes[1].float() * scales[1][..., None, None]).abs().max()
+    tol = bound * (1 + 2.0 ** -24) + 2 * extra * float(values) + np.abs(ref) * 2.0 ** -24
+    assert (np.abs(got.cpu().double().numpy() - ref) <= tol).all(), float((np.abs(got.cpu().double().numpy() - ref) / tol).max())
