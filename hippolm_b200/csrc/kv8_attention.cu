@@ -24,6 +24,7 @@
 #include <cuda_bf16.h>
 #include "sm100.cuh"
 #include "host_utils.h"
+#include "ring.h"
 #include "kv8_common.cuh"
 
 namespace hippo {
@@ -438,8 +439,12 @@ __global__ void __launch_bounds__(32, KvShape<D, SETS>::kBlocks) kv8_attention_k
         first = false;
       }
     }
-    if (!alive) {                                    // a wait ran out: let the copies in flight land before the block ends
-      for (int i = 0; i < S::kStages; ++i) mbar_wait(&full[i], phase, kWaitTmaFull, -1);
+    if (!alive) {                                    // a wait ran out: the copies of the tiles from `get` to `put` land before the block ends
+      for (int i = 0; i < S::kStages && get.left != put.left; ++i) {
+        const RingPlace r = ring_place(stage, phase, i, S::kStages);
+        mbar_wait(&full[r.stage], r.parity, kWaitTmaFull, -1);
+        get.advance(a);
+      }
       found.x = -1;
     }
   }
