@@ -291,7 +291,8 @@ __global__ void __launch_bounds__(32, KvShape<D, SETS>::kBlocks) kv8_attention_k
           m[t] = mv[t] = -INFINITY; l[t] = 0.f;
         }
       }
-      if (!mbar_wait(&full[stage], phase, kWaitTmaFull, worker)) { alive = false; break; }
+      const bool landed = mbar_wait(&full[stage], phase, kWaitTmaFull, worker);
+      if (!__all_sync(0xffffffffu, landed)) { alive = false; break; }     // each lane has its own limit: the warp gives up together
       const uint8_t* kt = ring + stage * S::kStageBytes;
       const uint8_t* vt = kt + kTile * D;
       const int valid = min(kTile, get.len - get.tile * kTile);

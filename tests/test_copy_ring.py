@@ -44,3 +44,13 @@ def test_cache_attention_drains_the_places_of_its_copies():
     assert "get.left != put.left" in drain and "get.advance(a)" in drain
     assert re.search(r"ring_place\(stage, phase, \w+, S::kStages\)", drain)
     assert re.findall(r"mbar_wait\(&full\[([^\]]*)\], ([^,]*),", drain) == [("r.stage", "r.parity")]
+
+
+def test_cache_attention_gives_up_as_a_whole_warp():
+    """The lanes' waits run out one by one: the warp acts on their common result (its next shuffles name all lanes)."""
+    text = open(os.path.join(CSRC, "kv8_attention.cu")).read()
+    body = text[:text.index("if (!alive)")]
+    waits = [line.strip() for line in body.splitlines() if "mbar_wait(" in line]
+    assert waits and all(re.match(r"const bool (\w+) = mbar_wait\(.*\);", w) or "__all_sync(" in w for w in waits), waits
+    for name in re.findall(r"const bool (\w+) = mbar_wait\(", body):
+        assert re.search(rf"if \(!__all_sync\(0xffffffffu, {name}\)\)", body), name
