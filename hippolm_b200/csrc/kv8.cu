@@ -498,6 +498,8 @@ extern "C" int hippo_kv8_plan(const KvPlanCall* c) {
   kv8_plan_kernel<<<1, kPlanThreads, 0, st>>>(c->table, c->table_ld, c->M, c->lens, c->new_lens, c->N, c->free_list, c->cap,
                                               c->free_count, c->release, sh, c->num_tokens, c->slots, c->lens_out, c->count_out,
                                               c->served, c->cu, many ? 0 : 1);
+  const cudaError_t first = cudaGetLastError();
+  if (first != cudaSuccess) return (int)first;       // the ends of the tokens and the table are the first kernel's
   if (many)
     kv8_slots_kernel<<<(unsigned)((c->num_tokens + 1023) / 1024), 256, 0, st>>>(c->table, c->table_ld, c->lens_out, c->served,
                                                                                 c->cu, c->N, sh, c->num_tokens, c->slots);

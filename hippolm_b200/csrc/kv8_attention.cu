@@ -568,6 +568,8 @@ template <int D, int E4M3, int SETS> int launch_sets(const KvAttnArgs& a, const 
     if (dev >= 0 && dev < 16) set[dev] = true;
   }
   kv8_attention_kernel<D, E4M3, SETS><<<a.NW, 32, S::kSmem, st>>>(map, a);
+  const cudaError_t first = cudaGetLastError();
+  if (first != cudaSuccess) return (int)first;       // the joining kernel would follow descriptors that nobody wrote
   // the joining kernel is launched while the first one runs and waits for its end on the device
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.NW / kUnits));

@@ -276,3 +276,15 @@ def test_refusals():
         with pytest.raises(ValueError):
             f()
             pytest.fail(f"call {i} was not refused")
+
+
+def test_a_kernel_that_reads_anothers_workspace_runs_only_behind_it():
+    """Calls of two kernels, the second of which follows indexes that the first one leaves: not launched where the first was refused."""
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(ops.__file__))), "csrc")
+    for name, first, second in (("kv8_attention.cu", "kv8_attention_kernel<D, E4M3, SETS><<<", "cudaLaunchKernelEx("),
+                                ("kv8.cu", "kv8_plan_kernel<<<", "kv8_slots_kernel<<<")):
+        text = open(os.path.join(csrc, name)).read()
+        between = text[text.index(first):text.index(second, text.index(first))]
+        assert re.search(r"cudaGetLastError\(\)[^;]*;(?s:.*)\breturn\b", between), name
