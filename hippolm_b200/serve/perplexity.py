@@ -100,14 +100,15 @@ def score_documents(model, tokenizer, documents: Iterable[str], seq_len: int = 1
                     top_logprobs: int = 0, max_tokens: Optional[int] = None) -> Iterator[Dict[str, object]]:
     """Scores of every token, a row for each piece of at most ``seq_len`` tokens of a document (each piece on its own context, as
     in ``evaluate_perplexity``): ``{"document", "tokens", "logprobs", "entropy"}`` and, with ``top_logprobs``, ``"top_tokens"`` /
-    ``"top_logprobs"``. The first token of a piece has no score (null). Pieces run packed, some ``batch_tokens`` at a time."""
+    ``"top_logprobs"``. The first token of a piece has no score (null). Pieces run packed; a pass has less
+    than ``batch_tokens`` + ``seq_len`` tokens."""
     dev = next(model.parameters()).device
     eos = getattr(tokenizer, "eos_token_id", None)
     w = model.mesh.tp
     was_training = model.training
     model.eval()
     pending: List[Tuple[int, List[int]]] = []
-    seen = 0
+    seen = waiting = 0                                     # tokens scored or about to be, tokens in `pending`
 
     def flush() -> Iterator[Dict[str, object]]:
         nonlocal pending
@@ -139,8 +140,10 @@ def score_documents(model, tokenizer, documents: Iterable[str], seq_len: int = 1
                 if len(piece) >= 2:
                     pending.append((d, piece))
                     seen += len(piece) - 1
-            if sum(len(p) for _, p in pending) >= batch_tokens:
-                yield from flush()
+                    waiting += len(piece)
+                    if waiting >= batch_tokens:
+                        yield from flush()
+                        waiting = 0
             if max_tokens is not None and seen >= max_tokens:
                 break
         yield from flush()

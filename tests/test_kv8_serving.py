@@ -264,3 +264,30 @@ def test_tensor_parallel_ranks_decode_from_8_bit_caches(tmp_path):
     for s, lp in zip(scores, a["lp"]):
         assert torch.allclose(s.logprob, torch.tensor(lp), atol=1e-3)
     assert len(a["text"]) == 16 and a["text"][0] == a["text"][5] == 0.0
+
+
+def scorer(**kw):
+    cfg = HippoConfig(vocab_size=258, hidden_size=32, num_heads=2, head_dim=16, num_layers=2, num_blocks=1, intermediate_size=64,
+                      full_attn_interval=2, **kw)
+    return HippoModel(cfg, seed=1).eval()
+
+
+def passes_of(m, monkeypatch):
+    """The token counts of a model's scoring passes, as they happen."""
+    sizes, call = [], m.token_logprobs
+
+    def on_call(ids, **k):
+        sizes.append(ids.numel())
+        return call(ids, **k)
+    monkeypatch.setattr(m, "token_logprobs", on_call)
+    return sizes
+
+
+def test_scoring_a_long_document_runs_in_bounded_passes(monkeypatch):
+    from hippolm_b200.serve.perplexity import score_documents
+    m = scorer()
+    sizes = passes_of(m, monkeypatch)
+    doc = "".join(chr(97 + i % 26) for i in range(2999))
+    rows = list(score_documents(m, ByteTokenizer(), [doc, "short", doc[:700]], seq_len=64, batch_tokens=256))
+    assert max(sizes) < 256 + 64 and sum(sizes) == 3000 + 6 + 701
+    assert [t for r in rows if r["document"] == 0 for t in r["tokens"]] == list(doc.encode()) + [256]
