@@ -101,7 +101,7 @@ def score_documents(model, tokenizer, documents: Iterable[str], seq_len: int = 1
     """Scores of every token, a row for each piece of at most ``seq_len`` tokens of a document (each piece on its own context, as
     in ``evaluate_perplexity``): ``{"document", "tokens", "logprobs", "entropy"}`` and, with ``top_logprobs``, ``"top_tokens"`` /
     ``"top_logprobs"``. The first token of a piece has no score (null). Pieces run packed; a pass has less
-    than ``batch_tokens`` + ``seq_len`` tokens."""
+    than ``batch_tokens`` + ``seq_len`` tokens. ``max_tokens``: ends with the piece that brings so many scores."""
     dev = next(model.parameters()).device
     eos = getattr(tokenizer, "eos_token_id", None)
     w = model.mesh.tp
@@ -144,6 +144,8 @@ def score_documents(model, tokenizer, documents: Iterable[str], seq_len: int = 1
                     if waiting >= batch_tokens:
                         yield from flush()
                         waiting = 0
+                if max_tokens is not None and seen >= max_tokens:
+                    break
             if max_tokens is not None and seen >= max_tokens:
                 break
         yield from flush()

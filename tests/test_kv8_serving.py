@@ -291,3 +291,13 @@ def test_scoring_a_long_document_runs_in_bounded_passes(monkeypatch):
     rows = list(score_documents(m, ByteTokenizer(), [doc, "short", doc[:700]], seq_len=64, batch_tokens=256))
     assert max(sizes) < 256 + 64 and sum(sizes) == 3000 + 6 + 701
     assert [t for r in rows if r["document"] == 0 for t in r["tokens"]] == list(doc.encode()) + [256]
+
+
+def test_scoring_stops_inside_a_long_document(monkeypatch):
+    from hippolm_b200.serve.perplexity import score_documents
+    m = scorer()
+    sizes = passes_of(m, monkeypatch)
+    rows = list(score_documents(m, ByteTokenizer(), ["x" * 4000, "y" * 4000], seq_len=64, batch_tokens=256, max_tokens=300))
+    scored = sum(len(r["tokens"]) - 1 for r in rows)
+    assert 300 <= scored < 300 + 64 and sum(sizes) == sum(len(r["tokens"]) for r in rows)
+    assert all(r["document"] == 0 for r in rows)
