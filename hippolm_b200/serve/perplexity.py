@@ -42,6 +42,11 @@ def iter_documents(files: Iterable[str], text_field: str = "content") -> Iterato
                         yield doc
 
 
+def piece_length(cfg, seq_len: int) -> int:
+    """Tokens of a whole piece of a document: ``seq_len`` in whole chunks of the packer, one chunk at least."""
+    return max(cfg.pack_chunk_size, seq_len // cfg.pack_chunk_size * cfg.pack_chunk_size)
+
+
 @torch.no_grad()
 def evaluate_perplexity(model, tokenizer, documents: Iterable[str], seq_len: int = 1024, batch_rows: int = 4,
                         max_tokens: Optional[int] = None) -> Dict[str, float]:
@@ -51,7 +56,7 @@ def evaluate_perplexity(model, tokenizer, documents: Iterable[str], seq_len: int
     dev = next(model.parameters()).device
     eos = getattr(tokenizer, "eos_token_id", None)
     chunk = cfg.pack_chunk_size
-    seq_len = max(chunk, seq_len // chunk * chunk)
+    seq_len = piece_length(cfg, seq_len)
     was_training = model.training
     model.eval()
     total_nll, total_tok, n_docs = 0.0, 0, 0
@@ -98,12 +103,13 @@ def evaluate_perplexity(model, tokenizer, documents: Iterable[str], seq_len: int
 @torch.no_grad()
 def score_documents(model, tokenizer, documents: Iterable[str], seq_len: int = 1024, batch_tokens: int = 8192,
                     top_logprobs: int = 0, max_tokens: Optional[int] = None) -> Iterator[Dict[str, object]]:
-    """Scores of every token, a row for each piece of at most ``seq_len`` tokens of a document (each piece on its own context, as
-    in ``evaluate_perplexity``): ``{"document", "tokens", "logprobs", "entropy"}`` and, with ``top_logprobs``, ``"top_tokens"`` /
-    ``"top_logprobs"``. The first token of a piece has no score (null). Pieces run packed; a pass has less
-    than ``batch_tokens`` + ``seq_len`` tokens. ``max_tokens``: ends with the piece that brings so many scores."""
+    """Scores of every token, a row for each piece of a document (cut at the same places as in ``evaluate_perplexity``, each piece
+    on its own context): ``{"document", "tokens", "logprobs", "entropy"}`` and, with ``top_logprobs``, ``"top_tokens"`` /
+    ``"top_logprobs"``. The first token of a piece has no score (null). Pieces run packed; a pass holds fewer than
+    ``batch_tokens`` tokens and one piece. ``max_tokens``: ends with the piece that brings so many scores."""
     dev = next(model.parameters()).device
     eos = getattr(tokenizer, "eos_token_id", None)
+    seq_len = piece_length(model.cfg, seq_len)
     w = model.mesh.tp
     was_training = model.training
     model.eval()

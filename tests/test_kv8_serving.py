@@ -301,3 +301,14 @@ def test_scoring_stops_inside_a_long_document(monkeypatch):
     scored = sum(len(r["tokens"]) - 1 for r in rows)
     assert 300 <= scored < 300 + 64 and sum(sizes) == sum(len(r["tokens"]) for r in rows)
     assert all(r["document"] == 0 for r in rows)
+
+
+@pytest.mark.parametrize("seq_len", [100, 64, 10, 200])
+def test_token_scores_and_perplexity_cut_documents_alike(seq_len):
+    from hippolm_b200.serve.perplexity import evaluate_perplexity, score_documents
+    m, tok = scorer(), ByteTokenizer()
+    docs = ["".join(chr(97 + (i * i + k) % 26) for i in range(n)) for k, n in enumerate((333, 20, 64, 150))]
+    rows = list(score_documents(m, tok, docs, seq_len=seq_len, batch_tokens=150))
+    lp = [x for r in rows for x in r["logprobs"] if x is not None]
+    want = evaluate_perplexity(m, tok, docs, seq_len=seq_len)
+    assert len(lp) == want["tokens"] and -sum(lp) / len(lp) == pytest.approx(want["nll"], abs=1e-4)
