@@ -12,6 +12,7 @@ one request at a time with a full re-forward per token.
 from __future__ import annotations
 
 import json
+import os
 import queue
 import threading
 import time
@@ -162,16 +163,21 @@ class EvalService:
         return n
 
     def _logprobs_body(self, new, scores, n_top: int, chat: bool, text: str) -> dict:
-        """The ``logprobs`` object of a choice, for the tokens that begin within its text."""
+        """The ``logprobs`` object of a choice: its tokens up to the end-of-text token; where a stop string cut the text, those that
+        begin within it. A token that begins or goes on inside a character counts from that character's place."""
         eos = getattr(self.tok, "eos_token_id", None)
         say = lambda t: self.tok.decode([t], skip_special_tokens=False)                   # noqa: E731
         lp = scores.logprob.tolist()
         top_lp = scores.top_logprobs.tolist() if scores.top_logprobs is not None else [[]] * len(new)
         top_id = scores.top_ids.tolist() if scores.top_ids is not None else [[]] * len(new)
-        rows = []
+        full = self.tok.decode(new, skip_special_tokens=True)
+        cut = len(text) < len(full)
+        rows, offset = [], 0
         for i, t in enumerate(new):
-            offset = len(self.tok.decode(new[:i], skip_special_tokens=True))
-            if t == eos or (i > 0 and offset >= len(text)):
+            # (a prefix that ends inside a character decodes to replacement characters behind what it shares with the text)
+            before = self.tok.decode(new[:i], skip_special_tokens=True)
+            offset = max(offset, len(os.path.commonprefix([before, full])))
+            if t == eos or (cut and i > 0 and offset >= len(text)):
                 break
             rows.append((say(t), lp[i], [(say(j), x) for j, x in zip(top_id[i][:n_top], top_lp[i][:n_top])], offset))
         if chat:

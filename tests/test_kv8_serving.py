@@ -312,3 +312,33 @@ def test_token_scores_and_perplexity_cut_documents_alike(seq_len):
     lp = [x for r in rows for x in r["logprobs"] if x is not None]
     want = evaluate_perplexity(m, tok, docs, seq_len=seq_len)
     assert len(lp) == want["tokens"] and -sum(lp) / len(lp) == pytest.approx(want["nll"], abs=1e-4)
+
+
+def forced(svc, tokens, monkeypatch):
+    """A service whose next answers consist of ``tokens``; token i has log probability -i - 1, its alternatives are itself and 65."""
+    n = len(tokens)
+    scores = ops.TokenLogprobs(-1.0 - torch.arange(n, dtype=torch.float32), torch.zeros(n),
+                               torch.stack([-1.0 - torch.arange(n, dtype=torch.float32), torch.full((n,), -99.0)], 1),
+                               torch.tensor([[t, 65] for t in tokens], dtype=torch.int64).reshape(n, 2))
+    monkeypatch.setattr(svc, "_generate", lambda *a, **k: (list(tokens), "length") + ((scores,) if "logprobs" in k else ()))
+    return svc
+
+
+@pytest.mark.parametrize("text,offsets", [("ab€", [0, 1, 2, 2, 2]), ("日本", [0, 0, 0, 1, 1, 1]), ("é", [0, 0]), ("日a本b", [0, 0, 0, 1, 2, 2, 2, 3])])
+@pytest.mark.parametrize("ends", [False, True])
+def test_log_probabilities_of_characters_of_several_tokens(text, offsets, ends, monkeypatch):
+    """Every token of the answer has its log probability, also where a character's bytes are tokens of their own."""
+    tokens = list(text.encode()) + [256] * ends
+    svc = forced(small_service(), tokens, monkeypatch)
+    c = svc.complete({"prompt": "x", "logprobs": 2}, chat=False)["choices"][0]
+    n = len(text.encode())
+    assert c["text"] == text and c["logprobs"]["token_logprobs"] == [-1.0 - i for i in range(n)]
+    assert c["logprobs"]["text_offset"] == offsets and len(c["logprobs"]["tokens"]) == len(c["logprobs"]["top_logprobs"]) == n
+    chat = svc.complete({"messages": [{"role": "user", "content": "x"}], "logprobs": True, "top_logprobs": 1}, chat=True)["choices"][0]
+    assert [x["logprob"] for x in chat["logprobs"]["content"]] == [-1.0 - i for i in range(n)]
+    # a stop string ends the list with the tokens of the text before it
+    if text == "日a本b":
+        for stop, left in (("b", 7), ("本", 4), ("a", 3)):
+            c = svc.complete({"prompt": "x", "logprobs": 2, "stop": stop}, chat=False)["choices"][0]
+            assert len(c["logprobs"]["tokens"]) == left and c["finish_reason"] == "stop", stop
+    svc.close()
