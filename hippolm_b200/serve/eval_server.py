@@ -177,7 +177,7 @@ class EvalService:
             # (a prefix that ends inside a character decodes to replacement characters behind what it shares with the text)
             before = self.tok.decode(new[:i], skip_special_tokens=True)
             offset = max(offset, len(os.path.commonprefix([before, full])))
-            if t == eos or (cut and i > 0 and offset >= len(text)):
+            if t == eos or (cut and offset >= len(text)):
                 break
             rows.append((say(t), lp[i], [(say(j), x) for j, x in zip(top_id[i][:n_top], top_lp[i][:n_top])], offset))
         if chat:

@@ -342,3 +342,12 @@ def test_log_probabilities_of_characters_of_several_tokens(text, offsets, ends, 
             c = svc.complete({"prompt": "x", "logprobs": 2, "stop": stop}, chat=False)["choices"][0]
             assert len(c["logprobs"]["tokens"]) == left and c["finish_reason"] == "stop", stop
     svc.close()
+
+
+def test_no_log_probabilities_before_a_stop_string_at_the_start(monkeypatch):
+    svc = forced(small_service(), list("stop it".encode()), monkeypatch)
+    c = svc.complete({"prompt": "x", "logprobs": 2, "stop": ["it", "sto"]}, chat=False)["choices"][0]
+    assert c["text"] == "" and c["logprobs"]["tokens"] == c["logprobs"]["token_logprobs"] == c["logprobs"]["text_offset"] == []
+    chat = svc.complete({"messages": [], "logprobs": True, "stop": "s"}, chat=True)["choices"][0]
+    assert chat["message"]["content"] == "" and chat["logprobs"] == {"content": []}
+    svc.close()
