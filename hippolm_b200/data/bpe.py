@@ -153,6 +153,13 @@ class BPETokenizer:
         out.append(buf.decode("utf-8", errors="replace"))
         return "".join(out)
 
+    def token_bytes(self, token: int) -> Optional[bytes]:
+        """The bytes of one token (which may be a part of a character); None for ids outside the vocabulary."""
+        tok = self.id_to_token.get(int(token))
+        if tok is None:
+            return None
+        return tok.encode() if tok in self.special else bytes(_U2B[ch] for ch in tok if ch in _U2B)
+
     def apply_chat_template(self, messages, tokenize: bool = False, add_generation_prompt: bool = True):
         text = "".join(f"<|im_start|>{m['role']}\n{m['content']}<|im_end|>\n" for m in messages)
         if add_generation_prompt:

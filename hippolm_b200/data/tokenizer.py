@@ -24,6 +24,10 @@ class ByteTokenizer:
     def decode(self, ids, skip_special_tokens: bool = True) -> str:
         return bytes(i for i in ids if 0 <= int(i) < 256).decode("utf-8", errors="replace")
 
+    def token_bytes(self, token: int) -> Optional[bytes]:
+        """The bytes of one token; None for the special ones, which stand for no text."""
+        return bytes([token]) if 0 <= token < 256 else None
+
     def apply_chat_template(self, messages, tokenize: bool = False, add_generation_prompt: bool = True):
         text = "".join(f"<|im_start|>{m['role']}\n{m['content']}<|im_end|>\n" for m in messages)
         if add_generation_prompt:

@@ -18,7 +18,7 @@ import threading
 import time
 import uuid
 from http.server import BaseHTTPRequestHandler, ThreadingHTTPServer
-from typing import Optional
+from typing import List, Optional
 
 import torch
 
@@ -162,6 +162,15 @@ class EvalService:
             raise BadRequest(f"log probabilities of {n!r} alternatives: 0 .. {most}")
         return n
 
+    def _token_bytes(self, token: int) -> Optional[List[int]]:
+        """The bytes that a token stands for; None where the tokenizer does not tell them and its text may hide them."""
+        tell = getattr(self.tok, "token_bytes", None)
+        if tell is not None:
+            got = tell(token)
+            return None if got is None else list(got)
+        text = self.tok.decode([token], skip_special_tokens=False)
+        return None if "\ufffd" in text else list(text.encode())
+
     def _logprobs_body(self, new, scores, n_top: int, chat: bool, text: str) -> dict:
         """The ``logprobs`` object of a choice: its tokens up to the end-of-text token; where a stop string cut the text, those that
         begin within it. A token that begins or goes on inside a character counts from that character's place."""
@@ -179,17 +188,17 @@ class EvalService:
             offset = max(offset, len(os.path.commonprefix([before, full])))
             if t == eos or (cut and offset >= len(text)):
                 break
-            rows.append((say(t), lp[i], [(say(j), x) for j, x in zip(top_id[i][:n_top], top_lp[i][:n_top])], offset))
+            rows.append((t, lp[i], list(zip(top_id[i][:n_top], top_lp[i][:n_top])), offset))
         if chat:
-            item = lambda s, x: {"token": s, "logprob": x, "bytes": list(s.encode())}     # noqa: E731
-            return {"content": [dict(item(s, x), top_logprobs=[item(*a) for a in alts]) for s, x, alts, _ in rows]}
+            item = lambda t, x: {"token": say(t), "logprob": x, "bytes": self._token_bytes(t)}    # noqa: E731
+            return {"content": [dict(item(t, x), top_logprobs=[item(*a) for a in alts]) for t, x, alts, _ in rows]}
         tops = []
         for _, _, alts, _ in rows:
             d: dict = {}
-            for s, x in alts:                                          # tokens that print alike: the likeliest one counts
-                d.setdefault(s, x)
+            for t, x in alts:                                          # tokens that print alike: the likeliest one counts
+                d.setdefault(say(t), x)
             tops.append(d)
-        return {"tokens": [r[0] for r in rows], "token_logprobs": [r[1] for r in rows], "top_logprobs": tops if n_top else None,
+        return {"tokens": [say(r[0]) for r in rows], "token_logprobs": [r[1] for r in rows], "top_logprobs": tops if n_top else None,
                 "text_offset": [r[3] for r in rows]}
 
     def metrics_text(self) -> str:

@@ -351,3 +351,33 @@ def test_no_log_probabilities_before_a_stop_string_at_the_start(monkeypatch):
     chat = svc.complete({"messages": [], "logprobs": True, "stop": "s"}, chat=True)["choices"][0]
     assert chat["message"]["content"] == "" and chat["logprobs"] == {"content": []}
     svc.close()
+
+
+def test_bytes_of_chat_tokens_are_the_tokens_own(monkeypatch):
+    from hippolm_b200.data import bpe
+    svc = forced(small_service(), list("aé€".encode()), monkeypatch)
+    ask = {"messages": [{"role": "user", "content": "x"}], "logprobs": True, "top_logprobs": 2}
+    items = svc.complete(ask, chat=True)["choices"][0]["logprobs"]["content"]
+    assert [x["bytes"] for x in items] == [[b] for b in "aé€".encode()]
+    assert [[y["bytes"] for y in x["top_logprobs"]] for x in items] == [[[b], [65]] for b in "aé€".encode()]
+    svc.close()
+
+    tok = bpe.load_default()
+    svc = small_service()
+    svc.tok = tok
+    text = "some words, 日本 é"
+    forced(svc, tok.encode(text), monkeypatch)
+    items = svc.complete(ask, chat=True)["choices"][0]["logprobs"]["content"]
+    assert b"".join(bytes(x["bytes"]) for x in items).decode() == text
+    special = next(iter(tok.special.items()))
+    assert tok.token_bytes(special[1]) == special[0].encode() and ByteTokenizer().token_bytes(256) is None and tok.token_bytes(1 << 30) is None
+    svc.close()
+
+    class Other(ByteTokenizer):                                               # a tokenizer that does not tell its tokens' bytes
+        token_bytes = None
+    svc = small_service()
+    svc.tok = Other()
+    forced(svc, list("aé".encode()), monkeypatch)
+    items = svc.complete(ask, chat=True)["choices"][0]["logprobs"]["content"]
+    assert [x["bytes"] for x in items] == [[97], None, None]
+    svc.close()
