@@ -9,6 +9,19 @@ from typing import List, Optional, Sequence
 import torch
 
 from .. import ops
+from ..ops.kv8 import CODE_TYPES
+from ..ops.kv8_cuda import HEAD_DIMS
+
+
+def check_cache(dtype, head_dim: Optional[int], device) -> None:
+    """Refuses a cache type that there is none of, and a head size that the device's cache does not take. ``dtype`` None: no 8-bit
+    cache; ``head_dim`` None: no layer that keeps keys."""
+    if dtype is None:
+        return
+    if dtype not in CODE_TYPES and dtype not in CODE_TYPES.values():
+        raise ValueError(f"kv_cache {dtype}: int8 or e4m3")
+    if torch.device(device).type == "cuda" and head_dim is not None and head_dim not in HEAD_DIMS:
+        raise ValueError(f"kv_cache {dtype}: head_dim {head_dim}, the CUDA cache supports {' and '.join(map(str, HEAD_DIMS))}")
 
 
 class KV8Pages:

@@ -32,7 +32,7 @@ from ..parallel.collectives import gather_seq, reduce_scatter_seq, all_reduce_su
 from ..parallel.linear import column_linear_sp, row_linear_sp, nvfp4_column_linear_sp, nvfp4_row_linear_sp
 from ..parallel.mesh import get_mesh
 from ..ref.ops import positions_from_cu
-from .kv_pages import KV8Pages, layer_cache, pages_of
+from .kv_pages import KV8Pages, check_cache, layer_cache, pages_of
 from .nvfp4_linear import NVFP4Linear
 
 
@@ -781,6 +781,11 @@ class HippoModel(nn.Module):
             logits = logits.masked_fill(torch.zeros_like(drop).scatter(0, si, drop), float("-inf"))
         return torch.multinomial(logits.softmax(-1), 1)[0]
 
+    def check_kv_cache(self, kv_cache: Optional[str]) -> None:
+        """Raises ``ValueError`` where this model cannot decode from such a cache on its device."""
+        keeps = any(layer.kind != "kda" for layer in self.layers)
+        check_cache(kv_cache, self.cfg.head_dim if keeps else None, self.norm.weight.device)
+
     def new_decode_caches(self, capacity: int, n_seq: int = 1, kv_cache: Optional[str] = None,
                           limits: Optional[List[int]] = None) -> List[dict]:
         """Empty per-layer caches for ``n_seq`` sequences of at most ``capacity`` tokens each (keys / values of the
@@ -789,6 +794,7 @@ class HippoModel(nn.Module):
         every block of 64 tokens and head, in a pool of blocks for ``limits[n]`` tokens of sequence n (default: ``capacity``)."""
         cfg = self.cfg
         dev, dt = self.norm.weight.device, self.norm.weight.dtype
+        self.check_kv_cache(kv_cache)
         caches: List[dict] = []
         pages = KV8Pages(limits if limits is not None else [capacity] * n_seq, device=dev) if kv_cache is not None else None
         for layer in self.layers:
@@ -829,6 +835,7 @@ class HippoModel(nn.Module):
         m = self.mesh
         w = m.tp
         n_real = len(prompts)
+        self.check_kv_cache(kv_cache)
         if logprobs is not None and not 0 <= logprobs <= min(ops.MAX_TOP, self.cfg.vocab_size):
             raise ValueError(f"logprobs {logprobs}: 0 .. {min(ops.MAX_TOP, self.cfg.vocab_size)}")
         if n_real == 0:

@@ -14,6 +14,7 @@ DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _stream = torch._C._cuda_getCurrentRawStream            # the handle of a device's current stream
 _current = torch._C._cuda_getDevice                     # (the tensors of a call have initialised CUDA)
 ONE_BLOCK_TOKENS = 16384
+HEAD_DIMS = (64, 128)
 _FNS: dict = {}
 _SMS: dict = {}
 
@@ -62,7 +63,7 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 def write(k, v, slots, codes, scales, dev: int, ks, cs, window: int = 0):
     """``window``: tokens that a block looks through, 0 by size (tests give it)."""
     T, H, D = ks
-    if D != 128 and D != 64:
+    if D not in HEAD_DIMS:
         raise ValueError(f"head_dim {D}: the CUDA cache supports 64 and 128")
     k, v = _rows(k), _rows(v)
     (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
@@ -75,7 +76,7 @@ def write(k, v, slots, codes, scales, dev: int, ks, cs, window: int = 0):
 def attention_decode(q, codes, scales, table, lens, scale: float, dev: int, qs, cs, M: int):
     N, Hq, D = qs
     _, blocks, H, bs, _ = cs
-    if D != 128 and D != 64:
+    if D not in HEAD_DIMS:
         raise ValueError(f"head_dim {D}: the CUDA cache supports 64 and 128")
     if 2 * blocks * H * bs >= 1 << 31:
         raise ValueError("the cache has 2^31 rows or more")

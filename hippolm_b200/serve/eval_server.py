@@ -68,6 +68,8 @@ class BadRequest(ValueError):
 class EvalService:
     def __init__(self, model: HippoModel, tokenizer, model_name: str = "hippolm-b200", max_new_tokens: int = 256,
                  max_batch: int = 8, kv_cache: Optional[str] = None):
+        if kv_cache is not None:             # at the start, not with the first request
+            model.check_kv_cache(kv_cache)
         self.model, self.tok, self.name, self.max_new = model, tokenizer, model_name, max_new_tokens
         self.kv_cache = kv_cache             # None, "int8" or "e4m3": how the keys and values of a request are kept
         self.max_batch = max(1, int(max_batch))

@@ -381,3 +381,27 @@ def test_bytes_of_chat_tokens_are_the_tokens_own(monkeypatch):
     items = svc.complete(ask, chat=True)["choices"][0]["logprobs"]["content"]
     assert [x["bytes"] for x in items] == [[97], None, None]
     svc.close()
+
+
+def test_caches_that_cannot_be_kept_are_refused_at_once(monkeypatch):
+    """A cache type or head size that no pass could use is refused where the cache is asked for, not by the first pass."""
+    m = model()
+    for call in (lambda: m.generate_batch([], 3, kv_cache="int4"), lambda: m.generate_batch([torch.tensor([1])], 0, kv_cache="fp8"),
+                 lambda: m.new_decode_caches(8, 1, kv_cache="int4"), lambda: small_service(kv_cache="int4")):
+        with pytest.raises(ValueError, match="int8 or e4m3"):
+            call()
+    kv_pages.check_cache(None, 96, torch.device("cuda"))
+    kv_pages.check_cache("int8", 16, torch.device("cpu"))
+    for dim in (64, 128):
+        kv_pages.check_cache("e4m3", dim, torch.device("cuda"))
+    with pytest.raises(ValueError, match="head_dim 96"):
+        kv_pages.check_cache("int8", 96, torch.device("cuda"))
+    kv_pages.check_cache("int8", None, torch.device("cuda"))                  # nothing is kept
+    seen = []
+    monkeypatch.setattr("hippolm_b200.models.model.check_cache", lambda *a: seen.append(a))       # what the model asks, before anything else
+    m.new_decode_caches(8, 1, kv_cache="int8")
+    assert seen == [("int8", 16, m.norm.weight.device)]
+    # a model without full attention keeps no keys, and takes no unknown type either
+    monkeypatch.undo()
+    with pytest.raises(ValueError):
+        model(full_attn_interval=5).new_decode_caches(8, 1, kv_cache="int4")
