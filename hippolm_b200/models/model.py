@@ -941,7 +941,11 @@ class HippoModel(nn.Module):
         ``use_cache`` (default): incremental decoding (``generate_batch`` with one sequence): the prompt runs once, every
         further token is a one-token step on the carried KDA states and the cached keys / values, so a new token costs one
         pass over the weights instead of a pass over the whole sequence. ``use_cache=False`` re-runs the full forward for
-        every token as the reference does (``src/models/model.py:180-219``), with the prompt padded to a multiple of tp."""
+        every token as the reference does (``src/models/model.py:180-219``), with the prompt padded to a multiple of tp, and takes no
+        ``kv_cache`` (see ``generate_batch``)."""
+        self.check_kv_cache(kv_cache)
+        if kv_cache is not None and not use_cache:
+            raise ValueError(f"kv_cache {kv_cache} without a cache (use_cache=False)")
         ids = input_ids.reshape(-1).clone()
         w = self.mesh.tp
         if use_cache and max_new_tokens > 0 and ids.numel() > 0:

@@ -405,3 +405,14 @@ def test_caches_that_cannot_be_kept_are_refused_at_once(monkeypatch):
     monkeypatch.undo()
     with pytest.raises(ValueError):
         model(full_attn_interval=5).new_decode_caches(8, 1, kv_cache="int4")
+
+
+def test_generate_does_not_ignore_a_cache_type():
+    m = model()
+    ids = torch.tensor([1, 2, 3])
+    for kw in (dict(max_new_tokens=0, kv_cache="int4"), dict(max_new_tokens=2, kv_cache="int4", use_cache=False),
+               dict(max_new_tokens=2, kv_cache="int8", use_cache=False)):
+        with pytest.raises(ValueError):
+            m.generate(ids, **kw)
+    assert m.generate(ids, 0, kv_cache="int8").tolist() == [1, 2, 3]
+    assert m.generate(ids, 2, use_cache=False).numel() == m.generate(ids, 2, kv_cache="int8").numel() == 5
