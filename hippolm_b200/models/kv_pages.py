@@ -43,6 +43,8 @@ class KV8Pages:
     def plan(self, cu_seqlens: torch.Tensor, num_tokens: int) -> None:
         """Slots for the tokens of the next pass, ``cu_seqlens`` [sequences + 1] packed: the whole prompts first, then one token a
         sequence and pass. Sequences in ``release`` have their rows in the stream like the others."""
+        if self.passes and num_tokens != self.table.shape[0]:
+            raise ValueError("the cache takes whole prompts first, then one token per sequence and step")
         new = (cu_seqlens[1:] - cu_seqlens[:-1]).to(torch.int32)
         p = ops.kv8_plan(self.table, self.lens, new, self.free, self.free_count, self.block_size, num_tokens, release=self.release)
         self.slots, self.lens, self.free_count = p.slots, p.lens, p.free_count
@@ -54,8 +56,6 @@ class KV8Pages:
         ops.kv8_write(k, v.to(k.dtype), self.slots, codes, scales)
         if self.passes == 1:
             return None
-        if q.shape[0] != self.table.shape[0]:
-            raise ValueError("the cache takes whole prompts first, then one token per sequence and step")
         return ops.attention_decode_kv8(q, codes, scales, self.table, self.lens, scale)
 
 

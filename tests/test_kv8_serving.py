@@ -416,3 +416,29 @@ def test_generate_does_not_ignore_a_cache_type():
             m.generate(ids, **kw)
     assert m.generate(ids, 0, kv_cache="int8").tolist() == [1, 2, 3]
     assert m.generate(ids, 2, use_cache=False).numel() == m.generate(ids, 2, kv_cache="int8").numel() == 5
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_a_refused_pass_leaves_the_pages_as_they_were(kind):
+    m = model()
+    prompts = [torch.randint(0, 96, (n,)) for n in (5, 9)]
+    caches = m.new_decode_caches(40, 2, kv_cache=kind)
+    cu = torch.tensor([0, 5, 14], dtype=torch.int32)
+    cu1 = torch.arange(3, dtype=torch.int32)
+    with torch.no_grad():
+        _, st = m.hidden(torch.cat(prompts), cu_seqlens=cu, caches=caches)
+        pages = kv_pages.pages_of(caches)
+        layers = [c for c in caches if "pages" in c]
+
+        def held():
+            return [pages.lens.clone(), pages.free_count.clone(), pages.table.clone()] + [c[k].clone() for c in layers for k in ("codes", "scales")]
+        before = held()
+        with pytest.raises(ValueError):                                       # three tokens for two sequences
+            m.hidden(torch.tensor([1, 2, 3]), cu_seqlens=torch.tensor([0, 2, 3], dtype=torch.int32), kda_states=st, caches=caches)
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, held()))
+        other = m.new_decode_caches(40, 2, kv_cache=kind)
+        _, st2 = m.hidden(torch.cat(prompts), cu_seqlens=cu, caches=other)
+        pos, nxt = torch.tensor([5, 9]), torch.tensor([1, 2])
+        a, _ = m.hidden(nxt, cu_seqlens=cu1, kda_states=st, caches=caches, position_offset=pos)
+        b, _ = m.hidden(nxt, cu_seqlens=cu1, kda_states=st2, caches=other, position_offset=pos)
+        assert torch.equal(a, b)
