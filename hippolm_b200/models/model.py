@@ -913,21 +913,26 @@ class HippoModel(nn.Module):
         """How the model scores a text: for every token of the (packed) stream its log probability given the tokens before it in
         its document (0 for a document's first token), and the entropy and the ``top_k`` alternatives of the distribution that it
         was drawn from (of a first token: of the distribution behind the document's last one, which no token follows).
-        Logits exist for ``chunk_rows`` tokens at a time."""
+        Logits exist for ``chunk_rows`` tokens at a time. The documents of ``cu_seqlens`` cover the stream (``ValueError`` otherwise)."""
         ids = input_ids.reshape(-1)
         T = ids.numel()
-        if T == 0:
-            return ops.token_logprobs(torch.empty(0, self.cfg.vocab_size, device=ids.device), ids, top_k=top_k)
         if cu_seqlens is None:
             row = input_ids.shape[1] if input_ids.dim() == 2 else T
-            cu_seqlens = torch.arange(0, T + 1, max(row, 1), device=ids.device, dtype=torch.int32)
-        h, _ = self.hidden(ids, cu_seqlens=cu_seqlens)
-        cu = cu_seqlens.to(ids.device).long()
-        full = cu[1:] > cu[:-1]
+            ends = list(range(0, T + 1, max(row, 1)))
+        else:
+            ends = cu_seqlens.tolist()
+            if (cu_seqlens.dim() != 1 or cu_seqlens.is_floating_point() or ends[:1] != [0] or ends[-1] != T
+                    or any(e < s for s, e in zip(ends, ends[1:]))):
+                raise ValueError(f"cu_seqlens: whole numbers that ascend from 0 to the {T} tokens")
+            ends = sorted(set(ends))                                         # documents without tokens leave nothing
+        if T == 0:
+            return ops.token_logprobs(torch.empty(0, self.cfg.vocab_size, device=ids.device), ids, top_k=top_k)
+        cu = torch.tensor(ends, device=ids.device)
+        h, _ = self.hidden(ids, cu_seqlens=cu.int())
         prev = torch.arange(-1, T - 1, device=ids.device)                    # the row whose distribution scores token t
-        prev[cu[:-1][full]] = cu[1:][full] - 1
+        prev[cu[:-1]] = cu[1:] - 1
         targets = ids.clone()
-        targets[cu[:-1][full]] = -100
+        targets[cu[:-1]] = -100
         parts = [ops.token_logprobs(self.lm_head.logits(h, rows=prev[s:s + chunk_rows]), targets[s:s + chunk_rows], top_k=top_k)
                  for s in range(0, T, chunk_rows)]
         return ops.TokenLogprobs(*[torch.cat(x) if x[0] is not None else None for x in zip(*parts)])

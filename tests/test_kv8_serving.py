@@ -442,3 +442,19 @@ def test_a_refused_pass_leaves_the_pages_as_they_were(kind):
         a, _ = m.hidden(nxt, cu_seqlens=cu1, kda_states=st, caches=caches, position_offset=pos)
         b, _ = m.hidden(nxt, cu_seqlens=cu1, kda_states=st2, caches=other, position_offset=pos)
         assert torch.equal(a, b)
+
+
+def test_scores_of_documents_that_do_not_cover_the_text_are_refused():
+    m = model()
+    ids = torch.randint(0, 96, (20,))
+    for cu in ([0, 7, 12], [3, 20], [0, 7, 30], [0, 9, 7, 20], [0, -1, 20], [0], []):
+        with pytest.raises(ValueError, match="cu_seqlens"):
+            m.token_logprobs(ids, cu_seqlens=torch.tensor(cu, dtype=torch.int32))
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        m.token_logprobs(ids[:0], cu_seqlens=torch.tensor([0, 3], dtype=torch.int32))
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        m.token_logprobs(ids, cu_seqlens=torch.tensor([0, 20]).float())
+    full = m.token_logprobs(ids, cu_seqlens=torch.tensor([0, 7, 20], dtype=torch.int32))
+    empty = m.token_logprobs(ids, cu_seqlens=torch.tensor([0, 0, 7, 7, 20, 20]))               # documents without tokens, 64-bit ends
+    assert torch.allclose(full.logprob, empty.logprob, atol=1e-4)
+    assert m.token_logprobs(ids[:0], cu_seqlens=torch.tensor([0], dtype=torch.int32)).logprob.shape == (0,)
