@@ -914,6 +914,11 @@ class HippoModel(nn.Module):
         its document (0 for a document's first token), and the entropy and the ``top_k`` alternatives of the distribution that it
         was drawn from (of a first token: of the distribution behind the document's last one, which no token follows).
         Logits exist for ``chunk_rows`` tokens at a time. The documents of ``cu_seqlens`` cover the stream (``ValueError`` otherwise)."""
+        most = min(ops.MAX_TOP, self.cfg.vocab_size)
+        if not 0 <= top_k <= most:
+            raise ValueError(f"top_k {top_k}: 0 .. {most}")
+        if chunk_rows < 1:
+            raise ValueError(f"chunk_rows {chunk_rows}: 1 or more")
         ids = input_ids.reshape(-1)
         T = ids.numel()
         if cu_seqlens is None:

@@ -458,3 +458,15 @@ def test_scores_of_documents_that_do_not_cover_the_text_are_refused():
     empty = m.token_logprobs(ids, cu_seqlens=torch.tensor([0, 0, 7, 7, 20, 20]))               # documents without tokens, 64-bit ends
     assert torch.allclose(full.logprob, empty.logprob, atol=1e-4)
     assert m.token_logprobs(ids[:0], cu_seqlens=torch.tensor([0], dtype=torch.int32)).logprob.shape == (0,)
+
+
+def test_scores_of_a_text_are_refused_before_its_pass(monkeypatch):
+    from hippolm_b200.serve.perplexity import score_documents
+    m = scorer()
+    monkeypatch.setattr(m, "hidden", lambda *a, **k: pytest.fail("the pass ran"))
+    ids = torch.arange(8)
+    for kw in (dict(top_k=33), dict(top_k=-1), dict(chunk_rows=0), dict(chunk_rows=-4)):
+        with pytest.raises(ValueError):
+            m.token_logprobs(ids, **kw)
+    with pytest.raises(ValueError):
+        list(score_documents(m, ByteTokenizer(), ["some text"], top_logprobs=33))
