@@ -253,6 +253,7 @@ def run_perplexity(a) -> Dict:
     model = build_model_and_load(a.checkpoint, HippoConfig.from_namespace(args), dev, dtype)
     tok = load_tokenizer(a.tokenizer or args.tokenizer_path)
     if a.token_scores:
+        os.makedirs(os.path.dirname(os.path.abspath(a.token_scores)), exist_ok=True)
         with open(a.token_scores, "w") as f:
             for row in score_documents(model, tok, iter_documents(a.data_files.split(","), args.text_field), seq_len=a.seq_len,
                                        top_logprobs=a.top_logprobs, max_tokens=a.max_tokens):

@@ -470,3 +470,22 @@ def test_scores_of_a_text_are_refused_before_its_pass(monkeypatch):
             m.token_logprobs(ids, **kw)
     with pytest.raises(ValueError):
         list(score_documents(m, ByteTokenizer(), ["some text"], top_logprobs=33))
+
+
+def _eval_args(tmp_path, *more):
+    (tmp_path / "c.yml").write_text("vocab_size: 258\nhidden_size: 32\nnum_heads: 2\nhead_dim: 16\nnum_layers: 2\nnum_blocks: 1\n"
+                                    "intermediate_size: 64\nfull_attn_interval: 2\n")
+    (tmp_path / "d.txt").write_text("a first document\n\nand a second, longer one " + "with words " * 20)
+    return ["--config", str(tmp_path / "c.yml"), "--device", "cpu", "--data_files", str(tmp_path / "d.txt"),
+            "--work-dir", str(tmp_path / "w"), "--seq_len", "100", *more]
+
+
+def test_evaluation_script_writes_token_scores_where_no_folder_is_yet(tmp_path):
+    from hippolm_b200.serve import eval_driver
+    out = tmp_path / "w" / "scores" / "s.jsonl"
+    assert eval_driver.main(_eval_args(tmp_path, "--perplexity", "--token_scores", str(out), "--top_logprobs", "2")) == 0
+    rows = [json.loads(line) for line in out.read_text().splitlines()]
+    lp = [x for r in rows for x in r["logprobs"] if x is not None]
+    want = json.loads((tmp_path / "w" / "perplexity.json").read_text())
+    assert len(lp) == want["tokens"] and -sum(lp) / len(lp) == pytest.approx(want["nll"], abs=1e-4)
+    assert all(len(t) == 2 for r in rows for t in r["top_tokens"][1:])
