@@ -271,6 +271,14 @@ def run_perplexity(a) -> Dict:
 def main(argv=None) -> int:
     logging.basicConfig(level=logging.INFO, format="%(asctime)s [%(levelname)s] %(message)s")
     a = build_parser().parse_args(argv)
+    if a.token_scores and not a.perplexity:
+        raise SystemExit("--token_scores needs --perplexity")
+    if a.top_logprobs and not a.token_scores:
+        raise SystemExit("--top_logprobs needs --token_scores")
+    if a.top_logprobs:
+        from ..ops import MAX_TOP
+        if not 0 <= a.top_logprobs <= MAX_TOP:
+            raise SystemExit(f"--top_logprobs {a.top_logprobs}: 0 .. {MAX_TOP}")
     if a.perplexity:
         run_perplexity(a)
         return 0

@@ -489,3 +489,18 @@ def test_evaluation_script_writes_token_scores_where_no_folder_is_yet(tmp_path):
     want = json.loads((tmp_path / "w" / "perplexity.json").read_text())
     assert len(lp) == want["tokens"] and -sum(lp) / len(lp) == pytest.approx(want["nll"], abs=1e-4)
     assert all(len(t) == 2 for r in rows for t in r["top_tokens"][1:])
+
+
+def test_evaluation_script_refuses_scores_that_it_cannot_write(tmp_path, monkeypatch):
+    from hippolm_b200.serve import eval_driver
+    out = tmp_path / "s.jsonl"
+    out.write_text("kept")
+    monkeypatch.setattr("hippolm_b200.serve.eval_server.build_model_and_load", lambda *a: pytest.fail("the model was loaded"))
+    monkeypatch.setattr(eval_driver, "server_command", lambda *a: pytest.fail("a server was started"))
+    for more in (["--perplexity", "--token_scores", str(out), "--top_logprobs", "33"],
+                 ["--perplexity", "--token_scores", str(out), "--top_logprobs", "-1"],
+                 ["--perplexity", "--top_logprobs", "2"], ["--token_scores", str(out)]):
+        with pytest.raises(SystemExit) as e:
+            eval_driver.main(_eval_args(tmp_path, *more))
+        assert e.value.code not in (0, None), more
+    assert out.read_text() == "kept"
