@@ -26,29 +26,49 @@ def check_cache(dtype, head_dim: Optional[int], device) -> None:
 
 class KV8Pages:
     """Block table, lengths and free blocks of ``len(limits)`` sequences of at most ``limits[n]`` tokens each. The pool has exactly
-    the blocks that they can need, so every plan is served; a sequence in ``release`` gives its blocks back and stores nothing."""
+    the blocks that they can need, so every plan is served; a sequence in ``release`` gives its blocks back and stores nothing.
+    (The host keeps the lengths too, to refuse what goes beyond a limit: such a token would have no block.)"""
 
     def __init__(self, limits: Sequence[int], block_size: int = 64, device=None):
         need = [-(-max(x, 0) // block_size) for x in limits]
         i32 = dict(dtype=torch.int32, device=device)
-        self.block_size, self.blocks = block_size, max(1, sum(need))
+        self.limits, self.block_size, self.blocks = list(limits), block_size, max(1, sum(need))
         self.table = torch.full((len(need), max([1] + need)), -1, **i32)
         self.lens = torch.zeros(len(need), **i32)
         self.free = torch.arange(self.blocks - 1, -1, -1, **i32)
         self.free_count = torch.full((1,), self.blocks, **i32)
-        self.release: Optional[torch.Tensor] = None       # bool [sequences], read by the next plan
+        self.release = None
         self.slots: Optional[torch.Tensor] = None         # of the tokens of the pass that was planned last
         self.passes = 0
+        self._held = [0] * len(need)
+
+    @property
+    def release(self) -> Optional[torch.Tensor]:
+        """bool [sequences], read by the next plan"""
+        return self._release
+
+    @release.setter
+    def release(self, gone: Optional[torch.Tensor]) -> None:
+        self._release, self._gone = gone, [False] * len(self.limits) if gone is None else gone.tolist()
 
     def plan(self, cu_seqlens: torch.Tensor, num_tokens: int) -> None:
         """Slots for the tokens of the next pass, ``cu_seqlens`` [sequences + 1] packed: the whole prompts first, then one token a
         sequence and pass. Sequences in ``release`` have their rows in the stream like the others."""
         if self.passes and num_tokens != self.table.shape[0]:
             raise ValueError("the cache takes whole prompts first, then one token per sequence and step")
+        if cu_seqlens.numel() != len(self.limits) + 1:
+            raise ValueError(f"{cu_seqlens.numel() - 1} sequences, the cache has {len(self.limits)}")
+        ends = None if self.passes else cu_seqlens.tolist()
+        held = []
+        for n, (had, gone, limit) in enumerate(zip(self._held, self._gone, self.limits)):
+            held.append(0 if gone else had + (1 if self.passes else ends[n + 1] - ends[n]))
+            if held[n] > limit and not gone:
+                raise ValueError(f"sequence {n}: {held[n]} tokens, its limit is {limit}")
         new = (cu_seqlens[1:] - cu_seqlens[:-1]).to(torch.int32)
         p = ops.kv8_plan(self.table, self.lens, new, self.free, self.free_count, self.block_size, num_tokens, release=self.release)
         self.slots, self.lens, self.free_count = p.slots, p.lens, p.free_count
         self.passes += 1
+        self._held = held
 
     def attend(self, q, k, v, codes, scales, scale: float) -> Optional[torch.Tensor]:
         """Stores the pass's keys and values and, from the second pass on, returns the attention over each sequence's tokens (the

@@ -504,3 +504,30 @@ def test_evaluation_script_refuses_scores_that_it_cannot_write(tmp_path, monkeyp
             eval_driver.main(_eval_args(tmp_path, *more))
         assert e.value.code not in (0, None), more
     assert out.read_text() == "kept"
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_sequences_beyond_their_limit_are_refused(kind):
+    """The pool holds what the limits need: what goes beyond had no block, and was left out of the attention without a word."""
+    m = model()
+    cu1 = torch.arange(3, dtype=torch.int32)
+    cu = torch.tensor([0, 60, 66], dtype=torch.int32)
+    ids = torch.randint(0, 96, (66,))
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="sequence 1"):
+            m.hidden(ids, cu_seqlens=cu, caches=m.new_decode_caches(64, 2, kv_cache=kind, limits=[64, 5]))
+        with pytest.raises(ValueError, match="1 sequences"):
+            m.hidden(ids, cu_seqlens=cu[::2], caches=m.new_decode_caches(64, 2, kv_cache=kind))
+        caches = m.new_decode_caches(64, 2, kv_cache=kind, limits=[64, 64])
+        _, st = m.hidden(ids, cu_seqlens=cu, caches=caches)
+        pages = kv_pages.pages_of(caches)
+        for step in range(4):
+            pos = torch.tensor([60, 6]) + step
+            _, st = m.hidden(torch.tensor([1, 2]), cu_seqlens=cu1, kda_states=st, caches=caches, position_offset=pos)
+        before = pages.lens.clone(), pages.free_count.clone()
+        with pytest.raises(ValueError, match="sequence 0"):
+            m.hidden(torch.tensor([1, 2]), cu_seqlens=cu1, kda_states=st, caches=caches, position_offset=torch.tensor([64, 10]))
+        assert torch.equal(pages.lens, before[0]) and torch.equal(pages.free_count, before[1])
+        pages.release = torch.tensor([True, False])                           # the full one is done: the other goes on
+        m.hidden(torch.tensor([1, 2]), cu_seqlens=cu1, kda_states=st, caches=caches, position_offset=torch.tensor([64, 10]))
+        assert pages.lens.tolist() == [0, 11]
