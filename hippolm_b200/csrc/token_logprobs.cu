@@ -23,11 +23,12 @@
 #include <cuda_bf16.h>
 #include "sm100.cuh"
 #include "host_utils.h"
+#include "token_logprobs_launch.h"
 
 namespace cg = cooperative_groups;
 
 namespace hippo {
-constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;          // at most
+constexpr int kLpThreads = kLpWarps * 32;            // at most
 constexpr int kMaxGranules = 1024, kCand = 1024, kMaxTop = 32;
 constexpr float kL2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -573,16 +574,8 @@ template <typename T, int GR> int launch_granule(const LpArgs& a, cudaStream_t s
   const int sms = sm_count();
   int parts = 1;
   while (parts < 8 && a.rows * parts * 2 <= 3ll * sms && a.V >= parts * 2 * kLpWarps * 1024) parts *= 2;
-  // Warps of a block: as many as fill the card (32 a multiprocessor), and one for 10 segments or more (two for the alternatives),
-  // which amortise its start and the joining of its lanes; a power of two, as others leave a multiprocessor's registers unused.
-  // 4096 rows of 16000, 5 alternatives: 2 warps 39.8 us, 8 warps 51.3; of 32000 4 warps 60.6, 1 warp 73.5, 8 warps 70.1; of 64000 and
-  // 20 alternatives 4 warps 111, 6 warps 122, 8 warps 116; 8 rows of 4096 2.5 with 4 and more, 3.8 with 1.
   const int segs = max(1, a.V / parts / LpRow<T>::kSeg);
-  int least = 1;
-  while (least < kLpWarps && least * 2 <= (segs + 9) / 10) least *= 2;
-  if (a.top) least = max(least, 2);
-  const int fill = (int)(32ll * sms / (a.rows * parts));
-  const int threads = 32 * min(max(fill, least), min(segs, kLpWarps));
+  const int threads = 32 * logprob_warps(a.rows, parts, segs, sms, a.top > 0);
   if (parts == 1) {
     token_logprobs_kernel<T, GR><<<(unsigned)a.rows, threads, 0, st>>>(a);
     return (int)cudaGetLastError();
