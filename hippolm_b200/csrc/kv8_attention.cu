@@ -16,8 +16,9 @@
 // deliberate: with 1 to 8 live columns a 128-row tcgen05 tile would multiply zeros, and the kernel waits for memory.
 //
 // Measured, both kernels (device time in a row of calls, inputs above L2): 32 sequences of 6001 to 8192 tokens, 32 heads of 128, e4m3:
-// 300 us = 6.2 TB/s; 16 x 4096 tokens, 32 heads of 128: 93 us = 5.8 TB/s (int8 90); 2 x 131072, 4 heads of 128: 50.3 us = 5.3 TB/s;
-// 16 x 4096, 64 heads on 8 of 128: 38.1 us; 1 x 500, 16 heads: 9.0 us. Short calls wait for lens -> table -> first tiles (4 us) and for the join (3 us).
+// 300 us = 6.2 TB/s; 16 x 4096 tokens, 32 heads of 128: 94 us = 5.7 TB/s (int8 90); 2 x 131072, 4 heads of 128: 50.3 to 51.9 us = 5.2 TB/s;
+// 16 x 4096, 64 heads on 8 of 128: 38.6 us; 1 x 500, 16 heads: 9.0 us. Short calls wait for lens -> table -> first tiles (5 us) and for
+// the join (3.4 us, of long sequences 6.7).
 // In the reference a decoding step re-runs the whole forward (src/models/model.py:180-219).
 #include <type_traits>
 #include <cuda_fp16.h>

@@ -14,8 +14,9 @@
 // stay, with a warp of their own for the alternatives of the row before, were slower: 359 against 242 us for 4096 x 128256 and
 // k = 20, as that warp shares its multiprocessor's issue slots.)
 // The backward pass reads the logits once more and writes their gradient: HBM-bound.
-// Measured (device time, bf16): 4096 x 128256 without alternatives 158 us = 6.7 TB/s, with 5 178, with 20 186; 8 x 128256 with 5 7.0 us;
-// 3001 x 32000 fp32 forward and backward 193 us = 6.0 TB/s of 1.15 GB.
+// Measured (device time, bf16): 4096 x 128256 without alternatives 157 us = 6.7 TB/s, with 5 178, with 20 186 (after seconds of load,
+// under the power limit, 177, 179 to 204 and 191 to 196); 8 x 128256 with 5 7.0 us; 3001 x 32000 fp32 forward and backward 195 us =
+// 5.9 TB/s of 1.15 GB.
 // The reference computes losses only (fla/modules/fused_linear_cross_entropy.py:516-679); it has no per-token scores.
 #include <cooperative_groups.h>
 #include <type_traits>
